@@ -98,6 +98,29 @@ typedef struct wanb200_gemm_params {
 
 int wanb200_gemm_bf16(const wanb200_gemm_params* p, void* stream);
 
+/* ---------------------------------------------------------------- GEMM with low-rank adapters
+ * d = epilogue(a . w^T + scales[id] (a . down[id]^T) . up[id]^T), id = ids[row]: every row adds the
+ * low-rank update of its own adapter, or none where id < 0 -- the adapters of many requests in one
+ * batch, rows in any order (rows of one adapter next to each other cost least).  The update joins
+ * the accumulators before the epilogue (bias, GELU, gate, residual); all epilogues but SUMSQ and
+ * SCATTER.  The rank-wide intermediate is held in bf16, or for fp32 outputs in two bf16 planes
+ * (16 significant bits).  NaN or infinite weights of an adapter reach the rows that use it only.
+ * An id >= adapters counts as none and sets the device error word to 502.
+ * Limits: rank % 8 == 0, adapters * rank <= 4096, 16-byte aligned down and up, and the GEMM's. */
+typedef struct wanb200_lora_params {
+  wanb200_gemm_params gemm;
+  const void* down;      /* [adapters, rank, K] bf16 contiguous */
+  const void* up;        /* [N, adapters, rank] bf16 contiguous */
+  const float* scales;   /* [adapters], NULL = 1 */
+  const int32_t* ids;    /* [M] */
+  int adapters, rank;
+  void* lora_workspace; int64_t lora_workspace_bytes; /* 256-byte aligned, wanb200_lora_workspace_bytes() */
+} wanb200_lora_params;
+
+int wanb200_gemm_lora(const wanb200_lora_params* p, void* stream);
+/* Scratch of a call: M rows, adapters, rank, and whether the output is fp32; 0 for sizes out of range. */
+int64_t wanb200_lora_workspace_bytes(int64_t M, int adapters, int rank, int out_f32);
+
 /* ---------------------------------------------------------------- attention
  * o[b, i, h, :] = softmax_j(q[b,i,h,:] . k[b,j,h,:] * softmax_scale) v[b, j, h, :]
  * Exact (online-softmax) non-causal attention, head_dim 128, any q_len / kv_len >= 1.
@@ -219,6 +242,60 @@ typedef struct wanb200_qknorm_params {
 } wanb200_qknorm_params;
 
 int wanb200_qk_norm_rope(const wanb200_qknorm_params* p, void* stream);
+
+/* ---------------------------------------------------------------- per-head norm + rotation
+ * For each head (head_dim channels) of the sections of every row: y = x * rsqrt(mean(x^2) + eps) *
+ * gamma, then, with tables, the pairs (a, b) of the first rot channels become (a cos - b sin,
+ * a sin + b cos): pairs (2i, 2i+1) when interleaved, else (i, i + rot/2); the other channels stay
+ * unrotated.  The table row is positions[row] (0 <= p < table_rows), or row % table_rows without
+ * positions.  gamma[s] NULL: section s is rotated but not normed.  cos NULL: no rotation.  The
+ * sections are columns col0[s] .. col0[s] + heads[s] * head_dim of x and of out (head counts may
+ * differ: grouped key heads); out may be x (in place), else the two do not overlap; out's other
+ * columns are left alone.  A position outside the table sets the device error word to 501 and
+ * leaves its row as it was.  The per-head form of `_tp_rms_qk` + `_rope` (fast_dit.py:134-147,
+ * 163-169), which norm over the whole dim (wanb200_qk_norm_rope).
+ * Limits: head_dim 64, 128 or 256; rot % 16 == 0; ldx, ldo, col0 % 8 == 0; 16-byte aligned
+ * pointers (positions 4). */
+typedef struct wanb200_headnorm_params {
+  const void* x; int64_t ldx; void* out; int64_t ldo; int64_t rows;
+  int nsections; int64_t col0[2]; int heads[2]; const void* gamma[2]; /* [head_dim] bf16 */
+  int head_dim; float eps;
+  int rot, interleaved; const float* cos; const float* sin;           /* [table_rows, rot / 2] */
+  const int32_t* positions; int64_t table_rows;                       /* [rows] or NULL */
+} wanb200_headnorm_params;
+
+int wanb200_head_norm_rope(const wanb200_headnorm_params* p, void* stream);
+
+/* ---------------------------------------------------------------- attention over key ranges
+ * o[b,i,h,:] = sum_j w_j v[b,j,h/g,:] / sum_j w_j over the keys lo <= j < hi of row i (g = heads /
+ * kv_heads), w_j = exp(t_j), t_j = cap(scale * q . k_j) + bias:
+ *   lo, hi    [q_len] int32 per batch element (range_batch_stride elements apart, 0 = shared); the
+ *             range is clipped to 0 .. kv_len; a row with an empty range gives zeros.  Documents,
+ *             causal and frame-causal order, a prefix, a window and padding all are such ranges
+ *   softcap   cap(s) = softcap * tanh(s / softcap); 0 = none
+ *   slopes    bias = -slopes[h] * |j - pos|, [heads] fp32
+ *   dist_bias bias = dist_bias[h][clamp(j - pos, -reach, reach) + reach], [heads, 2 reach + 1] fp32
+ *             (a relative-position table; at most one of the two)
+ *   pos       [q_len] int32 like lo: the row's place among the keys (NULL = i)
+ * What keys outside a row's range hold (NaN, infinities) does not reach the row.  The masked,
+ * grouped, single-token companion of wanb200_attn_fwd.
+ * Limits: head_dim 64 or 128, heads % kv_heads == 0 with at most 128 heads a group, strides
+ * positive multiples of 8, 16-byte aligned tensors, kv_len and q_len < 2^30. */
+typedef struct wanb200_range_attn_params {
+  const void* q; int64_t q_tok_stride, q_batch_stride;
+  const void* k; int64_t k_tok_stride, k_batch_stride;
+  const void* v; int64_t v_tok_stride, v_batch_stride;
+  void* o; int64_t o_tok_stride, o_batch_stride;
+  int64_t batch, heads, kv_heads, q_len, kv_len, head_dim;
+  float softmax_scale, softcap;
+  const int32_t* lo; const int32_t* hi; const int32_t* pos; int64_t range_batch_stride;
+  const float* slopes; const float* dist_bias; int reach;
+  void* workspace; int64_t workspace_bytes; /* wanb200_range_attn_workspace_bytes(), 256-byte aligned */
+} wanb200_range_attn_params;
+
+int wanb200_range_attn_fwd(const wanb200_range_attn_params* p, void* stream);
+/* Scratch of a call with these params (only the sizes are read); 0 where none is needed. */
+int64_t wanb200_range_attn_workspace_bytes(const wanb200_range_attn_params* p);
 
 /* ---------------------------------------------------------------- partial-sum reduction
  * out[s * out_stride + row] = sum over k < parts of part[row * row_stride + part0[s] + k], for
@@ -385,7 +462,8 @@ int wanb200_device_error_async(int* host_out, void* stream);
 /* Library version, e.g. 201 for 0.2.1. */
 int wanb200_version(void);
 /* sizeof of the parameter structs (gemm, attn, ln, qknorm, residual, shard_gather, attn_fp8, block,
- * patchify, unpatchify, sumsq_reduce)
+ * patchify, unpatchify, sumsq_reduce, headnorm, range_attn,
+ * lora)
  * written to out[0..n); returns the number of structs.  Lets a binding detect a library built
  * from a different header. */
 int wanb200_struct_sizes(int64_t* out, int n);

@@ -130,6 +130,14 @@ int wanb200_gemm_bf16(const wanb200_gemm_params* p, void* stream) {
   return gemm_bf16(p, reinterpret_cast<cudaStream_t>(stream));
 }
 
+int wanb200_gemm_lora(const wanb200_lora_params* p, void* stream) {
+  return gemm_lora(p, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int64_t wanb200_lora_workspace_bytes(int64_t M, int adapters, int rank, int out_f32) {
+  return lora_workspace_bytes(M, adapters, rank, out_f32);
+}
+
 int wanb200_attn_fwd(const wanb200_attn_params* p, void* stream) {
   return attn_fwd(p, reinterpret_cast<cudaStream_t>(stream));
 }
@@ -161,6 +169,16 @@ int wanb200_layernorm(const wanb200_ln_params* p, void* stream) {
 int wanb200_qk_norm_rope(const wanb200_qknorm_params* p, void* stream) {
   return qk_norm_rope(p, reinterpret_cast<cudaStream_t>(stream));
 }
+
+int wanb200_head_norm_rope(const wanb200_headnorm_params* p, void* stream) {
+  return head_norm_rope(p, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int wanb200_range_attn_fwd(const wanb200_range_attn_params* p, void* stream) {
+  return range_attn_fwd(p, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int64_t wanb200_range_attn_workspace_bytes(const wanb200_range_attn_params* p) { return range_attn_workspace_bytes(p); }
 
 int wanb200_sumsq_reduce(const wanb200_sumsq_reduce_params* p, void* stream) {
   return sumsq_reduce(p, reinterpret_cast<cudaStream_t>(stream));
@@ -224,14 +242,15 @@ int wanb200_device_error_async(int* host_out, void* stream) {
 int wanb200_version(void) { return 201; }
 
 int wanb200_struct_sizes(int64_t* out, int n) {
-  const int64_t sizes[11] = {(int64_t)sizeof(wanb200_gemm_params), (int64_t)sizeof(wanb200_attn_params),
+  const int64_t sizes[14] = {(int64_t)sizeof(wanb200_gemm_params), (int64_t)sizeof(wanb200_attn_params),
                              (int64_t)sizeof(wanb200_ln_params), (int64_t)sizeof(wanb200_qknorm_params),
                              (int64_t)sizeof(wanb200_residual_params), (int64_t)sizeof(wanb200_shard_gather_params),
                              (int64_t)sizeof(wanb200_attn_fp8_params), (int64_t)sizeof(wanb200_block_params),
                              (int64_t)sizeof(wanb200_patchify_params), (int64_t)sizeof(wanb200_unpatchify_params),
-                             (int64_t)sizeof(wanb200_sumsq_reduce_params)};
-  for (int i = 0; i < n && i < 11; ++i) out[i] = sizes[i];
-  return 11;
+                             (int64_t)sizeof(wanb200_sumsq_reduce_params), (int64_t)sizeof(wanb200_headnorm_params),
+                             (int64_t)sizeof(wanb200_range_attn_params), (int64_t)sizeof(wanb200_lora_params)};
+  for (int i = 0; i < n && i < 14; ++i) out[i] = sizes[i];
+  return 14;
 }
 
 }  // extern "C"

@@ -26,6 +26,8 @@ enum DevError : int {
   kErrTimeoutAttnSoftmax = 203,
   kErrTimeoutDrain = 301,
   kErrTimeoutPeerBarrier = 401,
+  kErrBadPosition = 501,  // a rotation position outside the table
+  kErrBadAdapter = 502,   // an adapter id past the last adapter
 };
 
 // 2 s: far above any legitimate wait (a whole 30-layer step is ~0.2 s).
@@ -322,6 +324,11 @@ __device__ __forceinline__ void unpack_bf16x8(const uint4& u, float* f) {
     f[2 * i] = t.x;
     f[2 * i + 1] = t.y;
   }
+}
+
+// Non-zero when one of the two packed bf16 values is a NaN or an infinity (all exponent bits set).
+__device__ __forceinline__ int nonfinite_bf16x2(uint32_t u) {
+  return (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
 }
 
 // Hardware tanh (one MUFU op; PTX tanh.approx.f32, max relative error 2^-11, far below the bf16

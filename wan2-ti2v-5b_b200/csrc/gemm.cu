@@ -22,6 +22,7 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "lora.h"
 
 namespace wanb200 {
 
@@ -51,6 +52,7 @@ struct GemmCfg {
 // per instruction) instead of one row per lane (32 rows touched by every 16-byte access).  The
 // host uses it on 256-wide tiles, where it costs the TMA ring no stage.
 constexpr int G_RES_STAGING = G_EPI_WARPS * 32 * 32 * 4;  // 32 KB
+constexpr int G_LORA_SMEM = 64;  // the adapter kernels' static shared memory (the bad-step words)
 
 struct GemmArgs {
   void* d;  // bf16, or fp32 when out_f32
@@ -230,6 +232,33 @@ __device__ __forceinline__ void gemm_epilogue_chunk(const GemmArgs& a, float* v,
 __device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 
+// The steps of chunk c (4 bits) that the tile's MMA runs: used by one of its rows and finite.
+__device__ __forceinline__ uint32_t lora_chunk_steps(const uint32_t* mask, const uint32_t* bad, int c) {
+  return ((__ldg(mask + (c >> 3)) & ~bad[c >> 3]) >> ((c & 7) * 4)) & 0xfu;
+}
+
+// What the steps left out of the MMA (their up-projection holds a NaN or an infinity) add to the
+// output of `row` at `col`: the row's own adapter only.  Never taken with finite weights; one
+// value a call, so that the accumulator chunk stays in registers.
+__device__ __noinline__ float lora_slow_value(const LoraPlan* lo, const uint32_t* bad, int row, int col) {
+  const int id = __ldg(lo->ids + row);
+  if (id < 0 || id >= lo->adapters) return 0.f;
+  float v = 0.f;
+  for (int c = id * lo->rank; c < (id + 1) * lo->rank; ++c) {
+    if (!((bad[c >> 9] >> ((c >> 4) & 31)) & 1u)) continue;
+    float h = 0.f;
+    for (int pl = 0; pl < lo->planes; ++pl) h += __bfloat162float(lo->h[(pl * lo->rows_pad + row) * lo->cols + c]);
+    v = fmaf(h, __bfloat162float(lo->up[(int64_t)col * lo->adapters * lo->rank + c]), v);
+  }
+  return v;
+}
+
+__device__ __forceinline__ void lora_add_slow(const LoraPlan* lo, const uint32_t* bad, float* v, int row, int col0, int M) {
+  if (row >= M) return;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] += lora_slow_value(lo, bad, row, col0 + i);
+}
+
 // The fp32 residual epilogue of one tile for the epilogue warp on lane quarter `quad` that takes
 // the 32-column chunks half, half + 2, ...  Each 32 x 32 accumulator chunk (lane = row after the
 // tcgen05.ld) goes to the warp's 4 KB staging buffer and comes back with lane = (sub, cg): rows
@@ -238,9 +267,10 @@ __device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u 
 // swizzled by the row's low three bits: the row-per-lane writes and the row-segment reads are
 // both free of bank conflicts.  The arithmetic per element is gemm_epilogue_chunk's (bias add,
 // then r + v * g for GATE_RES, v + r for RES), so both paths give the same bits.
-template <int EPI>
-__device__ __forceinline__ void residual_tile_staged(const GemmArgs& a, float* stg, uint32_t t_row, int m0, int n0,
-                                                     int quad, int half, int lane) {
+template <int EPI, bool LORA>
+__device__ __forceinline__ void residual_tile_staged(const GemmArgs& a, const LoraPlan* lora, const uint32_t* slow,
+                                                     float* stg, uint32_t t_row, int m0, int n0, int quad, int half,
+                                                     int lane) {
   const int sub = lane >> 3, cg = lane & 7;
   const int rbase = m0 + quad * 32 + sub;  // the row of i = 0; a lane's rows step by 4
   int fr[8];
@@ -272,6 +302,9 @@ __device__ __forceinline__ void residual_tile_staged(const GemmArgs& a, float* s
     const bool more = c + 2 < nchunks && col0 + 64 < a.N;
     float v[32];
     tmem_ld32(t_row + c * 32, v);
+    if constexpr (LORA) {
+      if (slow) lora_add_slow(lora, slow, v, m0 + quad * 32 + lane, col0, a.M);
+    }
 #pragma unroll
     for (int q = 0; q < 8; ++q)
       *reinterpret_cast<float4*>(stg + lane * 32 + ((q ^ (lane & 7)) << 2)) =
@@ -314,10 +347,11 @@ __device__ __forceinline__ void residual_tile_staged(const GemmArgs& a, float* s
   }
 }
 
-template <int EPI>
-__global__ void __launch_bounds__(G_THREADS, 1)
-    gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                     const GemmArgs args) {
+// The kernel's body.  LORA: a tile's K loop goes on with the adapter steps that its rows use (h
+// through tmH, the up-projection columns through tmU), 64 columns per ring stage.
+template <int EPI, bool LORA>
+__device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap* tmH,
+                                          const CUtensorMap* tmU, const GemmArgs& args, const LoraPlan* lora) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
@@ -356,6 +390,19 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     tmem_alloc(smem_u32(tmem_slot), G_TMEM_COLS);
     tmem_relinquish();
   }
+  __shared__ uint32_t lora_bad[LORA ? LORA_MASK_WORDS : 1];  // steps left to the epilogue
+  if constexpr (LORA) {
+    if (warp == 2) {
+      for (int i = 0; i < LORA_MASK_WORDS; ++i) {
+        const int step = 32 * i + lane;
+        int bad = 0;
+        if (step < lora->steps)
+          for (int s = 0; s < LORA_SCAN; ++s) bad |= __ldg(lora->bad + step * LORA_SCAN + s);
+        const uint32_t word = __ballot_sync(0xffffffffu, bad != 0);
+        if (lane == 0) lora_bad[i] = word;
+      }
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -389,6 +436,28 @@ __global__ void __launch_bounds__(G_THREADS, 1)
           if (++stage == GSTAGES) {
             stage = 0;
             phase ^= 1;
+          }
+        }
+        if constexpr (LORA) {
+          const uint32_t* mask = lora->step_mask + m0 / GBM * LORA_MASK_WORDS;
+          for (int c = 0; ok && c < lora->cols / LORA_CHUNK; ++c) {
+            if (!lora_chunk_steps(mask, lora_bad, c)) continue;
+            for (int pl = 0; pl < lora->planes; ++pl) {
+              if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, abort_flag, err, kErrTimeoutGemmProducer)) {
+                ok = false;
+                break;
+              }
+              const uint32_t a_dst = tiles + stage * SB;
+              mbar_expect_tx(full0 + 8 * stage, G_A_BYTES + bn * GBK * 2);
+              tma_load_2d(a_dst, tmH, full0 + 8 * stage, c * LORA_CHUNK, (int)(pl * lora->rows_pad) + m0);
+              tma_load_2d(a_dst + G_A_BYTES, tmU, full0 + 8 * stage, c * LORA_CHUNK, n0);
+              issued |= 1u << stage;
+              last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
+              if (++stage == GSTAGES) {
+                stage = 0;
+                phase ^= 1;
+              }
+            }
           }
         }
       }
@@ -426,6 +495,34 @@ __global__ void __launch_bounds__(G_THREADS, 1)
             phase ^= 1;
           }
         }
+        if constexpr (LORA) {
+          int m0, n0;
+          tile_origin(tile, num_m, num_n, bn, m0, n0);
+          const uint32_t* mask = lora->step_mask + m0 / GBM * LORA_MASK_WORDS;
+          for (int c = 0; ok && c < lora->cols / LORA_CHUNK; ++c) {
+            const uint32_t steps = lora_chunk_steps(mask, lora_bad, c);
+            if (!steps) continue;
+            for (int pl = 0; pl < lora->planes; ++pl) {
+              if (!mbar_wait(full0 + 8 * stage, phase, abort_flag, err, kErrTimeoutGemmMma)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              const uint32_t a_addr = tiles + stage * SB;
+              const uint32_t b_addr = a_addr + G_A_BYTES;
+#pragma unroll
+              for (int kk = 0; kk < LORA_CHUNK / LORA_STEP; ++kk)
+                if ((steps >> kk) & 1u)
+                  umma_bf16(d_tmem, sw128_desc(a_addr + kk * 32, 16, 1024), sw128_desc(b_addr + kk * 32, 16, 1024), idesc,
+                            true);
+              umma_commit(empty0 + 8 * stage);
+              if (++stage == GSTAGES) {
+                stage = 0;
+                phase ^= 1;
+              }
+            }
+          }
+        }
         if (!ok) break;
         umma_commit(tfull0 + 8 * acc);
         acc ^= 1;
@@ -448,6 +545,13 @@ __global__ void __launch_bounds__(G_THREADS, 1)
       tile_origin(tile, num_m, num_n, bn, m0, n0);
       const int row = m0 + r;
       const uint32_t t_row = tmem_base + (uint32_t(quad * 32) << 16) + acc * GBN;
+      const uint32_t* slow = nullptr;  // the bad steps, where a row of this tile uses one of them
+      if constexpr (LORA) {
+        const uint32_t* mask = lora->step_mask + m0 / GBM * LORA_MASK_WORDS;
+        uint32_t any = 0;
+        for (int i = 0; i < LORA_MASK_WORDS; ++i) any |= __ldg(mask + i) & lora_bad[i];
+        if (any) slow = lora_bad;
+      }
       if constexpr (EPI == WANB200_EPI_SCATTER) {
         // stage this warp's 32 rows (lane = row), then write each row as one 512-byte segment
         // (the first warp of each lane quarter does the whole tile; the second only arrives)
@@ -476,7 +580,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
       } else if (epi_has_residual(EPI) && args.res_staging) {
         if constexpr (epi_has_residual(EPI)) {
           float* stg = reinterpret_cast<float*>(smem + args.tiles_bytes + GemmCfg<EPI>::STAGING) + (warp - 2) * 1024;
-          residual_tile_staged<EPI>(args, stg, t_row, m0, n0, quad, half, lane);
+          residual_tile_staged<EPI, LORA>(args, lora, slow, stg, t_row, m0, n0, quad, half, lane);
         }
       } else {
         uint4 res_next[8] = {}, res_cur[8];
@@ -500,6 +604,9 @@ __global__ void __launch_bounds__(G_THREADS, 1)
           }
           float v[32];
           tmem_ld32(t_row + c * 32, v);
+          if constexpr (LORA) {
+            if (slow) lora_add_slow(lora, slow, v, row, col0, args.M);
+          }
           gemm_epilogue_chunk<EPI>(args, v, row, col0, res_cur, gate_row);
         }
       }
@@ -516,7 +623,42 @@ __global__ void __launch_bounds__(G_THREADS, 1)
   if (warp == 1) tmem_dealloc(tmem_base, G_TMEM_COLS);
 }
 
+template <int EPI>
+__global__ void __launch_bounds__(G_THREADS, 1)
+    gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                     const GemmArgs args) {
+  gemm_body<EPI, false>(tmA, tmB, nullptr, nullptr, args, nullptr);
+}
+
+template <int EPI>
+__global__ void __launch_bounds__(G_THREADS, 1)
+    gemm_lora_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                     const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmU,
+                     const GemmArgs args, const __grid_constant__ LoraPlan lora) {
+  gemm_body<EPI, true>(tmA, tmB, &tmH, &tmU, args, &lora);
+}
+
 // ------------------------------------------------------------------ host launcher
+template <int EPI>
+static int launch_gemm_lora(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& th, const CUtensorMap& tu,
+                            const GemmArgs& ga, const LoraPlan& lora, int grid, cudaStream_t st) {
+  static std::atomic<bool> attr_set[kMaxDevices] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= kMaxDevices) return set_error(WANB200_EINVAL, "device index out of range");
+  if (!attr_set[dev].load(std::memory_order_acquire)) {
+    cudaError_t e = cudaFuncSetAttribute(gemm_lora_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         G_SMEM_LIMIT - G_LORA_SMEM);
+    if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute(gemm_lora)", e);
+    attr_set[dev].store(true, std::memory_order_release);
+  }
+  const int smem = (int)ga.tiles_bytes + GemmCfg<EPI>::FIXED + ga.res_staging;
+  gemm_lora_kernel<EPI><<<grid, G_THREADS, smem, st>>>(ta, tb, th, tu, ga, lora);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return set_cuda_error("gemm_lora_kernel launch", e);
+  return WANB200_OK;
+}
+
 template <int EPI>
 static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const GemmArgs& ga, int grid, cudaStream_t st) {
   // the shared-memory opt-in, once per device (setting it twice from racing threads is harmless)
@@ -541,11 +683,11 @@ static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const GemmA
 // smallest makespan waves * (BN + c), waves = ceil(tiles / SMs) over the persistent grid.  c
 // stands for the per-tile cost that does not shrink with BN (the A tile loads, the accumulator
 // hand-off); it keeps BN at 256 unless a narrower tile removes a mostly empty last wave.
-static int choose_tile_n(int64_t M, int64_t N, int sms) {
+static int choose_tile_n(int64_t M, int64_t N, int sms, int narrowest) {
   const int64_t num_m = (M + GBM - 1) / GBM;
   int best = GBN;
   double best_t = 1e300;
-  for (int bn = GBN; bn >= 128; bn -= 32) {
+  for (int bn = GBN; bn >= narrowest; bn -= 32) {
     const int64_t tiles = num_m * ((N + bn - 1) / bn);
     const double t = (double)((tiles + sms - 1) / sms) * (bn + 64.0);
     if (t < best_t - 1e-9) {
@@ -556,7 +698,7 @@ static int choose_tile_n(int64_t M, int64_t N, int sms) {
   return best;
 }
 
-int gemm_bf16(const wanb200_gemm_params* p, cudaStream_t st) {
+int gemm_validate(const wanb200_gemm_params* p) {
   if (!p) return set_error(WANB200_EINVAL, "gemm: null params");
   const int epi = p->epilogue;
   if (epi < WANB200_EPI_NONE || epi > WANB200_EPI_BIAS_SILU) return set_error(WANB200_EINVAL, "gemm: bad epilogue");
@@ -602,11 +744,22 @@ int gemm_bf16(const wanb200_gemm_params* p, cudaStream_t st) {
     if (!p->rowss || p->ss_cols <= 0 || (p->ss_cols % 32) || p->ss_cols > p->N)
       return set_error(WANB200_EINVAL, "gemm: sumsq epilogue needs rowss and ss_cols, a multiple of 32 in 32..N");
   }
+  return WANB200_OK;
+}
 
+int gemm_bf16(const wanb200_gemm_params* p, cudaStream_t st) {
+  const int rc = gemm_validate(p);
+  if (rc) return rc;
   int* err = device_error_word();
   if (!err) return WANB200_ECUDA;
+  return gemm_launch(p, nullptr, err, st);
+}
+
+int gemm_launch(const wanb200_gemm_params* p, const LoraPlan* lora, int* err, cudaStream_t st) {
+  const int epi = p->epilogue;
+  const bool scatter = epi == WANB200_EPI_SCATTER;
   const int sms = num_sms();
-  const int bn = p->tile_n ? p->tile_n : choose_tile_n(p->M, p->N, sms);
+  const int bn = p->tile_n ? p->tile_n : choose_tile_n(p->M, p->N, sms, lora ? 64 : 128);
   CUtensorMap ta, tb;
   int rc = make_tmap_2d(&ta, p->a, p->K, p->M, p->lda, GBK, GBM);
   if (rc) return rc;
@@ -641,7 +794,8 @@ int gemm_bf16(const wanb200_gemm_params* p, cudaStream_t st) {
   ga.bn = bn;
   ga.stage_bytes = (uint32_t)(G_A_BYTES + bn * GBK * 2);
   {
-    const int fixed = scatter ? GemmCfg<WANB200_EPI_SCATTER>::FIXED : GemmCfg<WANB200_EPI_NONE>::FIXED;
+    const int fixed = (scatter ? GemmCfg<WANB200_EPI_SCATTER>::FIXED : GemmCfg<WANB200_EPI_NONE>::FIXED) +
+                      (lora ? G_LORA_SMEM : 0);
     ga.stages = std::min<int>(G_MAX_STAGES, (G_SMEM_LIMIT - fixed) / (int)ga.stage_bytes);
     // the row-segment fp32 residual epilogue on full-width tiles, where its staging leaves the
     // ring depth as it is (measured at 15708 x 3072 x 3072: +6% GATE_RES, +10% RES; on 128-wide
@@ -657,6 +811,23 @@ int gemm_bf16(const wanb200_gemm_params* p, cudaStream_t st) {
 
   const int64_t tiles = ((p->M + GBM - 1) / GBM) * ((p->N + bn - 1) / bn);
   const int grid = (int)std::min<int64_t>(tiles, sms);
+  if (lora) {
+    CUtensorMap th, tu;
+    rc = make_tmap_2d(&th, lora->h, lora->cols, lora->planes * lora->rows_pad, lora->cols, GBK, GBM);
+    if (rc) return rc;
+    const int64_t up_cols = (int64_t)lora->adapters * lora->rank;
+    rc = make_tmap_2d(&tu, lora->up, up_cols, p->N, up_cols, GBK, bn);
+    if (rc) return rc;
+    switch (epi) {
+      case WANB200_EPI_NONE: return launch_gemm_lora<WANB200_EPI_NONE>(ta, tb, th, tu, ga, *lora, grid, st);
+      case WANB200_EPI_BIAS: return launch_gemm_lora<WANB200_EPI_BIAS>(ta, tb, th, tu, ga, *lora, grid, st);
+      case WANB200_EPI_BIAS_GELU: return launch_gemm_lora<WANB200_EPI_BIAS_GELU>(ta, tb, th, tu, ga, *lora, grid, st);
+      case WANB200_EPI_BIAS_SILU: return launch_gemm_lora<WANB200_EPI_BIAS_SILU>(ta, tb, th, tu, ga, *lora, grid, st);
+      case WANB200_EPI_BIAS_GATE_RES:
+        return launch_gemm_lora<WANB200_EPI_BIAS_GATE_RES>(ta, tb, th, tu, ga, *lora, grid, st);
+      default: return launch_gemm_lora<WANB200_EPI_BIAS_RES>(ta, tb, th, tu, ga, *lora, grid, st);
+    }
+  }
   switch (epi) {
     case WANB200_EPI_NONE: return launch_gemm<WANB200_EPI_NONE>(ta, tb, ga, grid, st);
     case WANB200_EPI_BIAS: return launch_gemm<WANB200_EPI_BIAS>(ta, tb, ga, grid, st);

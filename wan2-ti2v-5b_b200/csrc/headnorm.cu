@@ -1,0 +1,208 @@
+// RMS norm of every head of the query and key sections with the position rotation in the same
+// pass.  Per head x[0..D): y = x * rsqrt(mean(x^2) + eps) * gamma, then the pairs (a, b) of the
+// first `rot` channels become (a c - b s, a s + b c) with the angle of the row's position.  One
+// read and one write of 2 bytes per value: HBM-bound, and latency-bound at a few rows.
+#include "common.cuh"
+#include "internal.h"
+
+namespace wanb200 {
+
+struct HeadNormArgs {
+  const __nv_bfloat16* x;
+  __nv_bfloat16* out;
+  int64_t ldx, ldo, rows;
+  int64_t col0[2];
+  int heads0, heads;  // heads of section 0, of all sections
+  const __nv_bfloat16* gamma[2];
+  float eps;
+  int rot;
+  const float* cos;
+  const float* sin;
+  const int32_t* positions;
+  int64_t table_rows;
+  int groups;  // warps per row
+  int* err;
+};
+
+// A head is LPH = D / 8 lanes of 16 bytes, so a warp holds 32 / LPH heads at once and takes NV such
+// passes of one row, all loads in flight before the first use.  Sums and the norm are fp32 over
+// the head's lanes (a butterfly inside the lane group); the lane's angles are read once per row
+// and serve all its heads.  Interleaved pairs live inside a lane; half-split pairs (i, i + rot/2)
+// are exchanged with the partner lane by shuffles.  One rounding, to bf16, at the store.
+template <int LPH, int NV, bool INTER>
+__global__ void __launch_bounds__(256) head_norm_rope_kernel(const HeadNormArgs a) {
+  constexpr int HP = 32 / LPH, D = LPH * 8;
+  const int lane = threadIdx.x & 31;
+  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t row = w / a.groups;
+  if (row >= a.rows) return;  // warp-uniform
+  const int h0 = (int)(w - row * a.groups) * (HP * NV) + lane / LPH;
+  const int c = lane % LPH;  // this lane's 8 channels: 8c .. 8c + 7
+  uint4 raw[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int h = h0 + i * HP;
+    raw[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (h < a.heads) {
+      const int s = h >= a.heads0;
+      raw[i] = *reinterpret_cast<const uint4*>(a.x + row * a.ldx + (s ? a.col0[1] : a.col0[0]) +
+                                               (int64_t)(h - (s ? a.heads0 : 0)) * D + 8 * c);
+    }
+  }
+  const int half = a.rot >> 4;  // lanes of one half of the rotated channels (half-split pairs)
+  const bool turned = 8 * c < a.rot;
+  float cs[8], sn[8];
+  if (a.cos) {
+    const int64_t pos = a.positions ? (int64_t)__ldg(a.positions + row) : row % a.table_rows;
+    if (pos < 0 || pos >= a.table_rows) {  // warp-uniform: the row is left as it was
+      if (lane == 0) atomicCAS(a.err, 0, kErrBadPosition);
+      return;
+    }
+    if (turned) {
+      const int p0 = INTER ? 4 * c : 8 * (c < half ? c : c - half);
+      const float4* cp = reinterpret_cast<const float4*>(a.cos + pos * (a.rot >> 1) + p0);
+      const float4* sp = reinterpret_cast<const float4*>(a.sin + pos * (a.rot >> 1) + p0);
+#pragma unroll
+      for (int q = 0; q < (INTER ? 1 : 2); ++q) {
+        const float4 cv = __ldg(cp + q), sv = __ldg(sp + q);
+        cs[4 * q] = cv.x; cs[4 * q + 1] = cv.y; cs[4 * q + 2] = cv.z; cs[4 * q + 3] = cv.w;
+        sn[4 * q] = sv.x; sn[4 * q + 1] = sv.y; sn[4 * q + 2] = sv.z; sn[4 * q + 3] = sv.w;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int h = h0 + i * HP;
+    const int s = h >= a.heads0;
+    float x[8];
+    unpack_bf16x8(raw[i], x);
+    float q = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) q = fmaf(x[k], x[k], q);
+#pragma unroll
+    for (int o = LPH / 2; o; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+    const __nv_bfloat16* gamma = s ? a.gamma[1] : a.gamma[0];
+    if (gamma) {
+      const float rs = rsqrtf(q * (1.f / D) + a.eps);
+      float g[8];
+      unpack_bf16x8(__ldg(reinterpret_cast<const uint4*>(gamma) + c), g);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] *= rs * g[k];
+    }
+    if (a.cos) {
+      if constexpr (INTER) {
+        if (turned) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float u = x[2 * k], v = x[2 * k + 1];
+            x[2 * k] = u * cs[k] - v * sn[k];
+            x[2 * k + 1] = u * sn[k] + v * cs[k];
+          }
+        }
+      } else {
+        const int partner = lane + (c < half ? half : -half);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float o = __shfl_sync(0xffffffffu, x[k], partner & 31);
+          if (turned) x[k] = c < half ? x[k] * cs[k] - o * sn[k] : o * sn[k] + x[k] * cs[k];
+        }
+      }
+    }
+    if (h < a.heads) {
+      uint4 u;
+      u.x = pack_bf16x2(x[0], x[1]);
+      u.y = pack_bf16x2(x[2], x[3]);
+      u.z = pack_bf16x2(x[4], x[5]);
+      u.w = pack_bf16x2(x[6], x[7]);
+      *reinterpret_cast<uint4*>(a.out + row * a.ldo + (s ? a.col0[1] : a.col0[0]) +
+                                (int64_t)(h - (s ? a.heads0 : 0)) * D + 8 * c) = u;
+    }
+  }
+}
+
+template <int LPH, int NV>
+static void launch_head_norm(const HeadNormArgs& a, bool inter, unsigned blocks, cudaStream_t st) {
+  if (inter)
+    head_norm_rope_kernel<LPH, NV, true><<<blocks, 256, 0, st>>>(a);
+  else
+    head_norm_rope_kernel<LPH, NV, false><<<blocks, 256, 0, st>>>(a);
+}
+
+template <int LPH>
+static void launch_head_norm(const HeadNormArgs& a, int nv, bool inter, unsigned blocks, cudaStream_t st) {
+  if (nv == 1)
+    launch_head_norm<LPH, 1>(a, inter, blocks, st);
+  else
+    launch_head_norm<LPH, 4>(a, inter, blocks, st);
+}
+
+int head_norm_rope(const wanb200_headnorm_params* p, cudaStream_t st) {
+  if (!p) return set_error(WANB200_EINVAL, "head_norm_rope: null params");
+  if (!p->x || !p->out || p->rows <= 0) return set_error(WANB200_EINVAL, "head_norm_rope: need x, out, rows > 0");
+  if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)
+    return set_error(WANB200_EINVAL, "head_norm_rope: head_dim must be 64, 128 or 256");
+  if (p->nsections < 1 || p->nsections > 2)
+    return set_error(WANB200_EINVAL, "head_norm_rope: nsections must be 1 or 2");
+  if (p->ldx <= 0 || p->ldo <= 0 || p->ldx % 8 || p->ldo % 8 || !aligned16(p->x) || !aligned16(p->out))
+    return set_error(WANB200_EINVAL, "head_norm_rope: x / out need 16-byte aligned pointers and row strides % 8 == 0");
+  if (p->x == p->out && p->ldx != p->ldo)
+    return set_error(WANB200_EINVAL, "head_norm_rope: in place needs equal row strides");
+  int64_t heads = 0;
+  for (int s = 0; s < p->nsections; ++s) {
+    if (p->heads[s] <= 0 || p->heads[s] > 65535 || p->col0[s] < 0 || p->col0[s] % 8 ||
+        p->col0[s] + (int64_t)p->heads[s] * p->head_dim > std::min(p->ldx, p->ldo) || !aligned16(p->gamma[s]))
+      return set_error(WANB200_EINVAL, "head_norm_rope: bad section (col0 % 8 == 0, heads * head_dim inside the row, "
+                                       "16-byte aligned gamma)");
+    heads += p->heads[s];
+  }
+  if (p->nsections == 2) {  // a warp may hold heads of both, so they must not share channels
+    const int64_t e0 = p->col0[0] + (int64_t)p->heads[0] * p->head_dim, e1 = p->col0[1] + (int64_t)p->heads[1] * p->head_dim;
+    if (p->col0[0] < e1 && p->col0[1] < e0) return set_error(WANB200_EINVAL, "head_norm_rope: the sections overlap");
+  }
+  if ((!p->cos) != (!p->sin)) return set_error(WANB200_EINVAL, "head_norm_rope: cos and sin come together");
+  if (p->cos) {
+    if (p->rot <= 0 || p->rot % 16 || p->rot > p->head_dim)
+      return set_error(WANB200_EINVAL, "head_norm_rope: rot must be a multiple of 16 in 16..head_dim");
+    if (p->table_rows <= 0 || !aligned16(p->cos) || !aligned16(p->sin))
+      return set_error(WANB200_EINVAL, "head_norm_rope: rotation needs 16-byte aligned tables and table_rows > 0");
+  } else if (!p->gamma[0] && (p->nsections == 1 || !p->gamma[1])) {
+    return set_error(WANB200_EINVAL, "head_norm_rope: neither a gamma nor a rotation");
+  }
+  int* err = device_error_word();
+  if (!err) return WANB200_ECUDA;
+  HeadNormArgs a;
+  a.x = reinterpret_cast<const __nv_bfloat16*>(p->x);
+  a.out = reinterpret_cast<__nv_bfloat16*>(p->out);
+  a.ldx = p->ldx;
+  a.ldo = p->ldo;
+  a.rows = p->rows;
+  a.col0[0] = p->col0[0];
+  a.col0[1] = p->nsections > 1 ? p->col0[1] : 0;
+  a.heads0 = p->heads[0];
+  a.heads = (int)heads;
+  a.gamma[0] = reinterpret_cast<const __nv_bfloat16*>(p->gamma[0]);
+  a.gamma[1] = p->nsections > 1 ? reinterpret_cast<const __nv_bfloat16*>(p->gamma[1]) : nullptr;
+  a.eps = p->eps;
+  a.rot = p->cos ? p->rot : 0;
+  a.cos = p->cos;
+  a.sin = p->sin;
+  a.positions = p->cos ? p->positions : nullptr;
+  a.table_rows = p->cos ? p->table_rows : 1;
+  a.err = err;
+  const int lph = p->head_dim / 8, hp = 32 / lph;
+  const int nv = 4;
+  a.groups = (int)((heads + hp * nv - 1) / (hp * nv));
+  const int64_t blocks = (p->rows * a.groups + 7) / 8;
+  if (p->rows > INT32_MAX || blocks > INT32_MAX) return set_error(WANB200_EINVAL, "head_norm_rope: too many rows");
+  if (lph == 8)
+    launch_head_norm<8>(a, nv, p->interleaved != 0, (unsigned)blocks, st);
+  else if (lph == 16)
+    launch_head_norm<16>(a, nv, p->interleaved != 0, (unsigned)blocks, st);
+  else
+    launch_head_norm<32>(a, nv, p->interleaved != 0, (unsigned)blocks, st);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return set_cuda_error("head_norm_rope_kernel launch", e);
+  return WANB200_OK;
+}
+
+}  // namespace wanb200

@@ -38,6 +38,11 @@ int make_tmap_4d_u8(CUtensorMap* m, const void* base, const int64_t dims[4], con
 
 // Launchers (one per public entry point).
 int gemm_bf16(const wanb200_gemm_params* p, cudaStream_t st);
+struct LoraPlan;  // lora.h
+int gemm_validate(const wanb200_gemm_params* p);
+int gemm_launch(const wanb200_gemm_params* p, const LoraPlan* lora, int* err, cudaStream_t st);  // validated params
+int gemm_lora(const wanb200_lora_params* p, cudaStream_t st);
+int64_t lora_workspace_bytes(int64_t M, int adapters, int rank, int out_f32);
 int attn_fwd(const wanb200_attn_params* p, cudaStream_t st);
 // e4m3 operands of the attention (quantised by attn_fwd_fp8)
 struct AttnFp8Operands {
@@ -59,6 +64,9 @@ int attn_kv_splits(int64_t batch, int64_t heads, int64_t q_len, int64_t kv_len);
 int layernorm(const wanb200_ln_params* p, cudaStream_t st);
 int qk_norm_rope(const wanb200_qknorm_params* p, cudaStream_t st);
 int sumsq_reduce(const wanb200_sumsq_reduce_params* p, cudaStream_t st);
+int head_norm_rope(const wanb200_headnorm_params* p, cudaStream_t st);
+int range_attn_fwd(const wanb200_range_attn_params* p, cudaStream_t st);
+int64_t range_attn_workspace_bytes(const wanb200_range_attn_params* p);
 int bias_gate_residual(const wanb200_residual_params* p, cudaStream_t st);
 int peer_barrier(int* const* flags, int rank, int world, int epoch, cudaStream_t st);
 int shard_gather(const wanb200_shard_gather_params* p, cudaStream_t st);

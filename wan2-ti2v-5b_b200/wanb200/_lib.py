@@ -113,12 +113,38 @@ class BlockParams(ctypes.Structure):
                 ("all_reduce_ctx", c_void_p)]
 
 
+class HeadNormParams(ctypes.Structure):
+    _fields_ = [("x", c_void_p), ("ldx", c_int64), ("out", c_void_p), ("ldo", c_int64), ("rows", c_int64),
+                ("nsections", c_int), ("col0", c_int64 * 2), ("heads", c_int * 2), ("gamma", c_void_p * 2),
+                ("head_dim", c_int), ("eps", c_float), ("rot", c_int), ("interleaved", c_int), ("cos", c_void_p),
+                ("sin", c_void_p), ("positions", c_void_p), ("table_rows", c_int64)]
+
+
+class RangeAttnParams(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("q_tok_stride", c_int64), ("q_batch_stride", c_int64),
+                ("k", c_void_p), ("k_tok_stride", c_int64), ("k_batch_stride", c_int64),
+                ("v", c_void_p), ("v_tok_stride", c_int64), ("v_batch_stride", c_int64),
+                ("o", c_void_p), ("o_tok_stride", c_int64), ("o_batch_stride", c_int64),
+                ("batch", c_int64), ("heads", c_int64), ("kv_heads", c_int64), ("q_len", c_int64), ("kv_len", c_int64),
+                ("head_dim", c_int64), ("softmax_scale", c_float), ("softcap", c_float),
+                ("lo", c_void_p), ("hi", c_void_p), ("pos", c_void_p), ("range_batch_stride", c_int64),
+                ("slopes", c_void_p), ("dist_bias", c_void_p), ("reach", c_int), ("workspace", c_void_p),
+                ("workspace_bytes", c_int64)]
+
+
+class LoraParams(ctypes.Structure):
+    _fields_ = [("gemm", GemmParams), ("down", c_void_p), ("up", c_void_p), ("scales", c_void_p), ("ids", c_void_p),
+                ("adapters", c_int), ("rank", c_int), ("lora_workspace", c_void_p), ("lora_workspace_bytes", c_int64)]
+
+
 EXPORTS = ("wanb200_gemm_bf16", "wanb200_attn_fwd", "wanb200_layernorm", "wanb200_qk_norm_rope",
            "wanb200_bias_gate_residual", "wanb200_last_error", "wanb200_device_error", "wanb200_version",
            "wanb200_struct_sizes", "wanb200_peer_barrier", "wanb200_attn_workspace_bytes",
            "wanb200_attn_kv_splits", "wanb200_attn_fwd_noalloc", "wanb200_shard_gather", "wanb200_attn_fwd_fp8",
            "wanb200_attn_fp8_workspace_bytes", "wanb200_device_error_async", "wanb200_block_forward",
-           "wanb200_block_workspace_bytes", "wanb200_patchify", "wanb200_unpatchify_cfg", "wanb200_sumsq_reduce")
+           "wanb200_block_workspace_bytes", "wanb200_patchify", "wanb200_unpatchify_cfg", "wanb200_sumsq_reduce",
+           "wanb200_head_norm_rope", "wanb200_range_attn_fwd", "wanb200_range_attn_workspace_bytes",
+           "wanb200_gemm_lora", "wanb200_lora_workspace_bytes")
 
 _lock = threading.Lock()
 _lib = None
@@ -179,8 +205,19 @@ def load():
             lib.wanb200_unpatchify_cfg.restype = c_int
             lib.wanb200_sumsq_reduce.argtypes = [ctypes.POINTER(SumsqReduceParams), c_void_p]
             lib.wanb200_sumsq_reduce.restype = c_int
+            lib.wanb200_head_norm_rope.argtypes = [ctypes.POINTER(HeadNormParams), c_void_p]
+            lib.wanb200_head_norm_rope.restype = c_int
+            lib.wanb200_range_attn_fwd.argtypes = [ctypes.POINTER(RangeAttnParams), c_void_p]
+            lib.wanb200_range_attn_fwd.restype = c_int
+            lib.wanb200_range_attn_workspace_bytes.argtypes = [ctypes.POINTER(RangeAttnParams)]
+            lib.wanb200_range_attn_workspace_bytes.restype = c_int64
+            lib.wanb200_gemm_lora.argtypes = [ctypes.POINTER(LoraParams), c_void_p]
+            lib.wanb200_gemm_lora.restype = c_int
+            lib.wanb200_lora_workspace_bytes.argtypes = [c_int64, c_int, c_int, c_int]
+            lib.wanb200_lora_workspace_bytes.restype = c_int64
             structs = (GemmParams, AttnParams, LnParams, QkNormParams, ResidualParams, ShardGatherParams,
-                       AttnFp8Params, BlockParams, PatchifyParams, UnpatchifyParams, SumsqReduceParams)
+                       AttnFp8Params, BlockParams, PatchifyParams, UnpatchifyParams, SumsqReduceParams,
+                       HeadNormParams, RangeAttnParams, LoraParams)
             sizes = (c_int64 * len(structs))()
             n = lib.wanb200_struct_sizes(sizes, len(structs))
             want = [ctypes.sizeof(c) for c in structs]

@@ -6,6 +6,7 @@ library or a non-CUDA tensor raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 
@@ -386,6 +387,209 @@ def bias_gate_residual(residual, y, bias, gate=None, frames=None, out=None, nsum
     L.check(_launch(residual, "bias_gate_residual", (residual.element_size() + 2.0 * nsum + out.element_size()) * M * C,
                     lambda: lib.wanb200_bias_gate_residual(ctypes.byref(p), _stream(residual))),
             "wanb200_bias_gate_residual")
+    return out
+
+
+# ---------------------------------------------------------------------------- packed request batches
+def _same_device(*ts):
+    """All tensors on one CUDA device, which is returned."""
+    _cuda(*ts)
+    devs = {t.device for t in ts if t is not None}
+    _need(len(devs) == 1, f"all tensors must be on one device, got {sorted(map(str, devs))}")
+    return devs.pop()
+
+
+def _on(device):
+    """Context in which `device` is the current one (the library launches on the current device)."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _overlap(a, b):
+    """Whether the memory that two tensors span overlaps."""
+    def span(t):
+        last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def head_norm_rope(x, sections, head_dim, *, out=None, eps=1e-6, cos=None, sin=None, positions=None,
+                   interleaved=True, kind="head_norm_rope"):
+    """RMS norm of every head with the rotation in the same pass (wanb200_head_norm_rope): for each
+    section (col0, heads, gamma [head_dim] bf16 or None) of x [M, ld] bf16 the heads of head_dim
+    channels at columns col0.. are normed (gamma None: not normed) and, with cos / sin
+    [P, rot / 2] fp32, their first rot channels rotated by row positions[m] of the tables
+    (positions [M] int32; None: row m % P).  interleaved: pairs (2i, 2i+1), else (i, i + rot/2).
+    In place on x, or into the same columns of out, whose other columns stay as they are.
+    qk_norm_rope norms over the whole width instead and takes one sequence length.
+
+    A position outside 0..P-1 leaves its row as it was and sets the device error word (501)."""
+    dev = _same_device(x, out, cos, sin, positions, *[g for _, _, g in sections])
+    out = x if out is None else out
+    for name, t in (("x", x), ("out", out)):
+        _need(t.dtype == BF16, f"head_norm_rope: {name} must be bf16")
+    ldx, ldo = _rows(x, "x"), _rows(out, "out")
+    M = x.shape[0]
+    _need(out.shape[0] == M, "head_norm_rope: out must have x's rows")
+    _need(1 <= len(sections) <= 2, "head_norm_rope: one or two sections")
+    if M == 0:
+        return out
+    same = out.data_ptr() == x.data_ptr() and ldx == ldo
+    _need(same or not _overlap(x, out), "head_norm_rope: out must be x or not overlap it")
+    p = L.HeadNormParams()
+    p.x, p.ldx, p.out, p.ldo, p.rows, p.nsections = _p(x), ldx, _p(out), ldo, M, len(sections)
+    p.head_dim, p.eps = head_dim, eps
+    vals = 0
+    for i, (c0, heads, g) in enumerate(sections):
+        _need(g is None or (g.dtype == BF16 and g.is_contiguous() and g.numel() == head_dim),
+              "head_norm_rope: gamma must be bf16 [head_dim]")
+        _need(heads > 0 and c0 >= 0 and c0 + heads * head_dim <= min(x.shape[1], out.shape[1]),
+              "head_norm_rope: a section lies outside the columns of x or out")
+        p.col0[i], p.heads[i], p.gamma[i] = c0, heads, _p(g)
+        vals += M * heads * head_dim
+    if M == 1:  # a single row's stride is never used; torch may report any
+        p.ldx = p.ldo = max(ldx, ldo, *[c0 + heads * head_dim for c0, heads, _ in sections]) + 7 & ~7
+    _need((cos is None) == (sin is None), "head_norm_rope: cos and sin come together")
+    if cos is not None:
+        _need(cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.dim() == 2 and cos.shape == sin.shape and
+              cos.is_contiguous() and sin.is_contiguous(), "head_norm_rope: cos / sin must be contiguous fp32 [P, rot / 2]")
+        p.cos, p.sin, p.table_rows, p.rot, p.interleaved = _p(cos), _p(sin), cos.shape[0], 2 * cos.shape[1], int(interleaved)
+    if positions is not None:
+        _need(cos is not None, "head_norm_rope: positions need cos / sin")
+        _need(positions.dtype == torch.int32 and positions.is_contiguous() and positions.numel() == M,
+              "head_norm_rope: positions must be int32 [M]")
+        p.positions = _p(positions)
+    lib = L.load()
+    with _on(dev):
+        L.check(_launch(x, kind, 4.0 * vals, lambda: lib.wanb200_head_norm_rope(ctypes.byref(p), _stream(x))),
+                "wanb200_head_norm_rope")
+    return out
+
+
+def range_attention(q, k, v, lo, hi, *, pos=None, out=None, softmax_scale=None, softcap=0.0, slopes=None,
+                    dist_bias=None, kind="attn_range"):
+    """Attention of q [B, Lq, H, D] over the keys lo <= j < hi of each row, k / v [B, Lk, Hkv, D]
+    with H a multiple of Hkv (query head h reads key head h // (H / Hkv)), D 64 or 128, head stride
+    D.  lo, hi (and pos): int32 [Lq] for every batch element or [B, Lq]; a row with no keys gives
+    zeros.  softcap c > 0: scores c tanh(s / c).  slopes [H] fp32: bias -slopes[h] |j - pos|;
+    dist_bias [H, 2R + 1] fp32: bias dist_bias[h, clamp(j - pos, -R, R) + R]; pos defaults to the
+    row index.  lo, hi and pos are read on the device at every call, so a captured graph follows
+    them.  wanb200.ranges has the common masks (packed documents, caches)."""
+    dev = _same_device(q, k, v, lo, hi, pos, out, slopes, dist_bias)
+    for name, t in (("q", q), ("k", k), ("v", v)) + ((("out", out),) if out is not None else ()):
+        _need(t.dtype == BF16 and t.dim() == 4, f"range_attention: {name} must be bf16 [B, L, H, D]")
+    B, Lq, H, D = q.shape
+    Lk, Hkv = k.shape[1], k.shape[2]
+    _need(k.shape[0] == B and k.shape[3] == D and v.shape == k.shape, "range_attention: q/k/v shape mismatch")
+    _need(D in (64, 128), "range_attention: head_dim must be 64 or 128")
+    _need(Hkv > 0 and H % Hkv == 0, "range_attention: the query heads must be a multiple of the key heads")
+    if out is None:
+        out = torch.empty(B, Lq, H, D, dtype=BF16, device=q.device)
+    _need(out.shape == q.shape, "range_attention: out must have q's shape")
+    if out.numel() == 0:
+        return out
+    if Lk == 0:
+        return out.zero_()
+
+    def strides(t, name):
+        b, n, h, _ = t.shape
+        _need(t.stride(3) == 1 and (h == 1 or t.stride(2) == D), f"range_attention: {name} must have head stride {D}")
+        tok = t.stride(1) if n > 1 else h * D  # the stride of a dimension of one is never used
+        return tok, t.stride(0) if b > 1 else n * tok
+
+    p = L.RangeAttnParams()
+    p.q, (p.q_tok_stride, p.q_batch_stride) = _p(q), strides(q, "q")
+    p.k, (p.k_tok_stride, p.k_batch_stride) = _p(k), strides(k, "k")
+    p.v, (p.v_tok_stride, p.v_batch_stride) = _p(v), strides(v, "v")
+    p.o, (p.o_tok_stride, p.o_batch_stride) = _p(out), strides(out, "out")
+    p.batch, p.heads, p.kv_heads, p.q_len, p.kv_len, p.head_dim = B, H, Hkv, Lq, Lk, D
+    p.softmax_scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)
+    p.softcap = softcap
+    for name, t in (("lo", lo), ("hi", hi), ("pos", pos)):
+        _need(t is None or (t.dtype == torch.int32 and t.is_contiguous() and t.shape == lo.shape and
+                            t.shape in ((Lq,), (1, Lq), (B, Lq))),
+              f"range_attention: {name} must be contiguous int32 [Lq] or [B, Lq], all of one shape")
+    p.lo, p.hi, p.pos = _p(lo), _p(hi), _p(pos)
+    p.range_batch_stride = Lq if lo.dim() == 2 and lo.shape[0] == B and B > 1 else 0
+    _need(slopes is None or dist_bias is None, "range_attention: slopes or dist_bias, not both")
+    if slopes is not None:
+        _need(slopes.dtype == torch.float32 and slopes.is_contiguous() and slopes.shape == (H,),
+              "range_attention: slopes must be contiguous fp32 [H]")
+        p.slopes = _p(slopes)
+    if dist_bias is not None:
+        _need(dist_bias.dtype == torch.float32 and dist_bias.is_contiguous() and dist_bias.dim() == 2 and
+              dist_bias.shape[0] == H and dist_bias.shape[1] % 2 == 1,
+              "range_attention: dist_bias must be contiguous fp32 [H, 2R + 1]")
+        p.dist_bias, p.reach = _p(dist_bias), dist_bias.shape[1] // 2
+    _need(not any(_overlap(out, t) for t in (q, k, v)), "range_attention: out must not overlap q, k or v")
+    lib = L.load()
+    with _on(dev):
+        nbytes = lib.wanb200_range_attn_workspace_bytes(ctypes.byref(p))
+        if nbytes:  # from torch's allocator: ordered on this stream, and a captured graph's own
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            p.workspace, p.workspace_bytes = _p(ws), nbytes
+        # the work in the launch record is that of the full rectangle; the ranges are on the device
+        L.check(_launch(q, kind, 4.0 * B * H * Lq * Lk * D,
+                        lambda: lib.wanb200_range_attn_fwd(ctypes.byref(p), _stream(q))), "wanb200_range_attn_fwd")
+    return out
+
+
+def lora_linear(a, w, bias, down, up, ids, *, scales=None, epilogue=L.EPI_BIAS, out=None, residual=None, gate=None,
+                frames=None, kind="lora_linear", tile_n=0):
+    """`linear` with a low-rank adapter per row (wanb200_gemm_lora): out = epilogue(a @ w^T +
+    scales[id] (a @ down[id]^T) @ up[:, id]^T) with id = ids[row], no update where id < 0.
+    down [n, r, K] and up [N, n, r] bf16, the adapters of all requests side by side (r a multiple of
+    8, n r <= 4096; pad smaller ranks with zeros); ids [M] int32, any order (rows of one adapter
+    next to each other cost least); scales [n] fp32.  epilogue, residual, gate, frames, out as for
+    `linear`, but not EPI_BIAS_SUMSQ and EPI_SCATTER.  ids are read on the device at every call; an
+    id >= n counts as none and sets the device error word (502)."""
+    gm, ge = gate if gate is not None else (None, None)
+    dev = _same_device(a, w, bias, down, up, ids, scales, out, residual, gm, ge)
+    for name, t in (("a", a), ("w", w), ("down", down), ("up", up)):
+        _need(t.dtype == BF16, f"lora_linear: {name} must be bf16")
+    lda, ldw = _rows(a, "a"), _rows(w, "w")
+    M, K = a.shape
+    N = w.shape[0]
+    _need(w.shape[1] == K, f"lora_linear: a is [*, {K}] but w is {tuple(w.shape)}")
+    _need(down.dim() == 3 and down.is_contiguous() and down.shape[2] == K, "lora_linear: down must be contiguous [n, r, K]")
+    n, r = down.shape[:2]
+    _need(up.is_contiguous() and tuple(up.shape) == (N, n, r), "lora_linear: up must be contiguous [N, n, r]")
+    _need(ids.dtype == torch.int32 and ids.is_contiguous() and ids.numel() == M, "lora_linear: ids must be int32 [M]")
+    _need(scales is None or (scales.dtype == torch.float32 and scales.is_contiguous() and scales.numel() == n),
+          "lora_linear: scales must be contiguous fp32 [n]")
+    _need(bias is None or (bias.dtype == BF16 and bias.is_contiguous() and bias.numel() == N),
+          "lora_linear: bias must be contiguous bf16 [N]")
+    if out is None:
+        out = torch.empty(M, N, dtype=BF16, device=a.device)
+    for name, t in (("out", out), ("residual", residual)):
+        _need(t is None or (t.dtype in (BF16, torch.float32) and tuple(t.shape) == (M, N)),
+              f"lora_linear: {name} must be bf16 or fp32 [M, N]")
+    if M == 0:
+        return out
+    _need(not _overlap(out, a), "lora_linear: out must not overlap a")
+    p = L.LoraParams()
+    g = p.gemm
+    g.out_f32 = int(out.dtype == torch.float32)
+    g.residual_f32 = int(residual is not None and residual.dtype == torch.float32)
+    one = M == 1  # a single row's stride is never used; torch may report any
+    g.a, g.lda, g.w, g.ldw, g.d, g.ldd = _p(a), K if one else lda, _p(w), ldw, _p(out), N if one else _rows(out, "out")
+    g.M, g.N, g.K, g.epilogue, g.bias, g.tile_n = M, N, K, epilogue, _p(bias), tile_n
+    if residual is not None:
+        g.residual, g.ldr = _p(residual), N if one else _rows(residual, "residual")
+    if gate is not None:
+        _need(gm.dtype == BF16 and ge.dtype == torch.float32 and ge.stride(-1) == 1, "lora_linear: bad gate tensors")
+        g.gate_mod, g.gate_e0, g.gate_frame_stride = _p(gm), _p(ge), ge.stride(0)
+    if frames is not None:
+        _set_frames(g, frames)
+    p.down, p.up, p.scales, p.ids, p.adapters, p.rank = _p(down), _p(up), _p(scales), _p(ids), n, r
+    lib = L.load()
+    with _on(dev):
+        nbytes = lib.wanb200_lora_workspace_bytes(M, n, r, g.out_f32)
+        if nbytes:  # from torch's allocator: ordered on this stream, and a captured graph's own
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            p.lora_workspace, p.lora_workspace_bytes = _p(ws), nbytes
+        L.check(_launch(a, kind, 2.0 * M * N * K + 2.0 * M * r * (K + N),
+                        lambda: lib.wanb200_gemm_lora(ctypes.byref(p), _stream(a))), "wanb200_gemm_lora")
     return out
 
 
