@@ -384,6 +384,18 @@ def test_range_attention_documents(lengths, block, prefix, window, H, Hkv, D, wo
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lengths,block,prefix,H,Hkv,D", [
+    ([2600], 374, None, 16, 16, 128), ([3000, 77, 900], 1, 130, 8, 4, 128), ([1500, 2000], 0, None, 24, 24, 64)])
+def test_range_attention_many_units_a_block(lengths, block, prefix, H, Hkv, D, word):
+    """More units than SMs, each with a run of fully seen key tiles before the partly seen ones."""
+    T = sum(lengths)
+    q, k, v = randn(1, T, H, D, seed=4), randn(1, T, Hkv, D, seed=5), randn(1, T, Hkv, D, seed=6)
+    lo, hi = ranges.document_ranges(lengths, DEV, block=block, prefix=prefix)
+    got = check_attn(q, k, v, lo, hi)
+    assert torch.equal(got, ops.range_attention(q, k, v, lo, hi))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("cap", [0.0, 5.0, 50.0])
 @pytest.mark.parametrize("bias", ["none", "slopes", "table", "short_table", "flat_table"])

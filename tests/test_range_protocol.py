@@ -1,0 +1,203 @@
+"""CPU model of the barrier protocol of range_attn_kernel (wan2-ti2v-5b_b200/csrc/attn_range.cu).
+
+On top of the unmasked attention's protocol (test_attn_protocol.py) come a queue of units, query
+tiles of a pair that skip key tiles, and two warps that look through the V tiles which are not seen
+by every row before they are multiplied.  The model also notes which load a ring slot holds, so a
+wait that passes a phase too early shows as a wrong load."""
+import random
+
+from test_attn_protocol import Bar, _drive
+
+
+def run(units, ring, seed, check_waits_every_tile=True):
+    """units: [(ranges of tile 0, of tile 1, partial key tiles)], ranges as (first, end) key tiles."""
+    rnd = random.Random(seed)
+    kv_full, kv_empty = [Bar(1) for _ in range(ring)], [Bar(1) for _ in range(ring)]
+    v_ok = [Bar(2) for _ in range(ring)]
+    q_full, q_empty = Bar(1), Bar(1)
+    s_full, p_part, p_full, o_done = ([Bar(1) for _ in range(2)] for _ in range(4))
+    u_full, u_empty = [Bar(1) for _ in range(2)], [Bar(5) for _ in range(2)]  # MMA, 2 softmax groups, 2 checks
+    holds = [None] * ring
+    pipe, wrong = [], []
+
+    def has(u, t, j):
+        return u[t][0] <= j < u[t][1]
+
+    def tiles(u):
+        ends = [r for r in u[:2] if r[0] < r[1]]
+        return [j for j in range(min(r[0] for r in ends), max(r[1] for r in ends)) if has(u, 0, j) or has(u, 1, j)] \
+            if ends else []
+
+    def producer():
+        g = q = 0
+        for i in range(len(units) + 1):
+            yield ("wait", u_empty[i % 2], (i // 2 & 1) ^ 1)
+            u_full[i % 2].arrive()
+            if i == len(units):
+                return
+            js = tiles(units[i])
+            if not js:
+                continue
+            yield ("wait", q_empty, (q & 1) ^ 1)
+            q += 1
+            yield ("work", rnd.randint(1, 4))
+            q_full.arrive()
+            for j in js:
+                for x in "KV":
+                    yield ("wait", kv_empty[g % ring], (g // ring & 1) ^ 1)
+                    yield ("work", rnd.randint(1, 5))
+                    holds[g % ring] = (i, j, x)
+                    kv_full[g % ring].arrive()
+                    g += 1
+
+    def issuer():
+        g = q = 0
+        np, ok = [0, 0], [0] * ring
+        for i in range(len(units) + 1):
+            yield ("wait", u_full[i % 2], i // 2 & 1)
+            if i == len(units):
+                return
+            u_empty[i % 2].arrive()
+            u = units[i]
+            js = tiles(u)
+            if not js:
+                continue
+
+            def kv(r, j, x):
+                yield ("wait", kv_full[r % ring], r // ring & 1)
+                if holds[r % ring] != (i, j, x):
+                    wrong.append(("mma", i, j, x))
+
+            def qk(t):
+                pipe.append(["mma", rnd.randint(2, 4)])
+                pipe.append(["commit", s_full[t]])
+
+            def pv(t, j):
+                ph = np[t] & 1
+                np[t] += 1
+                yield ("wait", p_part[t], ph)
+                pipe.append(["mma", rnd.randint(1, 3)])
+                yield ("wait", p_full[t], ph)
+                pipe.append(["mma", rnd.randint(1, 2)])
+                if j == u[t][1] - 1:
+                    pipe.append(["commit", o_done[t]])
+
+            yield ("wait", q_full, q & 1)
+            q += 1
+            yield from kv(g, js[0], "K")
+            for t in (0, 1):
+                if has(u, t, js[0]):
+                    qk(t)
+            pipe.append(["commit", kv_empty[g % ring]])
+            if len(js) == 1:
+                pipe.append(["commit", q_empty])
+            for n, j in enumerate(js):
+                nxt = js[n + 1] if n + 1 < len(js) else None
+                vs, ks = (g + 1) % ring, (g + 2) % ring
+                yield from kv(g + 1, j, "V")
+                if j in u[2]:
+                    yield ("wait", v_ok[vs], ok[vs])
+                    ok[vs] ^= 1
+                if has(u, 0, j):
+                    yield from pv(0, j)
+                if nxt is not None:
+                    yield from kv(g + 2, nxt, "K")
+                    if has(u, 0, nxt):
+                        qk(0)
+                if has(u, 1, j):
+                    yield from pv(1, j)
+                pipe.append(["commit", kv_empty[vs]])
+                g += 2
+                if nxt is None:
+                    break
+                if has(u, 1, nxt):
+                    qk(1)
+                pipe.append(["commit", kv_empty[ks]])
+                if n + 2 == len(js):
+                    pipe.append(["commit", q_empty])
+
+    def check():
+        g = 0
+        for i in range(len(units) + 1):
+            yield ("wait", u_full[i % 2], i // 2 & 1)
+            if i == len(units):
+                return
+            u_empty[i % 2].arrive()
+            for j in tiles(units[i]):
+                r = g + 1
+                partial = j in units[i][2]
+                if check_waits_every_tile or partial:
+                    yield ("wait", kv_full[r % ring], r // ring & 1)
+                if partial:
+                    if holds[r % ring] != (i, j, "V"):
+                        wrong.append(("check", i, j))
+                    yield ("work", rnd.randint(1, 8))
+                    v_ok[r % ring].arrive()
+                g += 2
+
+    def softmax(t):
+        g = ns = no = 0
+        ok = [0] * ring
+        for i in range(len(units) + 1):
+            yield ("wait", u_full[i % 2], i // 2 & 1)
+            if i == len(units):
+                return
+            u_empty[i % 2].arrive()
+            u, any_tile = units[i], False
+            for j in tiles(u):
+                vs = (g + 1) % ring
+                g += 2
+                if not has(u, t, j):
+                    if j in u[2]:
+                        ok[vs] ^= 1
+                    continue
+                any_tile = True
+                yield ("wait", s_full[t], ns & 1)
+                ns += 1
+                yield ("work", rnd.randint(1, 6))
+                if j in u[2]:
+                    yield ("wait", v_ok[vs], ok[vs])
+                    ok[vs] ^= 1
+                    if holds[vs] != (i, j, "V"):
+                        wrong.append(("softmax", i, j))
+                yield ("work", rnd.randint(1, 6))
+                p_part[t].arrive()
+                yield ("work", rnd.randint(1, 3))
+                p_full[t].arrive()
+            if any_tile:
+                yield ("wait", o_done[t], no & 1)
+                no += 1
+            yield ("work", rnd.randint(1, 6))
+
+    agents = {"producer": producer(), "issuer": issuer(), "check0": check(), "check1": check(), "softmax0": softmax(0),
+              "softmax1": softmax(1)}
+    return _drive(agents, pipe, rnd) and not wrong
+
+
+def random_units(rnd):
+    units = []
+    for _ in range(rnd.randint(1, 6)):
+        r = []
+        for _ in range(2):
+            a = rnd.randint(0, 12)
+            r.append((a, a + rnd.choice([0, 1, 1, 2, 5, 9, 14])))
+        units.append((*r, {j for j in range(30) if rnd.random() < rnd.choice([0.1, 0.5, 1.0])}))
+    return units
+
+
+def test_range_protocol_never_deadlocks():
+    for seed in range(120):
+        units = random_units(random.Random(seed))
+        for ring in (5, 8):  # head_dim 128 and 64
+            assert run(units, ring, seed), (units, ring, seed)
+
+
+def test_checking_warps_must_wait_for_every_tile():
+    """Waiting only for the tiles that are looked through lets a warp run ahead of the ring by two
+    phases of a slot: it then reads an older load, and the protocol can stop."""
+    fails = 0
+    for seed in range(60):
+        rnd = random.Random(seed)
+        units = [((0, 20), (0, 20), {19}) for _ in range(rnd.randint(1, 4))]
+        fails += not run(units, 5, seed, check_waits_every_tile=False)
+    assert fails > 0

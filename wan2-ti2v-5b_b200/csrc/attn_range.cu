@@ -796,11 +796,13 @@ __global__ void __maxnreg__(160)
         for (int j = w.k0; ok && j < w.k1; ++j) {
           if (!unit_loads(w, j)) continue;
           const int slot = (gk + 1) % RING;
+          // every V tile is waited for, also one with nothing to look through: a warp that ran ahead
+          // would take an older fill of the slot for this one and arrive on v_ok a phase early
+          if (!mbar_wait_warp(kv_full + 8 * slot, ((gk + 1) / RING) & 1, abort_flag, err, kErrTimeoutAttnProducer)) {
+            ok = false;
+            break;
+          }
           if (unit_partial(w, j)) {
-            if (!mbar_wait_warp(kv_full + 8 * slot, ((gk + 1) / RING) & 1, abort_flag, err, kErrTimeoutAttnProducer)) {
-              ok = false;
-              break;
-            }
             bool wrote = false;
 #pragma unroll 1
             for (int x = 0; x < 2; ++x) {
