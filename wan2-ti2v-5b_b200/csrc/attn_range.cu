@@ -99,12 +99,6 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t zero_nonfinite(uint32_t u) {
-  if ((u & 0x7f80u) == 0x7f80u) u &= 0xffff0000u;
-  if ((u & 0x7f800000u) == 0x7f800000u) u &= 0xffffu;
-  return u;
-}
-
 template <int D, bool TWO, bool CAP, int BIAS>  // TWO: 9 to 16 rows (the second half of the MMA's rows is used)
 __global__ void __launch_bounds__(RD_WARPS * 32, TWO ? 2 : 3) range_decode_kernel(const RangeArgs a) {
   constexpr int KC = D / 32, VC = D / 64;  // 16-byte loads per K row, per V row
@@ -403,7 +397,7 @@ struct RangeTileCfg {
   static constexpr int TILE = RT_M * D * 2;
   static constexpr int RING = D == 128 ? 5 : 8;
   static constexpr int OFF_R = 2 * TILE, META = (2 + RING) * TILE;
-  static constexpr int SMEM = META + 512 + 1024;
+  static constexpr int SMEM = META + 640 + 1024;
 };
 
 // What the rows of one tile pair see: [t] key range of any row, key range of every row.
@@ -595,11 +589,13 @@ __global__ void __maxnreg__(160)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(meta + 320);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(meta + 324);
   uint32_t* bad = reinterpret_cast<uint32_t*>(meta + 336);  // [RING][4]: keys of the V tile with non-finite values
+  const uint32_t v_req = m0 + 464;  // RING
   int* err = g.err;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < RING; ++s) {
+      mbar_init(v_req + 8 * s, 1);
       mbar_init(kv_full + 8 * s, 1);
       mbar_init(kv_empty + 8 * s, 1);
       mbar_init(v_ok + 8 * s, 2);
@@ -691,6 +687,7 @@ __global__ void __maxnreg__(160)
               mbar_expect_tx(kv_full + 8 * slot, TILE);
               for (int h = 0; h < HALVES; ++h)
                 tma_load_4d(dst + h * RT_BLK, map, kv_full + 8 * slot, 64 * h, w.kh, j * RT_N, w.b);
+              if (x && unit_partial(w, j)) mbar_arrive(v_req + 8 * slot);
               issued |= 1u << slot;
               last_ph = (last_ph & ~(1u << slot)) | (ph << slot);
             }
@@ -785,7 +782,11 @@ __global__ void __maxnreg__(160)
       }
     } else {
       // ---------------------------------------------------------- non-finite values in partly seen V tiles
+      // The producer announces such a tile (v_req), so these warps pass over the others without a
+      // wait: the phases of v_req move only with the tiles they handle, and neither they nor
+      // kv_full can get a phase ahead before v_ok is given.
       int gk = 0;
+      uint32_t req_ph = 0;  // phase of v_req per ring slot
       bool ok = true;
       while (ok) {
         const int u = next_unit(kErrTimeoutAttnProducer);
@@ -796,13 +797,11 @@ __global__ void __maxnreg__(160)
         for (int j = w.k0; ok && j < w.k1; ++j) {
           if (!unit_loads(w, j)) continue;
           const int slot = (gk + 1) % RING;
-          // every V tile is waited for, also one with nothing to look through: a warp that ran ahead
-          // would take an older fill of the slot for this one and arrive on v_ok a phase early
-          if (!mbar_wait_warp(kv_full + 8 * slot, ((gk + 1) / RING) & 1, abort_flag, err, kErrTimeoutAttnProducer)) {
-            ok = false;
-            break;
-          }
           if (unit_partial(w, j)) {
+            ok = mbar_wait_warp(v_req + 8 * slot, (req_ph >> slot) & 1, abort_flag, err, kErrTimeoutAttnProducer) &&
+                 mbar_wait_warp(kv_full + 8 * slot, ((gk + 1) / RING) & 1, abort_flag, err, kErrTimeoutAttnProducer);
+            if (!ok) break;
+            req_ph ^= 1u << slot;
             bool wrote = false;
 #pragma unroll 1
             for (int x = 0; x < 2; ++x) {
@@ -824,7 +823,7 @@ __global__ void __maxnreg__(160)
               if (lane == 0) bad[slot * 4 + word] = bits;
               wrote |= bits != 0;
             }
-            if (wrote) fence_proxy_async_smem();
+            if (wrote) fence_proxy_async_smem();  // uniform over the warp: each lane for its own stores
             __syncwarp();
             if (lane == 0) mbar_arrive(v_ok + 8 * slot);
           }

@@ -331,6 +331,18 @@ __device__ __forceinline__ int nonfinite_bf16x2(uint32_t u) {
   return (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
 }
 
+// The packed pair with its NaNs and infinities replaced by zeros.
+__device__ __forceinline__ uint32_t zero_nonfinite(uint32_t u) {
+  if ((u & 0x7f80u) == 0x7f80u) u &= 0xffff0000u;
+  if ((u & 0x7f800000u) == 0x7f800000u) u &= 0xffffu;
+  return u;
+}
+
+// Programmatic dependent launch: wait until the launch before has completed and its writes are
+// visible; allow the launch behind to start.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Hardware tanh (one MUFU op; PTX tanh.approx.f32, max relative error 2^-11, far below the bf16
 // rounding of the GEMM output it feeds).
 __device__ __forceinline__ float tanh_approx(float x) {

@@ -52,7 +52,8 @@ struct GemmCfg {
 // per instruction) instead of one row per lane (32 rows touched by every 16-byte access).  The
 // host uses it on 256-wide tiles, where it costs the TMA ring no stage.
 constexpr int G_RES_STAGING = G_EPI_WARPS * 32 * 32 * 4;  // 32 KB
-constexpr int G_LORA_SMEM = 64;  // the adapter kernels' static shared memory (the bad-step words)
+constexpr int G_LORA_SMEM = 256;  // room for the adapter kernels' static shared memory (barriers, flags)
+constexpr int G_LORA_THREADS = G_THREADS + 64;  // and the two checking warps
 
 struct GemmArgs {
   void* d;  // bf16, or fp32 when out_f32
@@ -232,31 +233,32 @@ __device__ __forceinline__ void gemm_epilogue_chunk(const GemmArgs& a, float* v,
 __device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 
-// The steps of chunk c (4 bits) that the tile's MMA runs: used by one of its rows and finite.
-__device__ __forceinline__ uint32_t lora_chunk_steps(const uint32_t* mask, const uint32_t* bad, int c) {
-  return ((__ldg(mask + (c >> 3)) & ~bad[c >> 3]) >> ((c & 7) * 4)) & 0xfu;
+// The steps of chunk c (4 bits) that a row of the tile uses.
+__device__ __forceinline__ uint32_t lora_chunk_steps(const uint32_t* mask, int c) {
+  return (__ldg(mask + (c >> 3)) >> ((c & 7) * 4)) & 0xfu;
 }
 
-// What the steps left out of the MMA (their up-projection holds a NaN or an infinity) add to the
-// output of `row` at `col`: the row's own adapter only.  Never taken with finite weights; one
-// value a call, so that the accumulator chunk stays in registers.
-__device__ __noinline__ float lora_slow_value(const LoraPlan* lo, const uint32_t* bad, int row, int col) {
+// What the non-finite up-projection weights (zeroed in shared memory ahead of the MMA) add to the
+// output of `row` at `col`: the row's own adapter only.  Never taken with finite weights; one value
+// a call, so that the accumulator chunk stays in registers.
+__device__ __noinline__ float lora_slow_value(const LoraPlan* lo, int row, int col) {
   const int id = __ldg(lo->ids + row);
   if (id < 0 || id >= lo->adapters) return 0.f;
   float v = 0.f;
   for (int c = id * lo->rank; c < (id + 1) * lo->rank; ++c) {
-    if (!((bad[c >> 9] >> ((c >> 4) & 31)) & 1u)) continue;
+    const float u = __bfloat162float(lo->up[(int64_t)col * lo->adapters * lo->rank + c]);
+    if (isfinite(u)) continue;
     float h = 0.f;
     for (int pl = 0; pl < lo->planes; ++pl) h += __bfloat162float(lo->h[(pl * lo->rows_pad + row) * lo->cols + c]);
-    v = fmaf(h, __bfloat162float(lo->up[(int64_t)col * lo->adapters * lo->rank + c]), v);
+    v = fmaf(h, u, v);
   }
   return v;
 }
 
-__device__ __forceinline__ void lora_add_slow(const LoraPlan* lo, const uint32_t* bad, float* v, int row, int col0, int M) {
+__device__ __forceinline__ void lora_add_slow(const LoraPlan* lo, float* v, int row, int col0, int M) {
   if (row >= M) return;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] += lora_slow_value(lo, bad, row, col0 + i);
+  for (int i = 0; i < 32; ++i) v[i] += lora_slow_value(lo, row, col0 + i);
 }
 
 // The fp32 residual epilogue of one tile for the epilogue warp on lane quarter `quad` that takes
@@ -268,9 +270,8 @@ __device__ __forceinline__ void lora_add_slow(const LoraPlan* lo, const uint32_t
 // both free of bank conflicts.  The arithmetic per element is gemm_epilogue_chunk's (bias add,
 // then r + v * g for GATE_RES, v + r for RES), so both paths give the same bits.
 template <int EPI, bool LORA>
-__device__ __forceinline__ void residual_tile_staged(const GemmArgs& a, const LoraPlan* lora, const uint32_t* slow,
-                                                     float* stg, uint32_t t_row, int m0, int n0, int quad, int half,
-                                                     int lane) {
+__device__ __forceinline__ void residual_tile_staged(const GemmArgs& a, const LoraPlan* lora, bool slow, float* stg,
+                                                     uint32_t t_row, int m0, int n0, int quad, int half, int lane) {
   const int sub = lane >> 3, cg = lane & 7;
   const int rbase = m0 + quad * 32 + sub;  // the row of i = 0; a lane's rows step by 4
   int fr[8];
@@ -303,7 +304,7 @@ __device__ __forceinline__ void residual_tile_staged(const GemmArgs& a, const Lo
     float v[32];
     tmem_ld32(t_row + c * 32, v);
     if constexpr (LORA) {
-      if (slow) lora_add_slow(lora, slow, v, m0 + quad * 32 + lane, col0, a.M);
+      if (slow) lora_add_slow(lora, v, m0 + quad * 32 + lane, col0, a.M);
     }
 #pragma unroll
     for (int q = 0; q < 8; ++q)
@@ -375,7 +376,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       mbar_init(empty0 + 8 * s, 1);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(tfull0 + 8 * b, 1);
+      mbar_init(tfull0 + 8 * b, LORA ? 2 : 1);  // LORA: the MMA commit, and its thread once tile_bad is written
       mbar_init(tempty0 + 8 * b, 32 * G_EPI_WARPS);
     }
     mbar_init(done_bar, 1);
@@ -390,17 +391,19 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
     tmem_alloc(smem_u32(tmem_slot), G_TMEM_COLS);
     tmem_relinquish();
   }
-  __shared__ uint32_t lora_bad[LORA ? LORA_MASK_WORDS : 1];  // steps left to the epilogue
+  // LORA: u_ok[stage] says that the stage's up-projection tile was looked through; bad[stage] by
+  // which of the two checking warps found something; tile_bad: the tile of an accumulator had some
+  __shared__ uint64_t lora_ok_bar[LORA ? 2 * G_MAX_STAGES : 1];  // u_ok, u_req
+  __shared__ int lora_bad[LORA ? 2 * G_MAX_STAGES : 1];
+  __shared__ int lora_tile_bad[LORA ? 2 : 1];
+  const uint32_t u_ok0 = smem_u32(lora_ok_bar), u_req0 = u_ok0 + 8 * G_MAX_STAGES;
   if constexpr (LORA) {
-    if (warp == 2) {
-      for (int i = 0; i < LORA_MASK_WORDS; ++i) {
-        const int step = 32 * i + lane;
-        int bad = 0;
-        if (step < lora->steps)
-          for (int s = 0; s < LORA_SCAN; ++s) bad |= __ldg(lora->bad + step * LORA_SCAN + s);
-        const uint32_t word = __ballot_sync(0xffffffffu, bad != 0);
-        if (lane == 0) lora_bad[i] = word;
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < GSTAGES; ++i) {
+        mbar_init(u_ok0 + 8 * i, 2);
+        mbar_init(u_req0 + 8 * i, 1);
       }
+      fence_mbar_init();
     }
   }
   tc_fence_before();
@@ -439,9 +442,10 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
           }
         }
         if constexpr (LORA) {
+          pdl_wait();  // h and the step bits come from the launch before, which runs beside this K loop
           const uint32_t* mask = lora->step_mask + m0 / GBM * LORA_MASK_WORDS;
           for (int c = 0; ok && c < lora->cols / LORA_CHUNK; ++c) {
-            if (!lora_chunk_steps(mask, lora_bad, c)) continue;
+            if (!lora_chunk_steps(mask, c)) continue;
             for (int pl = 0; pl < lora->planes; ++pl) {
               if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, abort_flag, err, kErrTimeoutGemmProducer)) {
                 ok = false;
@@ -451,6 +455,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
               mbar_expect_tx(full0 + 8 * stage, G_A_BYTES + bn * GBK * 2);
               tma_load_2d(a_dst, tmH, full0 + 8 * stage, c * LORA_CHUNK, (int)(pl * lora->rows_pad) + m0);
               tma_load_2d(a_dst + G_A_BYTES, tmU, full0 + 8 * stage, c * LORA_CHUNK, n0);
+              mbar_arrive(u_req0 + 8 * stage);
               issued |= 1u << stage;
               last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
               if (++stage == GSTAGES) {
@@ -471,6 +476,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       const uint32_t idesc = idesc_bf16_f32(GBM, bn, false, false);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
+      [[maybe_unused]] uint32_t u_ok_ph = 0;  // phase of u_ok per stage
       bool ok = true;
       for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
         if (!mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag, err, kErrTimeoutGemmMma)) break;
@@ -496,17 +502,21 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
           }
         }
         if constexpr (LORA) {
-          int m0, n0;
+          int m0, n0, bad = 0;
           tile_origin(tile, num_m, num_n, bn, m0, n0);
+          pdl_wait();
           const uint32_t* mask = lora->step_mask + m0 / GBM * LORA_MASK_WORDS;
           for (int c = 0; ok && c < lora->cols / LORA_CHUNK; ++c) {
-            const uint32_t steps = lora_chunk_steps(mask, lora_bad, c);
+            const uint32_t steps = lora_chunk_steps(mask, c);
             if (!steps) continue;
             for (int pl = 0; pl < lora->planes; ++pl) {
-              if (!mbar_wait(full0 + 8 * stage, phase, abort_flag, err, kErrTimeoutGemmMma)) {
+              if (!mbar_wait(full0 + 8 * stage, phase, abort_flag, err, kErrTimeoutGemmMma) ||
+                  !mbar_wait(u_ok0 + 8 * stage, (u_ok_ph >> stage) & 1, abort_flag, err, kErrTimeoutGemmMma)) {
                 ok = false;
                 break;
               }
+              u_ok_ph ^= 1u << stage;
+              bad |= lora_bad[2 * stage] | lora_bad[2 * stage + 1];
               tc_fence_after();
               const uint32_t a_addr = tiles + stage * SB;
               const uint32_t b_addr = a_addr + G_A_BYTES;
@@ -522,8 +532,10 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
               }
             }
           }
+          lora_tile_bad[acc] = bad;
         }
         if (!ok) break;
+        if constexpr (LORA) mbar_arrive(tfull0 + 8 * acc);
         umma_commit(tfull0 + 8 * acc);
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
@@ -531,6 +543,53 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       // every UMMA issued by this thread has completed once done_bar flips
       umma_commit(done_bar);
       mbar_drain(done_bar, 0, err);
+    }
+  } else if (LORA && warp >= 2 + G_EPI_WARPS) {
+    // Two warps look through the up-projection tiles: h = 0 keeps a row clear of another adapter's
+    // finite weights, but 0 * NaN does not, so non-finite weights are zeroed before the MMA and added
+    // by the epilogue to the rows whose adapter has them.  The producer announces each such stage
+    // (u_req), so these warps pass over the others without a wait: its phases move only with the
+    // stages they handle, and neither they nor `full` can get a phase ahead before u_ok is given.
+    if constexpr (LORA) {
+      int load = 0;         // stage loads before this point
+      uint32_t req_ph = 0;  // phase of u_req per stage
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
+        int m0, n0;
+        tile_origin(tile, num_m, num_n, bn, m0, n0);
+        load += kblocks;
+        pdl_wait();
+        const uint32_t* mask = lora->step_mask + m0 / GBM * LORA_MASK_WORDS;
+        for (int c = 0; ok && c < lora->cols / LORA_CHUNK; ++c) {
+          if (!lora_chunk_steps(mask, c)) continue;
+          for (int pl = 0; pl < lora->planes; ++pl, ++load) {
+            const int stage = load % GSTAGES;
+            ok = mbar_wait_warp(u_req0 + 8 * stage, (req_ph >> stage) & 1, abort_flag, err, kErrTimeoutGemmProducer) &&
+                 mbar_wait_warp(full0 + 8 * stage, (load / GSTAGES) & 1, abort_flag, err, kErrTimeoutGemmProducer);
+            if (!ok) break;
+            req_ph ^= 1u << stage;
+            uint8_t* u = smem + (size_t)stage * SB + G_A_BYTES;
+            int hit = 0;
+            for (int r = (warp & 1) * 32 + lane; r < bn; r += 64) {
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {  // 16-byte groups in an order that spreads a quarter-warp over the banks
+                uint4* pq = reinterpret_cast<uint4*>(u + r * 128 + (((q + lane) & 7) << 4));
+                const uint4 v = *pq;
+                if (nonfinite_bf16x2(v.x) | nonfinite_bf16x2(v.y) | nonfinite_bf16x2(v.z) | nonfinite_bf16x2(v.w)) {
+                  *pq = make_uint4(zero_nonfinite(v.x), zero_nonfinite(v.y), zero_nonfinite(v.z), zero_nonfinite(v.w));
+                  hit = 1;
+                }
+              }
+            }
+            if (hit) fence_proxy_async_smem();
+            hit = __any_sync(0xffffffffu, hit);
+            if (lane == 0) {
+              lora_bad[2 * stage + (warp & 1)] = hit;
+              mbar_arrive(u_ok0 + 8 * stage);
+            }
+          }
+        }
+      }
     }
   } else {
     const int quad = warp & 3;
@@ -545,13 +604,8 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       tile_origin(tile, num_m, num_n, bn, m0, n0);
       const int row = m0 + r;
       const uint32_t t_row = tmem_base + (uint32_t(quad * 32) << 16) + acc * GBN;
-      const uint32_t* slow = nullptr;  // the bad steps, where a row of this tile uses one of them
-      if constexpr (LORA) {
-        const uint32_t* mask = lora->step_mask + m0 / GBM * LORA_MASK_WORDS;
-        uint32_t any = 0;
-        for (int i = 0; i < LORA_MASK_WORDS; ++i) any |= __ldg(mask + i) & lora_bad[i];
-        if (any) slow = lora_bad;
-      }
+      bool slow = false;
+      if constexpr (LORA) slow = *reinterpret_cast<volatile int*>(lora_tile_bad + acc) != 0;
       if constexpr (EPI == WANB200_EPI_SCATTER) {
         // stage this warp's 32 rows (lane = row), then write each row as one 512-byte segment
         // (the first warp of each lane quarter does the whole tile; the second only arrives)
@@ -605,7 +659,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
           float v[32];
           tmem_ld32(t_row + c * 32, v);
           if constexpr (LORA) {
-            if (slow) lora_add_slow(lora, slow, v, row, col0, args.M);
+            if (slow) lora_add_slow(lora, v, row, col0, args.M);
           }
           gemm_epilogue_chunk<EPI>(args, v, row, col0, res_cur, gate_row);
         }
@@ -631,7 +685,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
 }
 
 template <int EPI>
-__global__ void __launch_bounds__(G_THREADS, 1)
+__global__ void __launch_bounds__(G_LORA_THREADS, 1)
     gemm_lora_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmU,
                      const GemmArgs args, const __grid_constant__ LoraPlan lora) {
@@ -653,8 +707,18 @@ static int launch_gemm_lora(const CUtensorMap& ta, const CUtensorMap& tb, const 
     attr_set[dev].store(true, std::memory_order_release);
   }
   const int smem = (int)ga.tiles_bytes + GemmCfg<EPI>::FIXED + ga.res_staging;
-  gemm_lora_kernel<EPI><<<grid, G_THREADS, smem, st>>>(ta, tb, th, tu, ga, lora);
-  cudaError_t e = cudaGetLastError();
+  // programmatic dependence: starts while the down-projection runs; pdl_wait() above waits for it
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(G_LORA_THREADS);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_lora_kernel<EPI>, ta, tb, th, tu, ga, lora);
   if (e != cudaSuccess) return set_cuda_error("gemm_lora_kernel launch", e);
   return WANB200_OK;
 }

@@ -1,123 +1,255 @@
 // Low-rank adapters of many requests beside one projection:
 //   y = epilogue(x W^T + bias + s_id (x A_id^T) B_id^T),  id = ids[row], none where id < 0.
-// Two launches: this file's kernel forms h = s_id x A_id^T for every row into the columns of its
+// More than 16 rows: lora_down_kernel forms h = s_id x A_id^T for every row into the columns of its
 // adapter, zero in the other columns that the row's 128-row tile uses, and the GEMM (gemm.cu) runs
 // those columns as further K steps: acc += h . B^T with B as stored [N, adapters * rank].  A
 // tile multiplies only the 16-column steps that one of its rows uses, so sorted requests cost one
 // adapter's rank per tile and interleaved ones the ranks that really occur in it.
+// Up to 16 rows: reading W once bounds the call, and two small kernels stream it.
+#include <atomic>
+
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "lora.h"
 
 namespace wanb200 {
 
+namespace cg = cooperative_groups;
+
+constexpr int LD_THREADS = 192;  // TMA, MMA, 4 epilogue warps
+constexpr int LD_BM = 128, LD_BK = 64, LD_GROUP = 4;  // chunks of one pass: N = 256
+constexpr int LD_STAGES = 4;
+constexpr int LD_STAGE_BYTES = LD_BM * LD_BK * 2 + LD_GROUP * LORA_CHUNK * LD_BK * 2;  // 48 KB
+constexpr int LD_RED_LD = LD_GROUP * LORA_CHUNK + 4;  // fp32 row of the partial sums, padded against bank conflicts
+constexpr int LD_SMEM = LD_STAGES * LD_STAGE_BYTES + 1024;
+static_assert(LD_BM * LD_RED_LD * 4 <= LD_STAGES * LD_STAGE_BYTES, "the partial sums reuse the ring");
+
 struct LoraDownArgs {
-  const __nv_bfloat16* x;
-  int64_t ldx;
-  int M, N, K;
-  const __nv_bfloat16* down;  // [adapters * rank, K]
-  const __nv_bfloat16* up;    // [N, adapters * rank]
+  int M, K;
   const float* scales;
   const int32_t* ids;
-  int adapters, rank, cols, steps, planes;
+  int adapters, rank, cols, planes, kblocks_per_rank;
   int64_t rows_pad;
   uint32_t* step_mask;
-  int* bad;
   __nv_bfloat16* h;
-  int num_m;
   int* err;
 };
 
-__device__ __forceinline__ int lora_id(const LoraDownArgs& a, int row) {
-  const int id = __ldg(a.ids + row);
-  if (id >= a.adapters) atomicCAS(a.err, 0, kErrBadAdapter);
-  return id >= 0 && id < a.adapters ? id : -1;
+__device__ __forceinline__ uint2 bf16x4(const float4& v) { return make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w)); }
+
+// Four adjacent columns of a row of h: the row's adapter's columns scaled, zeros elsewhere (selected,
+// so a NaN of another adapter's product goes no further), rounded to bf16 -- the operand type of the
+// MMA that takes them; for an fp32 output a second plane holds what the rounding left.
+__device__ __forceinline__ void lora_store_h(const LoraDownArgs& a, int row, int col, float4 v, int first, int last, float scale) {
+  v.x = col >= first && col < last ? v.x * scale : 0.f;
+  v.y = col + 1 >= first && col + 1 < last ? v.y * scale : 0.f;
+  v.z = col + 2 >= first && col + 2 < last ? v.z * scale : 0.f;
+  v.w = col + 3 >= first && col + 3 < last ? v.w * scale : 0.f;
+  __nv_bfloat16* hp = a.h + (int64_t)row * a.cols + col;
+  const uint2 hi = bf16x4(v);
+  *reinterpret_cast<uint2*>(hp) = hi;
+  if (a.planes > 1) {
+    float4 r;
+    r.x = v.x - __uint_as_float(hi.x << 16);
+    r.y = v.y - __uint_as_float(hi.x & 0xffff0000u);
+    r.z = v.z - __uint_as_float(hi.y << 16);
+    r.w = v.w - __uint_as_float(hi.y & 0xffff0000u);
+    // an infinite h has no remainder
+    r.x = isfinite(r.x) ? r.x : 0.f, r.y = isfinite(r.y) ? r.y : 0.f;
+    r.z = isfinite(r.z) ? r.z : 0.f, r.w = isfinite(r.w) ? r.w : 0.f;
+    *reinterpret_cast<uint2*>(hp + a.rows_pad * a.cols) = bf16x4(r);
+  }
 }
 
-// Blocks 0 .. num_m - 1: the step bits of a row tile.  The others: one (step, slice of N) each, a
-// scan of the step's `up` columns for values that are not finite.  h = 0 keeps a row clear of
-// another adapter's finite values, but 0 * NaN does not, so the GEMM leaves such steps out and its
-// epilogue adds them to the rows that use them one by one.
-__global__ void __launch_bounds__(128) lora_plan_kernel(const LoraDownArgs a) {
-  if ((int)blockIdx.x < a.num_m) {
-    __shared__ uint32_t bits[LORA_MASK_WORDS];
-    if (threadIdx.x < LORA_MASK_WORDS) bits[threadIdx.x] = 0u;
-    __syncthreads();
-    const int row = blockIdx.x * 128 + threadIdx.x;
-    const int id = row < a.M ? lora_id(a, row) : -1;
+// One cluster per 128-row tile, its blocks sharing K (one block where there are row tiles enough to
+// fill the SMs): x tile x the tile's used chunks of A, up to four (N = 256) in one pass over x.  The
+// read of x bounds it; with few row tiles the split of K brings enough SMs to the read.  The
+// partial sums meet in the cluster's shared memory, each block adding its share of the rows.
+__global__ void __launch_bounds__(LD_THREADS, 1)
+    lora_down_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmD,
+                     const __grid_constant__ LoraDownArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t bars[2 * LD_STAGES + 3];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  __shared__ uint32_t bits[LORA_MASK_WORDS];
+  __shared__ int ids[LD_BM];
+  __shared__ int chunks[LORA_MAX_COLS / LORA_CHUNK];
+  __shared__ int num_chunks;
+  pdl_launch();  // the GEMM behind starts its own K loop; it waits for this kernel before it reads h
+  cg::cluster_group cluster = cg::this_cluster();
+  const int krank = blockIdx.x, ksize = gridDim.x, m0 = blockIdx.y * LD_BM;
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * LD_STAGES, tfull = empty0 + 8 * LD_STAGES;
+  const uint32_t tempty = tfull + 8, done_bar = tfull + 16;
+  volatile int* abort_flag = &abort_word;
+  int* err = a.err;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x < LORA_MASK_WORDS) bits[threadIdx.x] = 0u;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < LD_STAGES; ++s) {
+      mbar_init(full0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    mbar_init(tfull, 1);
+    mbar_init(tempty, 128);
+    mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmD);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&tmem_slot), LD_GROUP * LORA_CHUNK);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  if (threadIdx.x < LD_BM) {
+    const int row = m0 + threadIdx.x;
+    int id = row < a.M ? __ldg(a.ids + row) : -1;
+    if (id >= a.adapters) {
+      atomicCAS(a.err, 0, kErrBadAdapter);
+      id = -1;
+    }
+    ids[threadIdx.x] = id;
     if (id >= 0)
       for (int s = id * a.rank / LORA_STEP; s * LORA_STEP < (id + 1) * a.rank; ++s) atomicOr(bits + (s >> 5), 1u << (s & 31));
-    __syncthreads();
-    if (threadIdx.x < LORA_MASK_WORDS) a.step_mask[blockIdx.x * LORA_MASK_WORDS + threadIdx.x] = bits[threadIdx.x];
-    return;
   }
-  const int unit = blockIdx.x - a.num_m, step = unit / LORA_SCAN, slice = unit % LORA_SCAN;
-  const int c0 = step * LORA_STEP, c1 = min(c0 + LORA_STEP, a.adapters * a.rank);
-  int used = 0, bad = 0;
-  for (int row = threadIdx.x; row < a.M && !used; row += 128) {
-    const int id = __ldg(a.ids + row);
-    used = id >= 0 && id < a.adapters && id * a.rank < c1 && (id + 1) * a.rank > c0;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (threadIdx.x < LORA_MASK_WORDS && krank == 0)
+    a.step_mask[blockIdx.y * LORA_MASK_WORDS + threadIdx.x] = bits[threadIdx.x];
+  if (threadIdx.x == 0) {
+    int n = 0;
+    for (int c = 0; c < a.cols / LORA_CHUNK; ++c)
+      if ((bits[c >> 3] >> ((c & 7) * 4)) & 0xfu) chunks[n++] = c;
+    num_chunks = n;
   }
-  if (__syncthreads_or(used)) {
-    const int n1 = min(a.N, (slice + 1) * ((a.N + LORA_SCAN - 1) / LORA_SCAN));
-    for (int n = slice * ((a.N + LORA_SCAN - 1) / LORA_SCAN) + threadIdx.x; n < n1; n += 128) {
-      const uint4* p = reinterpret_cast<const uint4*>(a.up + (int64_t)n * a.adapters * a.rank + c0);
-      for (int q = 0; q < (c1 - c0) / 8; ++q) {
-        const uint4 u = __ldg(p + q);
-        bad |= nonfinite_bf16x2(u.x) | nonfinite_bf16x2(u.y) | nonfinite_bf16x2(u.z) | nonfinite_bf16x2(u.w);
+  __syncthreads();
+  const uint32_t tmem_base = tmem_slot;
+  const int kb0 = krank * a.kblocks_per_rank, kblocks = min(a.K / LD_BK - kb0, a.kblocks_per_rank);  // >= 1 (host)
+  const int passes = (num_chunks + LD_GROUP - 1) / LD_GROUP;
+  uint32_t ph = 0, issued = 0, last_ph = 0;  // ring phases, per role
+  int stage = 0;
+
+  for (int pass = 0; pass < passes; ++pass) {
+    const int c0 = pass * LD_GROUP, nc = min(LD_GROUP, num_chunks - c0);
+    if (warp == 0) {
+      if (lane == 0) {
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!mbar_wait(empty0 + 8 * stage, ph ^ 1, abort_flag, err, kErrTimeoutGemmProducer)) break;
+          const uint32_t dst = sbase + stage * LD_STAGE_BYTES;
+          mbar_expect_tx(full0 + 8 * stage, LD_BM * LD_BK * 2 + nc * LORA_CHUNK * LD_BK * 2);
+          tma_load_2d(dst, &tmX, full0 + 8 * stage, (kb0 + kb) * LD_BK, m0);
+          for (int c = 0; c < nc; ++c)
+            tma_load_2d(dst + LD_BM * LD_BK * 2 + c * LORA_CHUNK * LD_BK * 2, &tmD, full0 + 8 * stage, (kb0 + kb) * LD_BK,
+                        chunks[c0 + c] * LORA_CHUNK);
+          issued |= 1u << stage;
+          last_ph = (last_ph & ~(1u << stage)) | (ph << stage);
+          if (++stage == LD_STAGES) stage = 0, ph ^= 1;
+        }
       }
+    } else if (warp == 1) {
+      if (lane == 0) {
+        const uint32_t idesc = idesc_bf16_f32(LD_BM, nc * LORA_CHUNK, false, false);
+        bool ok = mbar_wait(tempty, (pass & 1) ^ 1, abort_flag, err, kErrTimeoutGemmMma);
+        tc_fence_after();
+        for (int kb = 0; ok && kb < kblocks; ++kb) {
+          ok = mbar_wait(full0 + 8 * stage, ph, abort_flag, err, kErrTimeoutGemmMma);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t x_addr = sbase + stage * LD_STAGE_BYTES, d_addr = x_addr + LD_BM * LD_BK * 2;
+#pragma unroll
+          for (int kk = 0; kk < LD_BK / 16; ++kk)
+            umma_bf16(tmem_base, sw128_desc(x_addr + kk * 32, 16, 1024), sw128_desc(d_addr + kk * 32, 16, 1024), idesc,
+                      (kb | kk) != 0);
+          umma_commit(empty0 + 8 * stage);
+          if (++stage == LD_STAGES) stage = 0, ph ^= 1;
+        }
+        if (ok) umma_commit(tfull);
+      }
+    } else {
+      const int quad = warp & 3, r = quad * 32 + lane, row = m0 + r;
+      const int id = ids[r];
+      const int first = id < 0 ? 0 : id * a.rank, last = id < 0 ? 0 : first + a.rank;
+      const float scale = id >= 0 && a.scales ? __ldg(a.scales + id) : 1.f;
+      const bool ok = mbar_wait_warp(tfull, pass & 1, abort_flag, err, kErrTimeoutGemmEpilogue);
+      if (ok) {
+        tc_fence_after();
+        for (int c = 0; c < nc * 2; ++c) {
+          float v[32];
+          tmem_ld32(tmem_base + (uint32_t(quad * 32) << 16) + c * 32, v);
+          if (ksize == 1) {
+            if (row < a.M) {
+              const int col = chunks[c0 + (c >> 1)] * LORA_CHUNK + (c & 1) * 32;
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                lora_store_h(a, row, col + 4 * q, make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]), first, last,
+                             scale);
+            }
+          } else {  // the ring is free: every MMA of the pass has completed
+            float4* red = reinterpret_cast<float4*>(smem + (r * LD_RED_LD + c * 32) * 4);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) red[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          }
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(tempty);
+    }
+    if (ksize > 1) {
+      __syncwarp();
+      cluster.sync();
+      const int per = LD_BM / ksize, groups = nc * LORA_CHUNK / 4;
+      for (int i = threadIdx.x; i < per * groups; i += LD_THREADS) {
+        const int r = krank * per + i / groups, g = i % groups, row = m0 + r;
+        if (row >= a.M) continue;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < ksize; ++k) {  // in order, so that the sum is the same in every run
+          const float4 v = *cluster.map_shared_rank(reinterpret_cast<float4*>(smem + (r * LD_RED_LD + g * 4) * 4), k);
+          sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
+        const int id = ids[r];
+        lora_store_h(a, row, chunks[c0 + (g >> 4)] * LORA_CHUNK + (g & 15) * 4, sum, id < 0 ? 0 : id * a.rank,
+                     id < 0 ? 0 : (id + 1) * a.rank, id >= 0 && a.scales ? __ldg(a.scales + id) : 1.f);
+      }
+      fence_proxy_async_smem();  // the next pass's loads overwrite what was read and written here
+      cluster.sync();
     }
   }
-  bad = __syncthreads_or(bad);
-  if (threadIdx.x == 0) a.bad[unit] = bad;
+  if (warp == 0 && lane == 0 && *abort_flag) {  // let every load in flight land
+    for (int s = 0; s < LD_STAGES; ++s)
+      if ((issued >> s) & 1) mbar_drain(full0 + 8 * s, (last_ph >> s) & 1, err);
+  }
+  if (warp == 1 && lane == 0) {
+    umma_commit(done_bar);
+    mbar_drain(done_bar, 0, err);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem_base, LD_GROUP * LORA_CHUNK);
 }
 
-// One block per row, one warp per column of the tile's used steps.
-__global__ void __launch_bounds__(256) lora_down_rows_kernel(const LoraDownArgs a) {
-  const int row = blockIdx.x, lane = threadIdx.x & 31;
-  const int id = lora_id(a, row);
-  const float scale = id >= 0 && a.scales ? __ldg(a.scales + id) : 1.f;
-  const uint32_t* mask = a.step_mask + (row >> 7) * LORA_MASK_WORDS;
-  for (int c = threadIdx.x >> 5; c < a.cols; c += 8) {
-    if (!((__ldg(mask + (c >> 9)) >> ((c >> 4) & 31)) & 1u)) continue;
-    float v = 0.f;
-    if (id >= 0 && c >= id * a.rank && c < (id + 1) * a.rank) {
-      const uint4* xp = reinterpret_cast<const uint4*>(a.x + row * a.ldx);
-      const uint4* dp = reinterpret_cast<const uint4*>(a.down + (int64_t)c * a.K);
-      for (int k = lane; k < a.K / 8; k += 32) {
-        float f[8], g[8];
-        unpack_bf16x8(__ldg(xp + k), f);
-        unpack_bf16x8(__ldg(dp + k), g);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v = fmaf(f[i], g[i], v);
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      v *= scale;
-    }
-    if (lane == 0) {
-      __nv_bfloat16* hp = a.h + (int64_t)row * a.cols + c;
-      const __nv_bfloat16 hi = __float2bfloat16(v);
-      hp[0] = hi;
-      // the second plane keeps h's rounding out of an fp32 output
-      if (a.planes > 1) hp[a.rows_pad * a.cols] = __float2bfloat16(isfinite(v) ? v - __bfloat162float(hi) : 0.f);
-    }
-  }
-}
-
+// ------------------------------------------------------------------ host launcher
 struct LoraLayout {
-  int64_t rows_pad, num_m, bad_off, h_off, bytes;
-  int cols, steps, planes;
+  int64_t rows_pad, num_m, h_off, bytes;
+  int cols, planes;
 };
 
 static LoraLayout lora_layout(int64_t M, int adapters, int rank, int out_f32) {
   LoraLayout l;
-  l.num_m = (M + 127) / 128;
-  l.rows_pad = l.num_m * 128;
+  l.num_m = (M + LD_BM - 1) / LD_BM;
+  l.rows_pad = l.num_m * LD_BM;
   l.cols = (adapters * rank + LORA_CHUNK - 1) / LORA_CHUNK * LORA_CHUNK;
-  l.steps = (adapters * rank + LORA_STEP - 1) / LORA_STEP;
   l.planes = out_f32 ? 2 : 1;
-  l.bad_off = (l.num_m * LORA_MASK_WORDS * 4 + 255) / 256 * 256;
-  l.h_off = l.bad_off + (l.steps * LORA_SCAN * 4 + 255) / 256 * 256;
+  l.h_off = (l.num_m * LORA_MASK_WORDS * 4 + 255) / 256 * 256;
   l.bytes = l.h_off + l.planes * l.rows_pad * l.cols * 2;
   return l;
 }
@@ -136,7 +268,7 @@ int gemm_lora(const wanb200_lora_params* p, cudaStream_t st) {
   const wanb200_gemm_params* g = &p->gemm;
   if (g->epilogue == WANB200_EPI_SCATTER || g->epilogue == WANB200_EPI_BIAS_SUMSQ)
     return set_error(WANB200_EINVAL, "gemm_lora: the SCATTER and SUMSQ epilogues take no adapters");
-  const int rc = gemm_validate(g);
+  int rc = gemm_validate(g);
   if (rc) return rc;
   if (!lora_sizes_ok(g->M, p->adapters, p->rank))
     return set_error(WANB200_EINVAL, "gemm_lora: need adapters > 0, rank a positive multiple of 8, adapters * rank <= 4096");
@@ -145,44 +277,68 @@ int gemm_lora(const wanb200_lora_params* p, cudaStream_t st) {
   const LoraLayout l = lora_layout(g->M, p->adapters, p->rank, g->out_f32 != 0);
   if (!p->lora_workspace || (reinterpret_cast<uintptr_t>(p->lora_workspace) & 255u) || p->lora_workspace_bytes < l.bytes)
     return set_error(WANB200_EINVAL, "gemm_lora: need a 256-byte aligned workspace of wanb200_lora_workspace_bytes()");
+  if (l.num_m > 65535) return set_error(WANB200_EINVAL, "gemm_lora: too many rows");
   int* err = device_error_word();
   if (!err) return WANB200_ECUDA;
   uint8_t* ws = static_cast<uint8_t*>(p->lora_workspace);
+  CUtensorMap tx, td;
+  rc = make_tmap_2d(&tx, g->a, g->K, g->M, g->lda, LD_BK, LD_BM);
+  if (rc) return rc;
+  rc = make_tmap_2d(&td, p->down, g->K, (int64_t)p->adapters * p->rank, g->K, LD_BK, LORA_CHUNK);
+  if (rc) return rc;
   LoraDownArgs a;
-  a.x = reinterpret_cast<const __nv_bfloat16*>(g->a);
-  a.ldx = g->lda;
   a.M = (int)g->M;
-  a.N = (int)g->N;
   a.K = (int)g->K;
-  a.down = reinterpret_cast<const __nv_bfloat16*>(p->down);
-  a.up = reinterpret_cast<const __nv_bfloat16*>(p->up);
   a.scales = p->scales;
   a.ids = p->ids;
   a.adapters = p->adapters;
   a.rank = p->rank;
   a.cols = l.cols;
-  a.steps = l.steps;
   a.planes = l.planes;
   a.rows_pad = l.rows_pad;
   a.step_mask = reinterpret_cast<uint32_t*>(ws);
-  a.bad = reinterpret_cast<int*>(ws + l.bad_off);
   a.h = reinterpret_cast<__nv_bfloat16*>(ws + l.h_off);
-  a.num_m = (int)l.num_m;
   a.err = err;
-  lora_plan_kernel<<<(unsigned)(l.num_m + l.steps * LORA_SCAN), 128, 0, st>>>(a);
-  lora_down_rows_kernel<<<(unsigned)g->M, 256, 0, st>>>(a);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return set_cuda_error("lora down-projection launch", e);
+  // blocks along K: as many as bring the row tiles to the SM count, at least 4 K blocks each
+  const int kblocks = a.K / LD_BK;
+  int ksize = 1;
+  while (ksize < 8 && l.num_m * ksize * 2 <= num_sms() && kblocks >= ksize * 2 * 4) ksize *= 2;
+  a.kblocks_per_rank = (kblocks + ksize - 1) / ksize;
+  while ((ksize - 1) * a.kblocks_per_rank >= kblocks) {  // no block without work
+    ksize /= 2;
+    a.kblocks_per_rank = (kblocks + ksize - 1) / ksize;
+  }
+  static std::atomic<bool> attr_set[kMaxDevices] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= kMaxDevices) return set_error(WANB200_EINVAL, "device index out of range");
+  cudaError_t e;
+  if (!attr_set[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(lora_down_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LD_SMEM);
+    if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute(lora_down)", e);
+    attr_set[dev].store(true, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ksize, (unsigned)l.num_m);
+  cfg.blockDim = dim3(LD_THREADS);
+  cfg.dynamicSmemBytes = LD_SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ksize;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, lora_down_kernel, tx, td, a);
+  if (e != cudaSuccess) return set_cuda_error("lora_down_kernel launch", e);
   LoraPlan plan;
   plan.step_mask = a.step_mask;
-  plan.bad = a.bad;
   plan.h = a.h;
-  plan.up = a.up;
+  plan.up = reinterpret_cast<const __nv_bfloat16*>(p->up);
   plan.ids = a.ids;
   plan.adapters = a.adapters;
   plan.rank = a.rank;
   plan.cols = a.cols;
-  plan.steps = a.steps;
   plan.planes = a.planes;
   plan.rows_pad = a.rows_pad;
   return gemm_launch(g, &plan, err, st);

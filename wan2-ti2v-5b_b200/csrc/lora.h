@@ -1,5 +1,5 @@
-// Low-rank adapters beside a projection: what lora.cu (the down-projection and the plan) hands to
-// the GEMM (gemm.cu), which adds the up-projection to its accumulators.
+// Low-rank adapters beside a projection: what lora.cu (the down-projection) hands to the GEMM
+// (gemm.cu), which adds the up-projection to its accumulators.
 #pragma once
 
 #include "internal.h"
@@ -10,16 +10,14 @@ namespace wanb200 {
 // the K of one tcgen05.mma, and loaded in chunks of 64, one 128-byte swizzle row.
 constexpr int LORA_STEP = 16, LORA_CHUNK = 64, LORA_MAX_COLS = 4096;
 constexpr int LORA_MASK_WORDS = LORA_MAX_COLS / LORA_STEP / 32;  // 8 words of step bits per row tile
-constexpr int LORA_SCAN = 8;  // slices of N that the scan for non-finite `up` values is split into
 
-// Workspace of one call: [row tiles][8] step bits | [steps][LORA_SCAN] scan flags | h planes.
+// Workspace of one call: [row tiles][8] step bits | h planes.
 struct LoraPlan {
   const uint32_t* step_mask;  // steps that some row of the tile uses
-  const int* bad;             // != 0: the step's `up` columns hold a NaN or an infinity in this slice
   const __nv_bfloat16* h;     // [planes][rows_pad][cols]: scale * (x . down^T) in bf16 planes that add up
   const __nv_bfloat16* up;    // [N][adapters * rank]
   const int32_t* ids;
-  int adapters, rank, cols, steps, planes;
+  int adapters, rank, cols, planes;
   int64_t rows_pad;
 };
 

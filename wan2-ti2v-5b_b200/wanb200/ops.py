@@ -6,7 +6,6 @@ library or a non-CUDA tensor raises.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 
@@ -391,26 +390,40 @@ def bias_gate_residual(residual, y, bias, gate=None, frames=None, out=None, nsum
 
 
 # ---------------------------------------------------------------------------- packed request batches
-def _same_device(*ts):
-    """All tensors on one CUDA device, which is returned."""
-    _cuda(*ts)
-    devs = {t.device for t in ts if t is not None}
-    _need(len(devs) == 1, f"all tensors must be on one device, got {sorted(map(str, devs))}")
-    return devs.pop()
+# These calls also serve single tokens, where the host's share of a call counts: shapes and strides
+# are read once, the parameter struct is filled in one go.
+def _device_index(*ts):
+    """The index of the one CUDA device that holds all the tensors (None is skipped)."""
+    dev = -1
+    for t in ts:
+        if t is not None:
+            d = t.get_device()
+            if d < 0:
+                raise L.WanB200Error("libwanb200 ops need CUDA tensors (no CPU fallback)")
+            if d != dev:
+                _need(dev < 0, "all tensors must be on one device")
+                dev = d
+    return dev
 
 
-def _on(device):
-    """Context in which `device` is the current one (the library launches on the current device)."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _call(t, dev, kind, work, fn, params, what):
+    """One library call on `dev` (made current for it) and t's current stream."""
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return _call(t, dev, kind, work, fn, params, what)
+    ref = ctypes.byref(params)
+    rc = _launch(t, kind, work, lambda: fn(ref, torch._C._cuda_getCurrentRawStream(dev)))
+    if rc:
+        L.check(rc, what)
 
 
-def _overlap(a, b):
-    """Whether the memory that two tensors span overlaps."""
-    def span(t):
-        last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+def _row_major(t, name, what):
+    """(rows, columns, row stride) of a bf16 or fp32 matrix with unit column stride; the stride of a
+    single row, which is never used, is given as the columns."""
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] != 1):
+        raise ValueError(f"{what}: {name} must be 2-D with unit column stride")
+    (m, n), sm = t.shape, t.stride(0)
+    return m, n, sm if m != 1 else (n + 7) // 8 * 8
 
 
 def head_norm_rope(x, sections, head_dim, *, out=None, eps=1e-6, cos=None, sin=None, positions=None,
@@ -424,45 +437,41 @@ def head_norm_rope(x, sections, head_dim, *, out=None, eps=1e-6, cos=None, sin=N
     qk_norm_rope norms over the whole width instead and takes one sequence length.
 
     A position outside 0..P-1 leaves its row as it was and sets the device error word (501)."""
-    dev = _same_device(x, out, cos, sin, positions, *[g for _, _, g in sections])
-    out = x if out is None else out
-    for name, t in (("x", x), ("out", out)):
-        _need(t.dtype == BF16, f"head_norm_rope: {name} must be bf16")
-    ldx, ldo = _rows(x, "x"), _rows(out, "out")
-    M = x.shape[0]
-    _need(out.shape[0] == M, "head_norm_rope: out must have x's rows")
     _need(1 <= len(sections) <= 2, "head_norm_rope: one or two sections")
+    c0, h0, g0 = sections[0]
+    c1, h1, g1 = sections[1] if len(sections) == 2 else (0, 0, None)
+    dev = _device_index(x, out, cos, sin, positions, g0, g1)
+    M, cols, ldx = _row_major(x, "x", "head_norm_rope")
+    _need(x.dtype == BF16, "head_norm_rope: x must be bf16")
+    xp, op_, ldo = x.data_ptr(), x.data_ptr(), ldx
+    if out is None or out is x:
+        out = x
+    else:
+        mo, no, ldo = _row_major(out, "out", "head_norm_rope")
+        _need(out.dtype == BF16 and mo == M, "head_norm_rope: out must be bf16 with x's rows")
+        op_ = out.data_ptr()
+        _need((op_ == xp and ldo == ldx) or op_ >= xp + 2 * ((M - 1) * ldx + cols) or
+              xp >= op_ + 2 * ((M - 1) * ldo + no), "head_norm_rope: out must be x or not overlap it")
+        cols = min(cols, no)
     if M == 0:
         return out
-    same = out.data_ptr() == x.data_ptr() and ldx == ldo
-    _need(same or not _overlap(x, out), "head_norm_rope: out must be x or not overlap it")
-    p = L.HeadNormParams()
-    p.x, p.ldx, p.out, p.ldo, p.rows, p.nsections = _p(x), ldx, _p(out), ldo, M, len(sections)
-    p.head_dim, p.eps = head_dim, eps
-    vals = 0
-    for i, (c0, heads, g) in enumerate(sections):
-        _need(g is None or (g.dtype == BF16 and g.is_contiguous() and g.numel() == head_dim),
-              "head_norm_rope: gamma must be bf16 [head_dim]")
-        _need(heads > 0 and c0 >= 0 and c0 + heads * head_dim <= min(x.shape[1], out.shape[1]),
-              "head_norm_rope: a section lies outside the columns of x or out")
-        p.col0[i], p.heads[i], p.gamma[i] = c0, heads, _p(g)
-        vals += M * heads * head_dim
-    if M == 1:  # a single row's stride is never used; torch may report any
-        p.ldx = p.ldo = max(ldx, ldo, *[c0 + heads * head_dim for c0, heads, _ in sections]) + 7 & ~7
+    for c, h, g in sections:
+        _need(h > 0 and c >= 0 and c + h * head_dim <= cols, "head_norm_rope: a section lies outside the columns of x or out")
+        _need(g is None or (g.dtype == BF16 and g.shape == (head_dim,) and g.is_contiguous()),
+              f"head_norm_rope: gamma must be contiguous bf16 [{head_dim}]")
+    P = rot = 0
     _need((cos is None) == (sin is None), "head_norm_rope: cos and sin come together")
     if cos is not None:
         _need(cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.dim() == 2 and cos.shape == sin.shape and
               cos.is_contiguous() and sin.is_contiguous(), "head_norm_rope: cos / sin must be contiguous fp32 [P, rot / 2]")
-        p.cos, p.sin, p.table_rows, p.rot, p.interleaved = _p(cos), _p(sin), cos.shape[0], 2 * cos.shape[1], int(interleaved)
+        P, rot = cos.shape
     if positions is not None:
         _need(cos is not None, "head_norm_rope: positions need cos / sin")
-        _need(positions.dtype == torch.int32 and positions.is_contiguous() and positions.numel() == M,
-              "head_norm_rope: positions must be int32 [M]")
-        p.positions = _p(positions)
-    lib = L.load()
-    with _on(dev):
-        L.check(_launch(x, kind, 4.0 * vals, lambda: lib.wanb200_head_norm_rope(ctypes.byref(p), _stream(x))),
-                "wanb200_head_norm_rope")
+        _need(positions.dtype == torch.int32 and positions.shape == (M,) and positions.is_contiguous(),
+              "head_norm_rope: positions must be contiguous int32 [M]")
+    p = L.HeadNormParams(xp, ldx, op_, ldo, M, len(sections), (c0, c1), (h0, h1), (_p(g0), _p(g1)), head_dim, eps,
+                         2 * rot, interleaved, _p(cos), _p(sin), _p(positions), P)
+    _call(x, dev, kind, 4.0 * M * (h0 + h1) * head_dim, L.load().wanb200_head_norm_rope, p, "wanb200_head_norm_rope")
     return out
 
 
@@ -475,62 +484,67 @@ def range_attention(q, k, v, lo, hi, *, pos=None, out=None, softmax_scale=None, 
     dist_bias [H, 2R + 1] fp32: bias dist_bias[h, clamp(j - pos, -R, R) + R]; pos defaults to the
     row index.  lo, hi and pos are read on the device at every call, so a captured graph follows
     them.  wanb200.ranges has the common masks (packed documents, caches)."""
-    dev = _same_device(q, k, v, lo, hi, pos, out, slopes, dist_bias)
-    for name, t in (("q", q), ("k", k), ("v", v)) + ((("out", out),) if out is not None else ()):
-        _need(t.dtype == BF16 and t.dim() == 4, f"range_attention: {name} must be bf16 [B, L, H, D]")
+    dev = _device_index(q, k, v, lo, hi, pos, out, slopes, dist_bias)
+    _need(q.dim() == 4 and k.dim() == 4, "range_attention: q, k and v must be [B, L, H, D]")
     B, Lq, H, D = q.shape
-    Lk, Hkv = k.shape[1], k.shape[2]
-    _need(k.shape[0] == B and k.shape[3] == D and v.shape == k.shape, "range_attention: q/k/v shape mismatch")
-    _need(D in (64, 128), "range_attention: head_dim must be 64 or 128")
+    Bk, Lk, Hkv, Dk = k.shape
+    _need(Bk == B and Dk == D and v.shape == k.shape, "range_attention: q/k/v shape mismatch")
+    _need(D == 128 or D == 64, "range_attention: head_dim must be 64 or 128")
     _need(Hkv > 0 and H % Hkv == 0, "range_attention: the query heads must be a multiple of the key heads")
     if out is None:
         out = torch.empty(B, Lq, H, D, dtype=BF16, device=q.device)
-    _need(out.shape == q.shape, "range_attention: out must have q's shape")
-    if out.numel() == 0:
+        fresh = True
+    else:
+        _need(out.shape == q.shape, "range_attention: out must have q's shape")
+        fresh = False
+
+    def layout(t, name, n, h):
+        """(address, token stride, batch stride); the stride of a dimension of one is never used."""
+        sb, st, sh, sd = t.stride()
+        if t.dtype != BF16 or sd != 1 or (h != 1 and sh != D):
+            raise ValueError(f"range_attention: {name} must be bf16 with head stride {D}")
+        if n == 1:
+            st = h * D
+        return t.data_ptr(), st, sb if B > 1 else n * st
+
+    if B * Lq * H == 0:
         return out
     if Lk == 0:
         return out.zero_()
-
-    def strides(t, name):
-        b, n, h, _ = t.shape
-        _need(t.stride(3) == 1 and (h == 1 or t.stride(2) == D), f"range_attention: {name} must have head stride {D}")
-        tok = t.stride(1) if n > 1 else h * D  # the stride of a dimension of one is never used
-        return tok, t.stride(0) if b > 1 else n * tok
-
-    p = L.RangeAttnParams()
-    p.q, (p.q_tok_stride, p.q_batch_stride) = _p(q), strides(q, "q")
-    p.k, (p.k_tok_stride, p.k_batch_stride) = _p(k), strides(k, "k")
-    p.v, (p.v_tok_stride, p.v_batch_stride) = _p(v), strides(v, "v")
-    p.o, (p.o_tok_stride, p.o_batch_stride) = _p(out), strides(out, "out")
-    p.batch, p.heads, p.kv_heads, p.q_len, p.kv_len, p.head_dim = B, H, Hkv, Lq, Lk, D
-    p.softmax_scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)
-    p.softcap = softcap
-    for name, t in (("lo", lo), ("hi", hi), ("pos", pos)):
-        _need(t is None or (t.dtype == torch.int32 and t.is_contiguous() and t.shape == lo.shape and
-                            t.shape in ((Lq,), (1, Lq), (B, Lq))),
-              f"range_attention: {name} must be contiguous int32 [Lq] or [B, Lq], all of one shape")
-    p.lo, p.hi, p.pos = _p(lo), _p(hi), _p(pos)
-    p.range_batch_stride = Lq if lo.dim() == 2 and lo.shape[0] == B and B > 1 else 0
-    _need(slopes is None or dist_bias is None, "range_attention: slopes or dist_bias, not both")
+    qa, ka, va = layout(q, "q", Lq, H), layout(k, "k", Lk, Hkv), layout(v, "v", Lk, Hkv)
+    oa = layout(out, "out", Lq, H)
+    if not fresh:
+        def end(a, n, h):
+            return a[0] + 2 * ((B - 1) * a[2] + (n - 1) * a[1] + h * D)
+        oe = end(oa, Lq, H)
+        for a, n, h in ((qa, Lq, H), (ka, Lk, Hkv), (va, Lk, Hkv)):
+            _need(oa[0] >= end(a, n, h) or a[0] >= oe, "range_attention: out must not overlap q, k or v")
+    shape = lo.shape
+    _need(shape == (Lq,) or shape == (B, Lq) or shape == (1, Lq), "range_attention: lo must be [Lq] or [B, Lq]")
+    for t, name in ((lo, "lo"), (hi, "hi"), (pos, "pos")):
+        if t is not None and (t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous()):
+            raise ValueError(f"range_attention: {name} must be contiguous int32, lo, hi and pos of one shape")
+    reach = 0
     if slopes is not None:
-        _need(slopes.dtype == torch.float32 and slopes.is_contiguous() and slopes.shape == (H,),
+        _need(dist_bias is None, "range_attention: slopes or dist_bias, not both")
+        _need(slopes.dtype == torch.float32 and slopes.shape == (H,) and slopes.is_contiguous(),
               "range_attention: slopes must be contiguous fp32 [H]")
-        p.slopes = _p(slopes)
-    if dist_bias is not None:
-        _need(dist_bias.dtype == torch.float32 and dist_bias.is_contiguous() and dist_bias.dim() == 2 and
+    elif dist_bias is not None:
+        _need(dist_bias.dtype == torch.float32 and dist_bias.dim() == 2 and dist_bias.is_contiguous() and
               dist_bias.shape[0] == H and dist_bias.shape[1] % 2 == 1,
               "range_attention: dist_bias must be contiguous fp32 [H, 2R + 1]")
-        p.dist_bias, p.reach = _p(dist_bias), dist_bias.shape[1] // 2
-    _need(not any(_overlap(out, t) for t in (q, k, v)), "range_attention: out must not overlap q, k or v")
+        reach = dist_bias.shape[1] // 2
+    p = L.RangeAttnParams(*qa, *ka, *va, *oa, B, H, Hkv, Lq, Lk, D,
+                          softmax_scale if softmax_scale is not None else D ** -0.5, softcap, lo.data_ptr(),
+                          hi.data_ptr(), _p(pos), Lq if B > 1 and len(shape) == 2 and shape[0] == B else 0, _p(slopes),
+                          _p(dist_bias), reach)
     lib = L.load()
-    with _on(dev):
-        nbytes = lib.wanb200_range_attn_workspace_bytes(ctypes.byref(p))
-        if nbytes:  # from torch's allocator: ordered on this stream, and a captured graph's own
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            p.workspace, p.workspace_bytes = _p(ws), nbytes
-        # the work in the launch record is that of the full rectangle; the ranges are on the device
-        L.check(_launch(q, kind, 4.0 * B * H * Lq * Lk * D,
-                        lambda: lib.wanb200_range_attn_fwd(ctypes.byref(p), _stream(q))), "wanb200_range_attn_fwd")
+    nbytes = lib.wanb200_range_attn_workspace_bytes(p) if Lq * (H // Hkv) > 16 else 0
+    if nbytes:  # from torch's allocator: ordered on this stream, and a captured graph's own
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
+    # the work in the launch record is that of the full rectangle; the ranges are on the device
+    _call(q, dev, kind, 4.0 * B * H * Lq * Lk * D, lib.wanb200_range_attn_fwd, p, "wanb200_range_attn_fwd")
     return out
 
 
@@ -544,52 +558,60 @@ def lora_linear(a, w, bias, down, up, ids, *, scales=None, epilogue=L.EPI_BIAS, 
     `linear`, but not EPI_BIAS_SUMSQ and EPI_SCATTER.  ids are read on the device at every call; an
     id >= n counts as none and sets the device error word (502)."""
     gm, ge = gate if gate is not None else (None, None)
-    dev = _same_device(a, w, bias, down, up, ids, scales, out, residual, gm, ge)
-    for name, t in (("a", a), ("w", w), ("down", down), ("up", up)):
-        _need(t.dtype == BF16, f"lora_linear: {name} must be bf16")
-    lda, ldw = _rows(a, "a"), _rows(w, "w")
-    M, K = a.shape
-    N = w.shape[0]
-    _need(w.shape[1] == K, f"lora_linear: a is [*, {K}] but w is {tuple(w.shape)}")
-    _need(down.dim() == 3 and down.is_contiguous() and down.shape[2] == K, "lora_linear: down must be contiguous [n, r, K]")
+    dev = _device_index(a, w, bias, down, up, ids, scales, out, residual, gm, ge)
+    M, K, lda = _row_major(a, "a", "lora_linear")
+    N, Kw, ldw = _row_major(w, "w", "lora_linear")
+    _need(Kw == K, f"lora_linear: a is [*, {K}] but w is {tuple(w.shape)}")
+    _need(down.dim() == 3 and down.shape[2] == K and down.is_contiguous(), "lora_linear: down must be contiguous [n, r, K]")
     n, r = down.shape[:2]
-    _need(up.is_contiguous() and tuple(up.shape) == (N, n, r), "lora_linear: up must be contiguous [N, n, r]")
-    _need(ids.dtype == torch.int32 and ids.is_contiguous() and ids.numel() == M, "lora_linear: ids must be int32 [M]")
-    _need(scales is None or (scales.dtype == torch.float32 and scales.is_contiguous() and scales.numel() == n),
+    _need(up.shape == (N, n, r) and up.is_contiguous(), "lora_linear: up must be contiguous [N, n, r]")
+    _need(a.dtype == w.dtype == down.dtype == up.dtype == BF16, "lora_linear: a, w, down and up must be bf16")
+    _need(ids.dtype == torch.int32 and ids.shape == (M,) and ids.is_contiguous(), "lora_linear: ids must be contiguous int32 [M]")
+    _need(scales is None or (scales.dtype == torch.float32 and scales.shape == (n,) and scales.is_contiguous()),
           "lora_linear: scales must be contiguous fp32 [n]")
-    _need(bias is None or (bias.dtype == BF16 and bias.is_contiguous() and bias.numel() == N),
+    _need(bias is None or (bias.dtype == BF16 and bias.shape == (N,) and bias.is_contiguous()),
           "lora_linear: bias must be contiguous bf16 [N]")
+    ap = a.data_ptr()
     if out is None:
         out = torch.empty(M, N, dtype=BF16, device=a.device)
-    for name, t in (("out", out), ("residual", residual)):
-        _need(t is None or (t.dtype in (BF16, torch.float32) and tuple(t.shape) == (M, N)),
-              f"lora_linear: {name} must be bf16 or fp32 [M, N]")
+        ldd, f32 = N, 0
+    else:
+        mo, no, ldd = _row_major(out, "out", "lora_linear")
+        f32 = int(out.dtype == torch.float32)
+        _need((f32 or out.dtype == BF16) and mo == M and no == N, "lora_linear: out must be bf16 or fp32 [M, N]")
+        d, es = out.data_ptr(), 4 if f32 else 2
+        _need(d >= ap + 2 * ((M - 1) * lda + K) or ap >= d + es * ((M - 1) * ldd + N), "lora_linear: out must not overlap a")
     if M == 0:
         return out
-    _need(not _overlap(out, a), "lora_linear: out must not overlap a")
-    p = L.LoraParams()
-    g = p.gemm
-    g.out_f32 = int(out.dtype == torch.float32)
-    g.residual_f32 = int(residual is not None and residual.dtype == torch.float32)
-    one = M == 1  # a single row's stride is never used; torch may report any
-    g.a, g.lda, g.w, g.ldw, g.d, g.ldd = _p(a), K if one else lda, _p(w), ldw, _p(out), N if one else _rows(out, "out")
-    g.M, g.N, g.K, g.epilogue, g.bias, g.tile_n = M, N, K, epilogue, _p(bias), tile_n
+    res = (None, 0)
+    res_f32 = 0
     if residual is not None:
-        g.residual, g.ldr = _p(residual), N if one else _rows(residual, "residual")
+        mr, nr, ldr = _row_major(residual, "residual", "lora_linear")
+        res_f32 = int(residual.dtype == torch.float32)
+        _need((res_f32 or residual.dtype == BF16) and mr == M and nr == N, "lora_linear: residual must be bf16 or fp32 [M, N]")
+        res = (residual.data_ptr(), ldr)
+    p = L.LoraParams(L.GemmParams(ap, lda, w.data_ptr(), ldw, out.data_ptr(), ldd, M, N, K, epilogue, _p(bias), *res),
+                     down.data_ptr(), up.data_ptr(), _p(scales), ids.data_ptr(), n, r)
+    g = p.gemm
+    if f32:
+        g.out_f32 = 1
+    if res_f32:
+        g.residual_f32 = 1
+    if tile_n:
+        g.tile_n = tile_n
     if gate is not None:
-        _need(gm.dtype == BF16 and ge.dtype == torch.float32 and ge.stride(-1) == 1, "lora_linear: bad gate tensors")
-        g.gate_mod, g.gate_e0, g.gate_frame_stride = _p(gm), _p(ge), ge.stride(0)
+        _need(gm.dtype == BF16 and gm.shape == (N,) and gm.is_contiguous() and ge.dtype == torch.float32 and
+              ge.dim() == 2 and ge.shape[1] == N and ge.stride(1) == 1, "lora_linear: gate must be (bf16 [N], fp32 [F, N])")
+        _need(frames is not None, "lora_linear: a gate needs frames")
+        g.gate_mod, g.gate_e0, g.gate_frame_stride = gm.data_ptr(), ge.data_ptr(), ge.stride(0)
     if frames is not None:
         _set_frames(g, frames)
-    p.down, p.up, p.scales, p.ids, p.adapters, p.rank = _p(down), _p(up), _p(scales), _p(ids), n, r
     lib = L.load()
-    with _on(dev):
-        nbytes = lib.wanb200_lora_workspace_bytes(M, n, r, g.out_f32)
-        if nbytes:  # from torch's allocator: ordered on this stream, and a captured graph's own
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            p.lora_workspace, p.lora_workspace_bytes = _p(ws), nbytes
-        L.check(_launch(a, kind, 2.0 * M * N * K + 2.0 * M * r * (K + N),
-                        lambda: lib.wanb200_gemm_lora(ctypes.byref(p), _stream(a))), "wanb200_gemm_lora")
+    nbytes = lib.wanb200_lora_workspace_bytes(M, n, r, f32)
+    if nbytes:  # from torch's allocator: ordered on this stream, and a captured graph's own
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device)
+        p.lora_workspace, p.lora_workspace_bytes = ws.data_ptr(), nbytes
+    _call(a, dev, kind, 2.0 * M * N * K + 2.0 * M * r * (K + N), lib.wanb200_gemm_lora, p, "wanb200_gemm_lora")
     return out
 
 
