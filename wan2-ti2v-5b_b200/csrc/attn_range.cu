@@ -91,14 +91,6 @@ __device__ __forceinline__ float score_log2(const RangeArgs& a, float s, int h, 
 // below the bandwidth bound, so the warp-level MMA is enough here.
 constexpr int RD_WARPS = 4, RD_KEYS = 16;
 
-__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                          uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
 template <int D, bool TWO, bool CAP, int BIAS>  // TWO: 9 to 16 rows (the second half of the MMA's rows is used)
 __global__ void __launch_bounds__(RD_WARPS * 32, TWO ? 2 : 3) range_decode_kernel(const RangeArgs a) {
   constexpr int KC = D / 32, VC = D / 64;  // 16-byte loads per K row, per V row

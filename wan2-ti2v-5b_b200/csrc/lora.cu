@@ -7,6 +7,7 @@
 // adapter's rank per tile and interleaved ones the ranks that really occur in it.
 // Up to 16 rows: reading W once bounds the call, and two small kernels stream it.
 #include <atomic>
+#include <type_traits>
 
 #include <cooperative_groups.h>
 
@@ -237,6 +238,232 @@ __global__ void __launch_bounds__(LD_THREADS, 1)
   if (warp == 1) tmem_dealloc(tmem_base, LD_GROUP * LORA_CHUNK);
 }
 
+// ================================================================== up to 16 rows: W is read once
+constexpr int LF_ROWS = 16, LF_WARPS = 8;
+
+struct LoraFewArgs {
+  const __nv_bfloat16* x;
+  int64_t ldx;
+  const __nv_bfloat16* w;
+  int64_t ldw;
+  void* d;
+  int64_t ldd;
+  int M, N, K, out_f32, res_f32;
+  const __nv_bfloat16* bias;
+  const void* residual;
+  int64_t ldr;
+  const __nv_bfloat16* gate_mod;
+  const float* gate_e0;
+  int64_t gate_frame_stride, seq_len, tokens_per_frame, row_offset, rows_per_seq;
+  const __nv_bfloat16 *down, *up;
+  const float* scales;
+  const int32_t* ids;
+  int adapters, rank;
+  float* h;  // [M][rank]
+  int* err;
+};
+
+__device__ __forceinline__ int few_id(const LoraFewArgs& a, int row) {
+  const int id = __ldg(a.ids + row);
+  return id >= 0 && id < a.adapters ? id : -1;
+}
+
+// h[row][i] = scale * x[row] . down[id][i] in fp32, one warp per (row, i).
+__global__ void __launch_bounds__(256) lora_few_down_kernel(const LoraFewArgs a) {
+  pdl_launch();
+  const int w = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int row = w / a.rank, i = w - row * a.rank;
+  if (row >= a.M) return;  // warp-uniform
+  const int id = few_id(a, row);
+  if (id < 0) {
+    if (lane == 0 && i == 0 && __ldg(a.ids + row) >= a.adapters) atomicCAS(a.err, 0, kErrBadAdapter);
+    return;
+  }
+  const uint4* xp = reinterpret_cast<const uint4*>(a.x + row * a.ldx) + lane;
+  const uint4* dp = reinterpret_cast<const uint4*>(a.down + ((int64_t)id * a.rank + i) * a.K) + lane;
+  float v = 0.f;
+  const int n = a.K / 8;
+#pragma unroll 8
+  for (int k = 0; k < n; k += 32) {
+    if (k + lane < n) {
+      float f[8], g[8];
+      unpack_bf16x8(__ldg(xp + k), f);
+      unpack_bf16x8(__ldg(dp + k), g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v = fmaf(f[e], g[e], v);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (lane == 0) a.h[row * a.rank + i] = v * (a.scales ? __ldg(a.scales + id) : 1.f);
+}
+
+// 8 columns of the output a block (16 or 32 were slower up to N = 14336: fewer blocks to hide a block's
+// merge behind); its warps take blocks of 64 K values in turn.  W goes from
+// memory straight to the operand registers of mma.sync (16 rows x 8 columns): a dot product does
+// not care about the order of K, so a lane's 16 bytes serve two K steps with x permuted alike.  Bound by
+// the read of W, far below even the warp-level MMA's rate.  The partial sums of the warps meet in
+// shared memory; the adapter's part is added there in fp32, its h formed by the launch before while
+// W streams.
+template <int EPI, bool TWO>
+__global__ void __launch_bounds__(LF_WARPS * 32) lora_few_kernel(const LoraFewArgs a) {
+  constexpr int COLS = 8, ROWS = TWO ? 16 : 8, UNROLL = 4;
+  __shared__ float red[LF_WARPS][ROWS][COLS + 1];
+  __shared__ float delta[ROWS][COLS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, q4 = lane & 3;
+  const int n0 = blockIdx.x * COLS;
+  const __nv_bfloat16* wp = a.w + (int64_t)(n0 + g4) * a.ldw + 8 * q4;
+  // rows behind the last repeat it: their sums are not stored
+  const __nv_bfloat16* x0 = a.x + min(g4, a.M - 1) * a.ldx + 8 * q4;
+  const __nv_bfloat16* x1 = a.x + min(g4 + 8, a.M - 1) * a.ldx + 8 * q4;
+  // the adapters' part of this block's outputs is read at the end: brought to the L2 meanwhile
+  for (int i = threadIdx.x; i < a.M * COLS; i += LF_WARPS * 32) {
+    const int id = few_id(a, i / COLS);
+    if (id >= 0) {
+      const __nv_bfloat16* up = a.up + ((int64_t)(n0 + i % COLS) * a.adapters + id) * a.rank;
+      for (int k = 0; k < a.rank; k += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(up + k));
+    }
+  }
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  // a warp's turn: UNROLL blocks of 64 K values (one 128-byte line of each W row), all loads first
+  auto turn = [&](int c0, auto unroll) {
+    constexpr int U = decltype(unroll)::value;
+    uint4 wv[U][2], xv[U][2][TWO ? 2 : 1];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int k = 64 * (c0 + u * LF_WARPS) + 32 * y;
+        wv[u][y] = ld_stream(wp + k);
+        xv[u][y][0] = __ldg(reinterpret_cast<const uint4*>(x0 + k));
+        if constexpr (TWO) xv[u][y][1] = __ldg(reinterpret_cast<const uint4*>(x1 + k));
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const uint4 lo = xv[u][y][0], hi = TWO ? xv[u][y][TWO ? 1 : 0] : make_uint4(0u, 0u, 0u, 0u);
+        mma_16816(acc, lo.x, hi.x, lo.y, hi.y, wv[u][y].x, wv[u][y].y);
+        mma_16816(acc, lo.z, hi.z, lo.w, hi.w, wv[u][y].z, wv[u][y].w);
+      }
+  };
+  const int blocks = a.K / 64;
+  int c0 = warp;
+  for (; c0 + (UNROLL - 1) * LF_WARPS < blocks; c0 += LF_WARPS * UNROLL) turn(c0, std::integral_constant<int, UNROLL>());
+  for (; c0 < blocks; c0 += LF_WARPS) turn(c0, std::integral_constant<int, 1>());
+#pragma unroll
+  for (int e = 0; e < (TWO ? 4 : 2); ++e) red[warp][g4 + 8 * (e >> 1)][2 * q4 + (e & 1)] = acc[e];
+  pdl_wait();
+  // h . up[n][id], eight lanes an output so that its rank values are read as whole lines
+  const int l8 = lane & 7;
+#pragma unroll 2
+  for (int i = threadIdx.x >> 3; i < a.M * COLS; i += LF_WARPS * 4) {
+    const int row = i / COLS, id = few_id(a, row);
+    float s0 = 0.f, s1 = 0.f;
+    if (id >= 0) {
+      const uint4* up = reinterpret_cast<const uint4*>(a.up + ((int64_t)(n0 + i % COLS) * a.adapters + id) * a.rank);
+      const float4* h = reinterpret_cast<const float4*>(a.h + row * a.rank);
+      for (int k = l8; k < a.rank / 8; k += 8) {
+        float u[8];
+        unpack_bf16x8(__ldg(up + k), u);
+        const float4 h0 = h[2 * k], h1 = h[2 * k + 1];
+        s0 = fmaf(h0.x, u[0], s0), s1 = fmaf(h0.y, u[1], s1), s0 = fmaf(h0.z, u[2], s0), s1 = fmaf(h0.w, u[3], s1);
+        s0 = fmaf(h1.x, u[4], s0), s1 = fmaf(h1.y, u[5], s1), s0 = fmaf(h1.z, u[6], s0), s1 = fmaf(h1.w, u[7], s1);
+      }
+    }
+    s0 += s1;
+#pragma unroll
+    for (int o = 4; o; o >>= 1) s0 += __shfl_xor_sync(0xffu << (lane & 24), s0, o);
+    if (l8 == 0) delta[row][i % COLS] = s0;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.M * COLS; i += LF_WARPS * 32) {
+    const int row = i / COLS, col = i % COLS, n = n0 + col;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < LF_WARPS; ++w) v += red[w][row][col];
+    v += delta[row][col];
+    if constexpr (EPI != WANB200_EPI_NONE) v += __bfloat162float(a.bias[n]);
+    if constexpr (EPI == WANB200_EPI_BIAS_GELU) v = gelu_tanh(v);
+    if constexpr (EPI == WANB200_EPI_BIAS_SILU) v = silu(v);
+    if constexpr (EPI == WANB200_EPI_BIAS_GATE_RES || EPI == WANB200_EPI_BIAS_RES) {
+      const int64_t at = row * a.ldr + n;
+      const float r = a.res_f32 ? static_cast<const float*>(a.residual)[at]
+                                : __bfloat162float(static_cast<const __nv_bfloat16*>(a.residual)[at]);
+      if constexpr (EPI == WANB200_EPI_BIAS_GATE_RES) {
+        const int64_t f = frame_of_row(row, a.rows_per_seq, a.row_offset, a.seq_len, a.tokens_per_frame);
+        v = r + v * (__bfloat162float(a.gate_mod[n]) + a.gate_e0[f * a.gate_frame_stride + n]);
+      } else {
+        v += r;
+      }
+    }
+    if (a.out_f32)
+      static_cast<float*>(a.d)[row * a.ldd + n] = v;
+    else
+      static_cast<__nv_bfloat16*>(a.d)[row * a.ldd + n] = __float2bfloat16(v);
+  }
+}
+
+template <int EPI>
+static cudaError_t launch_lora_few(const LoraFewArgs& a, const cudaLaunchConfig_t& cfg) {
+  return a.M > 8 ? cudaLaunchKernelEx(&cfg, lora_few_kernel<EPI, true>, a) : cudaLaunchKernelEx(&cfg, lora_few_kernel<EPI, false>, a);
+}
+
+static int lora_few(const wanb200_lora_params* p, float* h, int* err, cudaStream_t st) {
+  const wanb200_gemm_params* g = &p->gemm;
+  LoraFewArgs a;
+  a.x = reinterpret_cast<const __nv_bfloat16*>(g->a);
+  a.ldx = g->lda;
+  a.w = reinterpret_cast<const __nv_bfloat16*>(g->w);
+  a.ldw = g->ldw;
+  a.d = g->d;
+  a.ldd = g->ldd;
+  a.M = (int)g->M;
+  a.N = (int)g->N;
+  a.K = (int)g->K;
+  a.out_f32 = g->out_f32 != 0;
+  a.res_f32 = g->residual_f32 != 0;
+  a.bias = reinterpret_cast<const __nv_bfloat16*>(g->bias);
+  a.residual = g->residual;
+  a.ldr = g->ldr;
+  a.gate_mod = reinterpret_cast<const __nv_bfloat16*>(g->gate_mod);
+  a.gate_e0 = g->gate_e0;
+  a.gate_frame_stride = g->gate_frame_stride;
+  a.seq_len = g->seq_len > 0 ? g->seq_len : 1;
+  a.tokens_per_frame = g->tokens_per_frame > 0 ? g->tokens_per_frame : 1;
+  a.row_offset = g->row_offset;
+  a.rows_per_seq = g->rows_per_seq;
+  a.down = reinterpret_cast<const __nv_bfloat16*>(p->down);
+  a.up = reinterpret_cast<const __nv_bfloat16*>(p->up);
+  a.scales = p->scales;
+  a.ids = p->ids;
+  a.adapters = p->adapters;
+  a.rank = p->rank;
+  a.h = h;
+  a.err = err;
+  lora_few_down_kernel<<<(unsigned)((a.M * a.rank + 7) / 8), 256, 0, st>>>(a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.N / 8));
+  cfg.blockDim = dim3(LF_WARPS * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e;
+  switch (g->epilogue) {
+    case WANB200_EPI_NONE: e = launch_lora_few<WANB200_EPI_NONE>(a, cfg); break;
+    case WANB200_EPI_BIAS: e = launch_lora_few<WANB200_EPI_BIAS>(a, cfg); break;
+    case WANB200_EPI_BIAS_GELU: e = launch_lora_few<WANB200_EPI_BIAS_GELU>(a, cfg); break;
+    case WANB200_EPI_BIAS_SILU: e = launch_lora_few<WANB200_EPI_BIAS_SILU>(a, cfg); break;
+    case WANB200_EPI_BIAS_GATE_RES: e = launch_lora_few<WANB200_EPI_BIAS_GATE_RES>(a, cfg); break;
+    default: e = launch_lora_few<WANB200_EPI_BIAS_RES>(a, cfg); break;
+  }
+  if (e != cudaSuccess) return set_cuda_error("lora_few_kernel launch", e);
+  return WANB200_OK;
+}
+
 // ------------------------------------------------------------------ host launcher
 struct LoraLayout {
   int64_t rows_pad, num_m, h_off, bytes;
@@ -244,7 +471,12 @@ struct LoraLayout {
 };
 
 static LoraLayout lora_layout(int64_t M, int adapters, int rank, int out_f32) {
-  LoraLayout l;
+  LoraLayout l = {};
+  if (M <= LF_ROWS) {  // h in fp32
+    l.num_m = 1;
+    l.bytes = M * rank * 4;
+    return l;
+  }
   l.num_m = (M + LD_BM - 1) / LD_BM;
   l.rows_pad = l.num_m * LD_BM;
   l.cols = (adapters * rank + LORA_CHUNK - 1) / LORA_CHUNK * LORA_CHUNK;
@@ -280,6 +512,7 @@ int gemm_lora(const wanb200_lora_params* p, cudaStream_t st) {
   if (l.num_m > 65535) return set_error(WANB200_EINVAL, "gemm_lora: too many rows");
   int* err = device_error_word();
   if (!err) return WANB200_ECUDA;
+  if (g->M <= LF_ROWS) return lora_few(p, static_cast<float*>(p->lora_workspace), err, st);
   uint8_t* ws = static_cast<uint8_t*>(p->lora_workspace);
   CUtensorMap tx, td;
   rc = make_tmap_2d(&tx, g->a, g->K, g->M, g->lda, LD_BK, LD_BM);
