@@ -84,19 +84,29 @@ __device__ __forceinline__ float score_log2(const RangeArgs& a, float s, int h, 
 // ================================================================== few rows: one pass over K and V
 // One cluster of blocks per (key head, batch element); the warps of a cluster take blocks of 16 keys in
 // turn and keep their own running maximum, sum and output, merged at the end over the block's
-// shared memory and then over the cluster's.  K and V go straight from global memory to the
-// operand registers of mma.sync m16n8k16 (16 rows x 16 keys): a dot product does not care about the
-// order of its channels, so each lane's 16-byte load is taken as the operand of two K steps, q
-// permuted alike, and the output channels come out permuted the same way.  The tensor work is far
-// below the bandwidth bound, so the warp-level MMA is enough here.
-constexpr int RD_WARPS = 4, RD_KEYS = 16;
+// shared memory and then over the cluster's.  K and V pass through a ring of asynchronous copies,
+// each lane's own 16-byte pieces, to the operand registers of mma.sync m16n8k16 (16 rows x 16
+// keys): a dot product does not care about the order of its channels, so a lane's piece is taken as
+// the operand of two K steps, q permuted alike, and the output channels come out permuted the same
+// way.  The tensor work is far below the bandwidth bound, so the warp-level MMA is enough here.
+constexpr int RD_WARPS = 4, RD_KEYS = 16, RD_STAGES = 2, RD_BLOCKS = 3;
+
+template <int D>
+struct RangeDecodeCfg {
+  static constexpr int KC = D / 32, VC = D / 64;     // 16-byte pieces per K row, per V row
+  static constexpr int PIECES = 2 * KC + 4 * VC;     // of a lane in one stage: 2 K rows, 4 V rows
+  static constexpr int RING = RD_WARPS * RD_STAGES * PIECES * 512;
+};
 
 template <int D, bool TWO, bool CAP, int BIAS>  // TWO: 9 to 16 rows (the second half of the MMA's rows is used)
-__global__ void __launch_bounds__(RD_WARPS * 32, TWO ? 2 : 3) range_decode_kernel(const RangeArgs a) {
-  constexpr int KC = D / 32, VC = D / 64;  // 16-byte loads per K row, per V row
+__global__ void __launch_bounds__(RD_WARPS * 32, RD_BLOCKS) range_decode_kernel(const RangeArgs a) {
+  constexpr int KC = RangeDecodeCfg<D>::KC, VC = RangeDecodeCfg<D>::VC, PIECES = RangeDecodeCfg<D>::PIECES;
   constexpr int HR = TWO ? 2 : 1;          // rows held by a lane: lane / 4 and, with TWO, lane / 4 + 8
   constexpr int ROWS = TWO ? 16 : 8;
-  __shared__ float o_sh[RD_WARPS][ROWS][D + 4];
+  // the ring [warp][stage][piece][lane], and after it the warps' outputs
+  extern __shared__ uint4 ring[];
+  float(*o_sh)[ROWS][D + 4] = reinterpret_cast<float(*)[ROWS][D + 4]>(ring);
+  static_assert(RD_WARPS * ROWS * (D + 4) * 4 <= RangeDecodeCfg<D>::RING, "the outputs reuse the ring");
   __shared__ float2 ml_sh[RD_WARPS][ROWS];
   __shared__ float o_cta[ROWS][D];
   __shared__ float2 ml_cta[ROWS];
@@ -147,30 +157,37 @@ __global__ void __launch_bounds__(RD_WARPS * 32, TWO ? 2 : 3) range_decode_kerne
     }
   }
 
-  const __nv_bfloat16* kbase = a.k + b * a.k_batch + (int64_t)kh * D + 8 * q4;
-  const __nv_bfloat16* vbase = a.v + b * a.v_batch + (int64_t)kh * D + 8 * g4;
-  uint4 kr[2][KC], vr[4][VC];
-  auto load_k = [&](int key0) {
+  const int step = csize * RD_WARPS * RD_KEYS;
+  const bool some = any_lo < any_hi;
+  int key0 = (some ? any_lo : 0) + (crank * RD_WARPS + warp) * RD_KEYS, fkey = key0, stage = 0;
+  // this lane's rows of the block of keys to be asked for next: K rows g4, g4 + 8; V rows 2 q4 + {0, 1}, + 8
+  const __nv_bfloat16* kp = a.k + b * a.k_batch + (int64_t)kh * D + 8 * q4 + (key0 + g4) * a.k_tok;
+  const __nv_bfloat16* vp = a.v + b * a.v_batch + (int64_t)kh * D + 8 * g4 + (key0 + 2 * q4) * a.v_tok;
+  const int64_t k8 = 8 * a.k_tok, v8 = 8 * a.v_tok, kstep = step * a.k_tok, vstep = step * a.v_tok;
+  const __nv_bfloat16 *k_any = a.k, *v_any = a.v;  // a valid address for the copies that write zeros
+  const uint32_t base = smem_u32(ring + warp * (RD_STAGES * PIECES * 32) + lane);
+  auto fetch = [&](int stg) {  // keys behind the last seen one are not read
+    const uint32_t dst = base + stg * PIECES * 512;
+    if (fkey < any_hi) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int j = key0 + 8 * t + g4;
+      for (int t = 0; t < 2; ++t) {
+        const bool in = fkey + 8 * t + g4 < any_hi;
+        const __nv_bfloat16* src = in ? kp + t * k8 : k_any;
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        kr[t][c] = make_uint4(0u, 0u, 0u, 0u);
-        if (j < any_hi) kr[t][c] = __ldcs(reinterpret_cast<const uint4*>(kbase + j * a.k_tok + 32 * c));
+        for (int c = 0; c < KC; ++c) cp_async16(dst + (t * KC + c) * 512, src + 32 * c, in);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const bool in = fkey + (t >> 1) * 8 + 2 * q4 + (t & 1) < any_hi;
+        const __nv_bfloat16* src = in ? vp + (t >> 1) * v8 + (t & 1) * a.v_tok : v_any;
+#pragma unroll
+        for (int c = 0; c < VC; ++c) cp_async16(dst + (2 * KC + t * VC + c) * 512, src + 64 * c, in);
       }
     }
-  };
-  auto load_v = [&](int key0) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int j = key0 + (t >> 1) * 8 + 2 * q4 + (t & 1);
-#pragma unroll
-      for (int c = 0; c < VC; ++c) {
-        vr[t][c] = make_uint4(0u, 0u, 0u, 0u);
-        if (j < any_hi) vr[t][c] = __ldcs(reinterpret_cast<const uint4*>(vbase + j * a.v_tok + 64 * c));
-      }
-    }
+    cp_async_commit();
+    fkey += step;
+    kp += kstep;
+    vp += vstep;
   };
 
   float o[VC * 8][2 * HR];  // n tile 8 c + i: channels 64 c + 8 (2 q4 + {0, 1}) + i of the lane's rows
@@ -182,27 +199,29 @@ __global__ void __launch_bounds__(RD_WARPS * 32, TWO ? 2 : 3) range_decode_kerne
 #pragma unroll
   for (int x = 0; x < HR; ++x) m[x] = -INFINITY, l[x] = 0.f;
 
-  const int step = csize * RD_WARPS * RD_KEYS;
-  const bool some = any_lo < any_hi;
-  int key0 = (some ? any_lo : 0) + (crank * RD_WARPS + warp) * RD_KEYS;
-  if (some && key0 < any_hi) {
-    load_k(key0);
-    load_v(key0);
-  }
+#pragma unroll
+  for (int i = 0; i < RD_STAGES - 1; ++i) fetch(i);
   for (; some && key0 < any_hi; key0 += step) {
+    fetch(stage == 0 ? RD_STAGES - 1 : stage - 1);  // the stage used last
+    cp_async_wait<RD_STAGES - 1>();
+    const uint32_t src = base + stage * PIECES * 512;
+    if (++stage == RD_STAGES) stage = 0;
     float s[2][4];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
+      float odd[4] = {0.f, 0.f, 0.f, 0.f};  // two chains of products, half as long
       s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
-        mma_16816(s[t], qa[0][2 * c][0], TWO ? qa[HR - 1][2 * c][0] : 0u, qa[0][2 * c][1], TWO ? qa[HR - 1][2 * c][1] : 0u,
-                  kr[t][c].x, kr[t][c].y);
-        mma_16816(s[t], qa[0][2 * c + 1][0], TWO ? qa[HR - 1][2 * c + 1][0] : 0u, qa[0][2 * c + 1][1],
-                  TWO ? qa[HR - 1][2 * c + 1][1] : 0u, kr[t][c].z, kr[t][c].w);
+        const uint4 k = ld_shared16(src + (t * KC + c) * 512);
+        mma_16816(s[t], qa[0][2 * c][0], TWO ? qa[HR - 1][2 * c][0] : 0u, qa[0][2 * c][1], TWO ? qa[HR - 1][2 * c][1] : 0u, k.x,
+                  k.y);
+        mma_16816(odd, qa[0][2 * c + 1][0], TWO ? qa[HR - 1][2 * c + 1][0] : 0u, qa[0][2 * c + 1][1],
+                  TWO ? qa[HR - 1][2 * c + 1][1] : 0u, k.z, k.w);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[t][e] += odd[e];
     }
-    if (key0 + step < any_hi) load_k(key0 + step);  // K's registers are free: the next block's loads run from here
 
     // the lane's scores: rows g4 (+ 8), keys key0 + 8 t + 2 q4 + e
     float p[HR][4];
@@ -250,14 +269,17 @@ __global__ void __launch_bounds__(RD_WARPS * 32, TWO ? 2 : 3) range_decode_kerne
       pa[x][0] = pack_bf16x2(p[x][0], p[x][1]);  // weights in bf16, the MMA's operand type; the sum keeps fp32
       pa[x][1] = pack_bf16x2(p[x][2], p[x][3]);
     }
+    uint4 vr[4][VC];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int c = 0; c < VC; ++c) vr[t][c] = ld_shared16(src + (2 * KC + t * VC + c) * 512);
     if (key0 < all_lo || key0 + RD_KEYS > all_hi) {  // some row does not see some key of this block
-      int bad = 0;
+      uint32_t bad = 0;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int c = 0; c < VC; ++c)
-          bad |= nonfinite_bf16x2(vr[t][c].x) | nonfinite_bf16x2(vr[t][c].y) | nonfinite_bf16x2(vr[t][c].z) |
-                 nonfinite_bf16x2(vr[t][c].w);
+        for (int c = 0; c < VC; ++c) bad |= nonfinite_bits(vr[t][c]);
       if (__any_sync(0xffffffffu, bad)) {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -308,8 +330,9 @@ __global__ void __launch_bounds__(RD_WARPS * 32, TWO ? 2 : 3) range_decode_kerne
         }
       }
     }
-    if (key0 + step < any_hi) load_v(key0 + step);
   }
+  cp_async_wait<0>();
+  __syncthreads();  // the ring becomes the merge buffer
 
   // merge: warps of the block, then blocks of the cluster (row r of the result by rank r % csize)
 #pragma unroll
@@ -637,31 +660,38 @@ __global__ void __maxnreg__(160)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n" ::: "memory");
     if (warp == 8) {
       // ---------------------------------------------------------- unit queue and TMA
-      if (lane == 0) {
+      {  // the whole warp walks the issue loops: see elect_one
         uint32_t issued = 0, last_ph = 0, q_ph = 0;
         int gk = 0, qi = 0;
         bool ok = true, q_pending = false;
         for (int i = 0; ok; ++i) {
           const int s = i % RT_QUEUE;
-          if (!mbar_wait(u_empty + 8 * s, ((i / RT_QUEUE) & 1) ^ 1, abort_flag, err, kErrTimeoutAttnProducer)) {
+          if (!mbar_wait_warp(u_empty + 8 * s, ((i / RT_QUEUE) & 1) ^ 1, abort_flag, err, kErrTimeoutAttnProducer)) {
             ok = false;
             break;
           }
-          int u = atomicAdd(g.counter, 1);
-          if (u >= g.units) u = -1;
-          queue[s] = u;
-          mbar_arrive(u_full + 8 * s);
+          int u = 0;
+          if (lane == 0) {
+            u = atomicAdd(g.counter, 1);
+            if (u >= g.units) u = -1;
+            queue[s] = u;
+            mbar_arrive(u_full + 8 * s);
+          }
+          u = __shfl_sync(0xffffffffu, u, 0);
           if (u < 0) break;
           const RangeUnit w = range_unit(g, u);
           if (w.k0 >= w.k1) continue;
-          if (!mbar_wait(q_empty, (qi & 1) ^ 1, abort_flag, err, kErrTimeoutAttnProducer)) {
+          if (!mbar_wait_warp(q_empty, (qi & 1) ^ 1, abort_flag, err, kErrTimeoutAttnProducer)) {
             ok = false;
             break;
           }
-          mbar_expect_tx(q_full, 2 * HALVES * g.tpt * g.a.group * 128);
-          for (int t = 0; t < 2; ++t)
-            for (int h = 0; h < HALVES; ++h)
-              tma_load_4d(sbase + t * TILE + h * RT_BLK, &tmQ, q_full, 64 * h, w.kh * g.a.group, w.tok0 + t * g.tpt, w.b);
+          if (elect_one()) {
+            mbar_expect_tx(q_full, 2 * HALVES * g.tpt * g.a.group * 128);
+            for (int t = 0; t < 2; ++t)
+              for (int h = 0; h < HALVES; ++h)
+                tma_load_4d(sbase + t * TILE + h * RT_BLK, &tmQ, q_full, 64 * h, w.kh * g.a.group, w.tok0 + t * g.tpt, w.b);
+          }
+          __syncwarp();
           q_pending = true;
           q_ph = qi & 1;
           ++qi;
@@ -670,16 +700,19 @@ __global__ void __maxnreg__(160)
             for (int x = 0; x < 2; ++x, ++gk) {
               const int slot = gk % RING;
               const uint32_t ph = (gk / RING) & 1;
-              if (!mbar_wait(kv_empty + 8 * slot, ph ^ 1, abort_flag, err, kErrTimeoutAttnProducer)) {
+              if (!mbar_wait_warp(kv_empty + 8 * slot, ph ^ 1, abort_flag, err, kErrTimeoutAttnProducer)) {
                 ok = false;
                 break;
               }
               const void* map = x ? static_cast<const void*>(&tmV) : static_cast<const void*>(&tmK);
               const uint32_t dst = sbase + C::OFF_R + slot * TILE;
-              mbar_expect_tx(kv_full + 8 * slot, TILE);
-              for (int h = 0; h < HALVES; ++h)
-                tma_load_4d(dst + h * RT_BLK, map, kv_full + 8 * slot, 64 * h, w.kh, j * RT_N, w.b);
-              if (x && unit_partial(w, j)) mbar_arrive(v_req + 8 * slot);
+              if (elect_one()) {
+                mbar_expect_tx(kv_full + 8 * slot, TILE);
+                for (int h = 0; h < HALVES; ++h)
+                  tma_load_4d(dst + h * RT_BLK, map, kv_full + 8 * slot, 64 * h, w.kh, j * RT_N, w.b);
+                if (x && unit_partial(w, j)) mbar_arrive(v_req + 8 * slot);
+              }
+              __syncwarp();
               issued |= 1u << slot;
               last_ph = (last_ph & ~(1u << slot)) | (ph << slot);
             }
@@ -693,64 +726,80 @@ __global__ void __maxnreg__(160)
       }
     } else if (warp == 9) {
       // ---------------------------------------------------------- MMA issue
-      if (lane == 0) {
+      {
         constexpr uint32_t idesc_s = idesc_bf16_f32(RT_M, RT_N, false, false);
         constexpr uint32_t idesc_o = idesc_bf16_f32(RT_M, D, false, true);
+        constexpr uint32_t hi = sw128_hi(1024);
+        const uint32_t q_lo = sw128_lo(sbase, 16), k_lo = sw128_lo(sbase + C::OFF_R, 16), v_lo = sw128_lo(sbase + C::OFF_R, RT_BLK);
+        auto commit = [](bool yes, uint32_t bar) {
+          if (yes && elect_one()) umma_commit(bar);
+          __syncwarp();
+        };
         int gk = 0, qi = 0, np[2] = {0, 0};
         uint32_t ok_ph = 0;  // phase of v_ok per ring slot
         bool ok = true;
         while (ok) {
           const int u = next_unit(kErrTimeoutAttnMma);
-          if (u < 0) break;
+          if (!__all_sync(0xffffffffu, u != -2) || u < 0) break;
           const RangeUnit w = range_unit(g, u);
-          release_unit();
+          __syncwarp();
+          if (lane == 0) release_unit();
           if (w.k0 >= w.k1) continue;
           auto kv_wait = [&](int r) -> bool {
-            return mbar_wait(kv_full + 8 * (r % RING), (r / RING) & 1, abort_flag, err, kErrTimeoutAttnMma);
+            return mbar_wait_warp(kv_full + 8 * (r % RING), (r / RING) & 1, abort_flag, err, kErrTimeoutAttnMma);
           };
           auto qk = [&](int t, int slot) {
             tc_fence_after();
-            const uint32_t d = tmem_base + t * RT_N, qb = sbase + t * TILE, kb = sbase + C::OFF_R + slot * TILE;
+            const uint32_t d = tmem_base + t * RT_N, qb = q_lo + t * (TILE >> 4), kb = k_lo + slot * (TILE >> 4);
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off = (kk >> 2) * RT_BLK + (kk & 3) * 32;
-              umma_bf16(d, sw128_desc(qb + off, 16, 1024), sw128_desc(kb + off, 16, 1024), idesc_s, kk != 0);
+              for (int kk = 0; kk < D / 16; ++kk) {
+                const uint32_t off = ((kk >> 2) * RT_BLK + (kk & 3) * 32) >> 4;
+                umma_bf16_w(d, qb + off, kb + off, hi, idesc_s, kk != 0);
+              }
+              umma_commit(s_full + 8 * t);
             }
-            umma_commit(s_full + 8 * t);
+            __syncwarp();
           };
           auto pv = [&](int t, int slot, bool last) -> bool {
             // P_t comes in two parts: the MMA over its first keys runs while the warps exponentiate the rest
             const uint32_t ph = np[t]++ & 1;
-            if (!mbar_wait(p_part + 8 * t, ph, abort_flag, err, kErrTimeoutAttnMma)) return false;
+            if (!mbar_wait_warp(p_part + 8 * t, ph, abort_flag, err, kErrTimeoutAttnMma)) return false;
             tc_fence_after();
-            const uint32_t d = tmem_base + 2 * RT_N + t * D, pa = tmem_base + t * RT_N, vb = sbase + C::OFF_R + slot * TILE;
+            const uint32_t d = tmem_base + 2 * RT_N + t * D, pa = tmem_base + t * RT_N, vb = v_lo + slot * (TILE >> 4);
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < RT_P_SPLIT / 16; ++kk)
-              umma_bf16_tmem_a(d, pa + kk * 8, sw128_desc(vb + kk * 2048, RT_BLK, 1024), idesc_o, true);
-            if (!mbar_wait(p_full + 8 * t, ph, abort_flag, err, kErrTimeoutAttnMma)) return false;
+              for (int kk = 0; kk < RT_P_SPLIT / 16; ++kk)
+                umma_bf16_tmem_a_w(d, pa + kk * 8, vb + kk * (2048 >> 4), hi, idesc_o);
+            }
+            __syncwarp();
+            if (!mbar_wait_warp(p_full + 8 * t, ph, abort_flag, err, kErrTimeoutAttnMma)) return false;
             tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = RT_P_SPLIT / 16; kk < RT_N / 16; ++kk)
-              umma_bf16_tmem_a(d, pa + kk * 8, sw128_desc(vb + kk * 2048, RT_BLK, 1024), idesc_o, true);
-            if (last) umma_commit(o_done + 8 * t);
+              for (int kk = RT_P_SPLIT / 16; kk < RT_N / 16; ++kk)
+                umma_bf16_tmem_a_w(d, pa + kk * 8, vb + kk * (2048 >> 4), hi, idesc_o);
+              if (last) umma_commit(o_done + 8 * t);
+            }
+            __syncwarp();
             return true;
           };
           int j = w.k0;
-          ok = mbar_wait(q_full, qi & 1, abort_flag, err, kErrTimeoutAttnMma) && kv_wait(gk);
+          ok = mbar_wait_warp(q_full, qi & 1, abort_flag, err, kErrTimeoutAttnMma) && kv_wait(gk);
           ++qi;
           if (!ok) break;
           int jn = j + 1;
           while (jn < w.k1 && !unit_loads(w, jn)) ++jn;
           for (int t = 0; t < 2; ++t)
             if (unit_has(w, t, j)) qk(t, gk % RING);
-          umma_commit(kv_empty + 8 * (gk % RING));
-          if (jn >= w.k1) umma_commit(q_empty);
+          commit(true, kv_empty + 8 * (gk % RING));
+          commit(jn >= w.k1, q_empty);
           while (true) {
             const int vslot = (gk + 1) % RING, kslot = (gk + 2) % RING;
             const bool more = jn < w.k1;
             if (!kv_wait(gk + 1)) { ok = false; break; }
             if (unit_partial(w, j)) {
-              if (!mbar_wait(v_ok + 8 * vslot, (ok_ph >> vslot) & 1, abort_flag, err, kErrTimeoutAttnMma)) { ok = false; break; }
+              if (!mbar_wait_warp(v_ok + 8 * vslot, (ok_ph >> vslot) & 1, abort_flag, err, kErrTimeoutAttnMma)) { ok = false; break; }
               ok_ph ^= 1u << vslot;
             }
             if (unit_has(w, 0, j) && !pv(0, vslot, j == w.z[0] - 1)) { ok = false; break; }
@@ -759,17 +808,17 @@ __global__ void __maxnreg__(160)
               if (unit_has(w, 0, jn)) qk(0, kslot);
             }
             if (unit_has(w, 1, j) && !pv(1, vslot, j == w.z[1] - 1)) { ok = false; break; }
-            umma_commit(kv_empty + 8 * vslot);
+            commit(true, kv_empty + 8 * vslot);
             gk += 2;
             if (!more) break;
             if (unit_has(w, 1, jn)) qk(1, kslot);
-            umma_commit(kv_empty + 8 * kslot);
+            commit(true, kv_empty + 8 * kslot);
             j = jn++;
             while (jn < w.k1 && !unit_loads(w, jn)) ++jn;
-            if (jn >= w.k1) umma_commit(q_empty);  // the unit's last QK is issued: Q may be overwritten after it
+            commit(jn >= w.k1, q_empty);  // the unit's last QK is issued: Q may be overwritten after it
           }
         }
-        umma_commit(done_bar);
+        commit(true, done_bar);
         mbar_drain(done_bar, 0, err);
       }
     } else {
@@ -799,18 +848,9 @@ __global__ void __maxnreg__(160)
             for (int x = 0; x < 2; ++x) {
               const int word = 2 * x + (warp - 10);
               uint8_t* row = smem + C::OFF_R + slot * TILE + (word * 32 + lane) * 128;
-              int hit = 0;
+              bool hit = false;
 #pragma unroll
-              for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {  // chunks in an order that spreads a quarter-warp over the banks
-                  uint4* pc = reinterpret_cast<uint4*>(row + h * RT_BLK + (((c + lane) & 7) << 4));
-                  const uint4 v = *pc;
-                  if (nonfinite_bf16x2(v.x) | nonfinite_bf16x2(v.y) | nonfinite_bf16x2(v.z) | nonfinite_bf16x2(v.w)) {
-                    *pc = make_uint4(zero_nonfinite(v.x), zero_nonfinite(v.y), zero_nonfinite(v.z), zero_nonfinite(v.w));
-                    hit = 1;
-                  }
-                }
+              for (int h = 0; h < HALVES; ++h) hit |= clean_row128(row + h * RT_BLK, lane);
               const uint32_t bits = __ballot_sync(0xffffffffu, hit);
               if (lane == 0) bad[slot * 4 + word] = bits;
               wrote |= bits != 0;
@@ -1167,12 +1207,27 @@ int64_t range_attn_workspace_bytes(const wanb200_range_attn_params* p) {
   return range_layout(p).bytes;
 }
 
+template <int D, bool TWO, bool CAP, int BIAS>
+static cudaError_t launch_range_decode(const RangeArgs& a, const cudaLaunchConfig_t& cfg, int dev) {
+  static std::atomic<bool> attr_set[kMaxDevices] = {};
+  if (!attr_set[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(range_decode_kernel<D, TWO, CAP, BIAS>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, RangeDecodeCfg<D>::RING);
+    if (e != cudaSuccess) return e;
+    attr_set[dev].store(true, std::memory_order_release);
+  }
+  return cudaLaunchKernelEx(&cfg, range_decode_kernel<D, TWO, CAP, BIAS>, a);
+}
+
 template <int D, bool CAP, int BIAS>
 static int launch_range_decode(const RangeArgs& a, int rows, cudaStream_t st) {
   // Blocks of a cluster share one (key head, batch element).  The cluster size is the one with the
   // smallest waves x (keys of a block + 160): the block's fixed costs (start, merges) weigh about as much
   // as 160 keys.
-  const int64_t units = (int64_t)a.batch * a.kv_heads, slots = (int64_t)num_sms() * (rows > 8 ? 2 : 3);
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= kMaxDevices) return set_error(WANB200_EINVAL, "device index out of range");
+  const int64_t units = (int64_t)a.batch * a.kv_heads, slots = (int64_t)num_sms() * RD_BLOCKS;
   int best = 1;
   double best_t = 1e300;
   for (int c = 1; c <= 8; c *= 2) {
@@ -1182,6 +1237,7 @@ static int launch_range_decode(const RangeArgs& a, int rows, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)best, (unsigned)a.kv_heads, (unsigned)a.batch);
   cfg.blockDim = dim3(RD_WARPS * 32);
+  cfg.dynamicSmemBytes = RangeDecodeCfg<D>::RING;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1189,8 +1245,8 @@ static int launch_range_decode(const RangeArgs& a, int rows, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = rows > 8 ? cudaLaunchKernelEx(&cfg, range_decode_kernel<D, true, CAP, BIAS>, a)
-                                 : cudaLaunchKernelEx(&cfg, range_decode_kernel<D, false, CAP, BIAS>, a);
+  const cudaError_t e = rows > 8 ? launch_range_decode<D, true, CAP, BIAS>(a, cfg, dev)
+                                 : launch_range_decode<D, false, CAP, BIAS>(a, cfg, dev);
   if (e != cudaSuccess) return set_cuda_error("range_decode_kernel launch", e);
   return WANB200_OK;
 }

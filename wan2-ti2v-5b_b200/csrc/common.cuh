@@ -72,6 +72,15 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+// True in one lane of a converged warp, the same one every time.  A warp that walks an issue loop
+// together and lets one lane issue keeps addresses and descriptors in uniform registers; a loop inside
+// `if (lane == 0)` moves each of them there for every instruction.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+  return p != 0;
+}
+
 // Wait for the phase with parity `parity` to complete.  Returns false (after recording `code`
 // and raising *abort) if the deadline passes or another thread of the CTA already aborted.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort, int* err,
@@ -304,6 +313,32 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lbo_byte
          (uint64_t((sbo_bytes >> 4) & 0x3FFFu) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
 
+// The same descriptor as two words: the low one advances with the address (in 16-byte units, so a
+// step inside a tile is one addition), the high one is the same for a whole launch.  One thread issues
+// every MMA of a block, and building each 64-bit descriptor anew took it longer than the MMA ran.
+__device__ __forceinline__ uint32_t sw128_lo(uint32_t saddr, uint32_t lbo_bytes) { return (saddr >> 4) | ((lbo_bytes >> 4) << 16); }
+constexpr uint32_t sw128_hi(uint32_t sbo_bytes) { return (sbo_bytes >> 4) | (1u << 14) | (2u << 29); }
+
+__device__ __forceinline__ void umma_bf16_w(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 ad, bd;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tmov.b64 ad, {%1, %3};\n\tmov.b64 bd, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %4, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// A from tensor memory (umma_bf16_tmem_a), B's descriptor in two words; always accumulates.
+__device__ __forceinline__ void umma_bf16_tmem_a_w(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 bd;\n\t"
+      "setp.eq.b32 p, 0, 0;\n\tmov.b64 bd, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], bd, %4, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc)
+      : "memory");
+}
+
 // ------------------------------------------------------------------ misc math
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
@@ -326,16 +361,35 @@ __device__ __forceinline__ void unpack_bf16x8(const uint4& u, float* f) {
   }
 }
 
-// Non-zero when one of the two packed bf16 values is a NaN or an infinity (all exponent bits set).
-__device__ __forceinline__ int nonfinite_bf16x2(uint32_t u) {
-  return (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
+// Bits 15 and 31 say which of the two packed bf16 values is a NaN or an infinity (exponent all
+// ones: adding one to it carries into the sign's place, which the mask cleared).
+__device__ __forceinline__ uint32_t nonfinite_bits(uint32_t u) { return ((u & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+__device__ __forceinline__ uint32_t nonfinite_bits(const uint4& v) {
+  return (((v.x & 0x7f807f80u) + 0x00800080u) | ((v.y & 0x7f807f80u) + 0x00800080u) | ((v.z & 0x7f807f80u) + 0x00800080u) |
+          ((v.w & 0x7f807f80u) + 0x00800080u)) &
+         0x80008000u;
 }
 
 // The packed pair with its NaNs and infinities replaced by zeros.
 __device__ __forceinline__ uint32_t zero_nonfinite(uint32_t u) {
-  if ((u & 0x7f80u) == 0x7f80u) u &= 0xffff0000u;
-  if ((u & 0x7f800000u) == 0x7f800000u) u &= 0xffffu;
-  return u;
+  const uint32_t bad = nonfinite_bits(u);
+  return u & ~((bad >> 15) * 0xffffu);
+}
+
+// Zeroes the non-finite values of the 128-byte row at `row` of a swizzled tile (16-byte groups in an
+// order that spreads a quarter-warp over the banks); true when there were any.
+__device__ __forceinline__ bool clean_row128(uint8_t* row, int lane) {
+  uint32_t bad = 0;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) bad |= nonfinite_bits(*reinterpret_cast<const uint4*>(row + (((q + lane) & 7) << 4)));
+  if (!bad) return false;
+#pragma unroll 1
+  for (int q = 0; q < 8; ++q) {
+    uint4* p = reinterpret_cast<uint4*>(row + (q << 4));
+    const uint4 v = *p;
+    *p = make_uint4(zero_nonfinite(v.x), zero_nonfinite(v.y), zero_nonfinite(v.z), zero_nonfinite(v.w));
+  }
+  return true;
 }
 
 // Programmatic dependent launch: wait until the launch before has completed and its writes are
@@ -343,12 +397,59 @@ __device__ __forceinline__ uint32_t zero_nonfinite(uint32_t u) {
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// Barrier over the cluster's threads (release / acquire), from any warp in any state of convergence.
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// 16 bytes of another block's shared memory of the cluster, at this block's address `addr`.
+__device__ __forceinline__ float4 ld_cluster16(uint32_t addr, uint32_t rank) {
+  float4 v;
+  asm volatile(
+      "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %4, %5;\n\t"
+      "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [ra];\n\t}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+      : "r"(addr), "r"(rank)
+      : "memory");
+  return v;
+}
+
+__device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ int ld_cluster_int(uint32_t addr, uint32_t rank) {
+  int v;
+  asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %1, %2;\n\tld.shared::cluster.u32 %0, [ra];\n\t}"
+               : "=r"(v)
+               : "r"(addr), "r"(rank)
+               : "memory");
+  return v;
+}
+
 // 16 bytes of data that is read once, past the L1.
 __device__ __forceinline__ uint4 ld_stream(const void* p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
+  return v;
+}
+
+// Asynchronous 16-byte copies to shared memory, counted in groups per thread; zeros, without a read,
+// where !in.  A thread that reads back only what it copied itself needs no barrier, only the wait:
+// a prefetch that takes no registers.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {  // all but the newest N groups have landed
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
 

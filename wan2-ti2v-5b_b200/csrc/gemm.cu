@@ -261,6 +261,85 @@ __device__ __forceinline__ void lora_add_slow(const LoraPlan* lo, float* v, int 
   for (int i = 0; i < 32; ++i) v[i] += lora_slow_value(lo, row, col0 + i);
 }
 
+// A tile whose K is shared by the blocks of a cluster.  Every block leaves its fp32 sums in its
+// shared memory (row r, column c at lora_part_offset); then each takes 128 / ksplit of the rows, adds
+// the blocks' sums in rank order and finishes them, four columns a thread, so that the reads from
+// the other SMs (a tile is 128 KB, and they run at a fraction of the local rate) are spread evenly.
+__device__ __forceinline__ uint32_t lora_part_offset(int bn, int r, int c) { return (uint32_t)(r * (bn + 4) + c) * 4; }
+
+template <int EPI>
+__device__ __forceinline__ void lora_join_rows(const GemmArgs& a, const LoraPlan* lora, uint32_t tiles, bool slow, int m0,
+                                               int n0, int krank, int tid) {
+  constexpr int U = 4;
+  const int ks = lora->ksplit, per = GBM / ks, groups = a.bn / 4, total = per * groups;
+  for (int i0 = tid; i0 < total; i0 += U * 32 * G_EPI_WARPS) {
+    float4 x[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * 32 * G_EPI_WARPS;
+      if (i < total) {
+        const uint32_t at = tiles + lora_part_offset(a.bn, krank * per + i / groups, i % groups * 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k < ks) x[u][k] = k == krank ? ld_shared_f4(at) : ld_cluster16(at, k);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * 32 * G_EPI_WARPS;
+      const int row = m0 + krank * per + i / groups, col = n0 + i % groups * 4;
+      if (i >= total || row >= a.M || col >= a.N) continue;
+      float v[4] = {x[u][0].x, x[u][0].y, x[u][0].z, x[u][0].w};
+#pragma unroll
+      for (int k = 1; k < 4; ++k)
+        if (k < ks) v[0] += x[u][k].x, v[1] += x[u][k].y, v[2] += x[u][k].z, v[3] += x[u][k].w;
+      if (slow) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += lora_slow_value(lora, row, col + j);
+      }
+      if constexpr (EPI != WANB200_EPI_NONE) {
+        const uint2 bu = __ldg(reinterpret_cast<const uint2*>(a.bias + col));
+        v[0] += __uint_as_float(bu.x << 16), v[1] += __uint_as_float(bu.x & 0xffff0000u);
+        v[2] += __uint_as_float(bu.y << 16), v[3] += __uint_as_float(bu.y & 0xffff0000u);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (EPI == WANB200_EPI_BIAS_GELU) v[j] = gelu_tanh(v[j]);
+        if constexpr (EPI == WANB200_EPI_BIAS_SILU) v[j] = silu(v[j]);
+      }
+      if constexpr (epi_has_residual(EPI)) {
+        float r[4];
+        if (a.res_f32) {
+          const float4 rv = *reinterpret_cast<const float4*>(static_cast<const float*>(a.residual) + (int64_t)row * a.ldr + col);
+          r[0] = rv.x, r[1] = rv.y, r[2] = rv.z, r[3] = rv.w;
+        } else {
+          const uint2 rv =
+              *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(a.residual) + (int64_t)row * a.ldr + col);
+          r[0] = __uint_as_float(rv.x << 16), r[1] = __uint_as_float(rv.x & 0xffff0000u);
+          r[2] = __uint_as_float(rv.y << 16), r[3] = __uint_as_float(rv.y & 0xffff0000u);
+        }
+        if constexpr (EPI == WANB200_EPI_BIAS_GATE_RES) {
+          const int64_t f = frame_of_row(row, a.rows_per_seq, a.row_offset, a.seq_len, a.tokens_per_frame);
+          const float4 e = __ldg(reinterpret_cast<const float4*>(a.gate_e0 + f * a.gate_frame_stride + col));
+          const uint2 gu = __ldg(reinterpret_cast<const uint2*>(a.gate_mod + col));
+          v[0] = r[0] + v[0] * (__uint_as_float(gu.x << 16) + e.x);
+          v[1] = r[1] + v[1] * (__uint_as_float(gu.x & 0xffff0000u) + e.y);
+          v[2] = r[2] + v[2] * (__uint_as_float(gu.y << 16) + e.z);
+          v[3] = r[3] + v[3] * (__uint_as_float(gu.y & 0xffff0000u) + e.w);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] += r[j];
+        }
+      }
+      if (a.out_f32)
+        *reinterpret_cast<float4*>(static_cast<float*>(a.d) + (int64_t)row * a.ldd + col) = make_float4(v[0], v[1], v[2], v[3]);
+      else
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.d) + (int64_t)row * a.ldd + col) =
+            make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    }
+  }
+}
+
 // The fp32 residual epilogue of one tile for the epilogue warp on lane quarter `quad` that takes
 // the 32-column chunks half, half + 2, ...  Each 32 x 32 accumulator chunk (lane = row after the
 // tcgen05.ld) goes to the warp's 4 KB staging buffer and comes back with lane = (sub, cg): rows
@@ -415,25 +494,40 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
   const int num_n = (args.N + bn - 1) / bn;
   const int num_m = (args.M + GBM - 1) / GBM;
   const int num_tiles = num_m * num_n;
-  const int kblocks = args.K / GBK;
+  // the block's tiles and, with LORA and a cluster, its share of its one tile's K: a
+  // run of K blocks each, and the adapter chunks in turn
+  int kblocks = args.K / GBK, kb0 = 0, krank = 0, tile0 = blockIdx.x, tile_step = gridDim.x;
+  if constexpr (LORA) {
+    if (lora->ksplit > 1) {
+      krank = blockIdx.x % lora->ksplit;
+      tile0 = blockIdx.x / lora->ksplit;
+      tile_step = gridDim.x / lora->ksplit;
+      const int per = (kblocks + lora->ksplit - 1) / lora->ksplit;
+      kb0 = krank * per;
+      kblocks = min(kblocks - kb0, per);  // >= 1 (host)
+    }
+  }
 
   if (warp == 0) {
-    if (lane == 0) {
+    {
       int stage = 0;
       uint32_t phase = 0, issued = 0, last_phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
+      for (int tile = tile0; ok && tile < num_tiles; tile += tile_step) {
         int m0, n0;
         tile_origin(tile, num_m, num_n, bn, m0, n0);
         for (int kb = 0; kb < kblocks; ++kb) {
-          if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, abort_flag, err, kErrTimeoutGemmProducer)) {
+          if (!mbar_wait_warp(empty0 + 8 * stage, phase ^ 1, abort_flag, err, kErrTimeoutGemmProducer)) {
             ok = false;
             break;
           }
           const uint32_t a_dst = tiles + stage * SB;
-          mbar_expect_tx(full0 + 8 * stage, G_A_BYTES + bn * GBK * 2);
-          tma_load_2d(a_dst, &tmA, full0 + 8 * stage, kb * GBK, m0);
-          tma_load_2d(a_dst + G_A_BYTES, &tmB, full0 + 8 * stage, kb * GBK, n0);
+          if (elect_one()) {
+            mbar_expect_tx(full0 + 8 * stage, G_A_BYTES + bn * GBK * 2);
+            tma_load_2d(a_dst, &tmA, full0 + 8 * stage, (kb0 + kb) * GBK, m0);
+            tma_load_2d(a_dst + G_A_BYTES, &tmB, full0 + 8 * stage, (kb0 + kb) * GBK, n0);
+          }
+          __syncwarp();
           issued |= 1u << stage;
           last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
           if (++stage == GSTAGES) {
@@ -444,18 +538,22 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
         if constexpr (LORA) {
           pdl_wait();  // h and the step bits come from the launch before, which runs beside this K loop
           const uint32_t* mask = lora->step_mask + m0 / GBM * LORA_MASK_WORDS;
-          for (int c = 0; ok && c < lora->cols / LORA_CHUNK; ++c) {
-            if (!lora_chunk_steps(mask, c)) continue;
+          const bool mixed = __ldg(lora->mixed + m0 / GBM) != 0;
+          for (int c = 0, n = 0; ok && c < lora->cols / LORA_CHUNK; ++c) {
+            if (!lora_chunk_steps(mask, c) || n++ % lora->ksplit != krank) continue;
             for (int pl = 0; pl < lora->planes; ++pl) {
-              if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, abort_flag, err, kErrTimeoutGemmProducer)) {
+              if (!mbar_wait_warp(empty0 + 8 * stage, phase ^ 1, abort_flag, err, kErrTimeoutGemmProducer)) {
                 ok = false;
                 break;
               }
               const uint32_t a_dst = tiles + stage * SB;
-              mbar_expect_tx(full0 + 8 * stage, G_A_BYTES + bn * GBK * 2);
-              tma_load_2d(a_dst, tmH, full0 + 8 * stage, c * LORA_CHUNK, (int)(pl * lora->rows_pad) + m0);
-              tma_load_2d(a_dst + G_A_BYTES, tmU, full0 + 8 * stage, c * LORA_CHUNK, n0);
-              mbar_arrive(u_req0 + 8 * stage);
+              if (elect_one()) {
+                mbar_expect_tx(full0 + 8 * stage, G_A_BYTES + bn * GBK * 2);
+                tma_load_2d(a_dst, tmH, full0 + 8 * stage, c * LORA_CHUNK, (int)(pl * lora->rows_pad) + m0);
+                tma_load_2d(a_dst + G_A_BYTES, tmU, full0 + 8 * stage, c * LORA_CHUNK, n0);
+                if (mixed) mbar_arrive(u_req0 + 8 * stage);
+              }
+              __syncwarp();
               issued |= 1u << stage;
               last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
               if (++stage == GSTAGES) {
@@ -472,30 +570,31 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    {
       const uint32_t idesc = idesc_bf16_f32(GBM, bn, false, false);
+      const uint32_t tiles_lo = sw128_lo(tiles, 16);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       [[maybe_unused]] uint32_t u_ok_ph = 0;  // phase of u_ok per stage
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
-        if (!mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag, err, kErrTimeoutGemmMma)) break;
+      for (int tile = tile0; ok && tile < num_tiles; tile += tile_step) {
+        if (!mbar_wait_warp(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag, err, kErrTimeoutGemmMma)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * GBN;
         for (int kb = 0; kb < kblocks; ++kb) {
-          if (!mbar_wait(full0 + 8 * stage, phase, abort_flag, err, kErrTimeoutGemmMma)) {
+          if (!mbar_wait_warp(full0 + 8 * stage, phase, abort_flag, err, kErrTimeoutGemmMma)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a_addr = tiles + stage * SB;
-          const uint32_t b_addr = a_addr + G_A_BYTES;
+          const uint32_t a_lo = tiles_lo + stage * (SB >> 4);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < GBK / 16; ++kk) {
-            umma_bf16(d_tmem, sw128_desc(a_addr + kk * 32, 16, 1024), sw128_desc(b_addr + kk * 32, 16, 1024), idesc,
-                      (kb | kk) != 0);
+            for (int kk = 0; kk < GBK / 16; ++kk)
+              umma_bf16_w(d_tmem, a_lo + kk * 2, a_lo + (G_A_BYTES >> 4) + kk * 2, sw128_hi(1024), idesc, (kb | kk) != 0);
+            umma_commit(empty0 + 8 * stage);
           }
-          umma_commit(empty0 + 8 * stage);
+          __syncwarp();
           if (++stage == GSTAGES) {
             stage = 0;
             phase ^= 1;
@@ -506,62 +605,77 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
           tile_origin(tile, num_m, num_n, bn, m0, n0);
           pdl_wait();
           const uint32_t* mask = lora->step_mask + m0 / GBM * LORA_MASK_WORDS;
-          for (int c = 0; ok && c < lora->cols / LORA_CHUNK; ++c) {
+          const bool mixed = __ldg(lora->mixed + m0 / GBM) != 0;
+          for (int c = 0, n = 0; ok && c < lora->cols / LORA_CHUNK; ++c) {
             const uint32_t steps = lora_chunk_steps(mask, c);
-            if (!steps) continue;
+            if (!steps || n++ % lora->ksplit != krank) continue;
             for (int pl = 0; pl < lora->planes; ++pl) {
-              if (!mbar_wait(full0 + 8 * stage, phase, abort_flag, err, kErrTimeoutGemmMma) ||
-                  !mbar_wait(u_ok0 + 8 * stage, (u_ok_ph >> stage) & 1, abort_flag, err, kErrTimeoutGemmMma)) {
+              if (!mbar_wait_warp(full0 + 8 * stage, phase, abort_flag, err, kErrTimeoutGemmMma) ||
+                  (mixed && !mbar_wait_warp(u_ok0 + 8 * stage, (u_ok_ph >> stage) & 1, abort_flag, err, kErrTimeoutGemmMma))) {
                 ok = false;
                 break;
               }
-              u_ok_ph ^= 1u << stage;
-              bad |= lora_bad[2 * stage] | lora_bad[2 * stage + 1];
+              if (mixed) {
+                u_ok_ph ^= 1u << stage;
+                bad |= lora_bad[2 * stage] | lora_bad[2 * stage + 1];
+              }
               tc_fence_after();
-              const uint32_t a_addr = tiles + stage * SB;
-              const uint32_t b_addr = a_addr + G_A_BYTES;
+              const uint32_t a_lo = tiles_lo + stage * (SB >> 4);
+              if (elect_one()) {
 #pragma unroll
-              for (int kk = 0; kk < LORA_CHUNK / LORA_STEP; ++kk)
-                if ((steps >> kk) & 1u)
-                  umma_bf16(d_tmem, sw128_desc(a_addr + kk * 32, 16, 1024), sw128_desc(b_addr + kk * 32, 16, 1024), idesc,
-                            true);
-              umma_commit(empty0 + 8 * stage);
+                for (int kk = 0; kk < LORA_CHUNK / LORA_STEP; ++kk)
+                  if ((steps >> kk) & 1u)
+                    umma_bf16_w(d_tmem, a_lo + kk * 2, a_lo + (G_A_BYTES >> 4) + kk * 2, sw128_hi(1024), idesc, true);
+                umma_commit(empty0 + 8 * stage);
+              }
+              __syncwarp();
               if (++stage == GSTAGES) {
                 stage = 0;
                 phase ^= 1;
               }
             }
           }
-          lora_tile_bad[acc] = bad;
+          if (lane == 0) lora_tile_bad[acc] = bad;
         }
         if (!ok) break;
-        if constexpr (LORA) mbar_arrive(tfull0 + 8 * acc);
-        umma_commit(tfull0 + 8 * acc);
+        if constexpr (LORA) {
+          if (lane == 0) mbar_arrive(tfull0 + 8 * acc);
+          __syncwarp();
+        }
+        if (elect_one()) umma_commit(tfull0 + 8 * acc);
+        __syncwarp();
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
       // every UMMA issued by this thread has completed once done_bar flips
-      umma_commit(done_bar);
+      if (elect_one()) umma_commit(done_bar);
+      __syncwarp();
       mbar_drain(done_bar, 0, err);
     }
   } else if (LORA && warp >= 2 + G_EPI_WARPS) {
     // Two warps look through the up-projection tiles: h = 0 keeps a row clear of another adapter's
     // finite weights, but 0 * NaN does not, so non-finite weights are zeroed before the MMA and added
-    // by the epilogue to the rows whose adapter has them.  The producer announces each such stage
+    // by the epilogue to the rows whose adapter has them; a tile whose rows all use one adapter needs
+    // none of it.  The producer announces each such stage
     // (u_req), so these warps pass over the others without a wait: its phases move only with the
     // stages they handle, and neither they nor `full` can get a phase ahead before u_ok is given.
     if constexpr (LORA) {
       int load = 0;         // stage loads before this point
       uint32_t req_ph = 0;  // phase of u_req per stage
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
+      for (int tile = tile0; ok && tile < num_tiles; tile += tile_step) {
         int m0, n0;
         tile_origin(tile, num_m, num_n, bn, m0, n0);
         load += kblocks;
         pdl_wait();
         const uint32_t* mask = lora->step_mask + m0 / GBM * LORA_MASK_WORDS;
-        for (int c = 0; ok && c < lora->cols / LORA_CHUNK; ++c) {
-          if (!lora_chunk_steps(mask, c)) continue;
+        const bool mixed = __ldg(lora->mixed + m0 / GBM) != 0;
+        for (int c = 0, n = 0; ok && c < lora->cols / LORA_CHUNK; ++c) {
+          if (!lora_chunk_steps(mask, c) || n++ % lora->ksplit != krank) continue;
+          if (!mixed) {
+            load += lora->planes;
+            continue;
+          }
           for (int pl = 0; pl < lora->planes; ++pl, ++load) {
             const int stage = load % GSTAGES;
             ok = mbar_wait_warp(u_req0 + 8 * stage, (req_ph >> stage) & 1, abort_flag, err, kErrTimeoutGemmProducer) &&
@@ -570,17 +684,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
             req_ph ^= 1u << stage;
             uint8_t* u = smem + (size_t)stage * SB + G_A_BYTES;
             int hit = 0;
-            for (int r = (warp & 1) * 32 + lane; r < bn; r += 64) {
-#pragma unroll
-              for (int q = 0; q < 8; ++q) {  // 16-byte groups in an order that spreads a quarter-warp over the banks
-                uint4* pq = reinterpret_cast<uint4*>(u + r * 128 + (((q + lane) & 7) << 4));
-                const uint4 v = *pq;
-                if (nonfinite_bf16x2(v.x) | nonfinite_bf16x2(v.y) | nonfinite_bf16x2(v.z) | nonfinite_bf16x2(v.w)) {
-                  *pq = make_uint4(zero_nonfinite(v.x), zero_nonfinite(v.y), zero_nonfinite(v.z), zero_nonfinite(v.w));
-                  hit = 1;
-                }
-              }
-            }
+            for (int r = (warp & 1) * 32 + lane; r < bn; r += 64) hit |= clean_row128(u + r * 128, lane);
             if (hit) fence_proxy_async_smem();
             hit = __any_sync(0xffffffffu, hit);
             if (lane == 0) {
@@ -597,13 +701,37 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
     const int r = quad * 32 + lane;
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x) {
-      if (!mbar_wait_warp(tfull0 + 8 * acc, acc_phase, abort_flag, err, kErrTimeoutGemmEpilogue)) break;
+    for (int tile = tile0; tile < num_tiles; tile += tile_step) {
+      const bool done = mbar_wait_warp(tfull0 + 8 * acc, acc_phase, abort_flag, err, kErrTimeoutGemmEpilogue);
       tc_fence_after();
+      const uint32_t t_row = tmem_base + (uint32_t(quad * 32) << 16) + acc * GBN;
+      if constexpr (LORA) {
+        if (lora->ksplit > 1) {
+          if (done) {  // the ring is free: every MMA of this block has completed
+            for (int c = half; c < bn / 32; c += 2) {
+              float v[32];
+              tmem_ld32(t_row + c * 32, v);
+              float4* part = reinterpret_cast<float4*>(smem + lora_part_offset(bn, r, c * 32));
+#pragma unroll
+              for (int q = 0; q < 8; ++q) part[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+            }
+          }
+          cluster_sync_all();  // the sums of all ranks are there
+          if (done) {
+            int m0, n0;
+            tile_origin(tile, num_m, num_n, bn, m0, n0);
+            int bad = 0;
+            for (int k = 0; k < lora->ksplit; ++k) bad |= ld_cluster_int(smem_u32(lora_tile_bad), k);
+            lora_join_rows<EPI>(args, lora, tiles, bad != 0, m0, n0, krank,
+                                (warp - 2) * 32 + lane);
+          }
+          break;  // a cluster has one tile
+        }
+      }
+      if (!done) break;
       int m0, n0;
       tile_origin(tile, num_m, num_n, bn, m0, n0);
       const int row = m0 + r;
-      const uint32_t t_row = tmem_base + (uint32_t(quad * 32) << 16) + acc * GBN;
       bool slow = false;
       if constexpr (LORA) slow = *reinterpret_cast<volatile int*>(lora_tile_bad + acc) != 0;
       if constexpr (EPI == WANB200_EPI_SCATTER) {
@@ -671,6 +799,12 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
     }
   }
 
+  if constexpr (LORA) {
+    if (lora->ksplit > 1) {
+      if (warp < 2 || warp >= 2 + G_EPI_WARPS) cluster_sync_all();  // the epilogue warps did so above
+      cluster_sync_all();  // the sums have been read
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -713,11 +847,14 @@ static int launch_gemm_lora(const CUtensorMap& ta, const CUtensorMap& tb, const 
   cfg.blockDim = dim3(G_LORA_THREADS);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)lora.ksplit;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = lora.ksplit > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_lora_kernel<EPI>, ta, tb, th, tu, ga, lora);
   if (e != cudaSuccess) return set_cuda_error("gemm_lora_kernel launch", e);
   return WANB200_OK;
@@ -747,11 +884,11 @@ static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const GemmA
 // smallest makespan waves * (BN + c), waves = ceil(tiles / SMs) over the persistent grid.  c
 // stands for the per-tile cost that does not shrink with BN (the A tile loads, the accumulator
 // hand-off); it keeps BN at 256 unless a narrower tile removes a mostly empty last wave.
-static int choose_tile_n(int64_t M, int64_t N, int sms, int narrowest) {
+static int choose_tile_n(int64_t M, int64_t N, int sms) {
   const int64_t num_m = (M + GBM - 1) / GBM;
   int best = GBN;
   double best_t = 1e300;
-  for (int bn = GBN; bn >= narrowest; bn -= 32) {
+  for (int bn = GBN; bn >= 128; bn -= 32) {
     const int64_t tiles = num_m * ((N + bn - 1) / bn);
     const double t = (double)((tiles + sms - 1) / sms) * (bn + 64.0);
     if (t < best_t - 1e-9) {
@@ -823,7 +960,7 @@ int gemm_launch(const wanb200_gemm_params* p, const LoraPlan* lora, int* err, cu
   const int epi = p->epilogue;
   const bool scatter = epi == WANB200_EPI_SCATTER;
   const int sms = num_sms();
-  const int bn = p->tile_n ? p->tile_n : choose_tile_n(p->M, p->N, sms, lora ? 64 : 128);
+  const int bn = lora ? lora->bn : p->tile_n ? p->tile_n : choose_tile_n(p->M, p->N, sms);
   CUtensorMap ta, tb;
   int rc = make_tmap_2d(&ta, p->a, p->K, p->M, p->lda, GBK, GBM);
   if (rc) return rc;
@@ -874,7 +1011,7 @@ int gemm_launch(const wanb200_gemm_params* p, const LoraPlan* lora, int* err, cu
   ga.err = err;
 
   const int64_t tiles = ((p->M + GBM - 1) / GBM) * ((p->N + bn - 1) / bn);
-  const int grid = (int)std::min<int64_t>(tiles, sms);
+  const int grid = lora ? lora->grid : (int)std::min<int64_t>(tiles, sms);
   if (lora) {
     CUtensorMap th, tu;
     rc = make_tmap_2d(&th, lora->h, lora->cols, lora->planes * lora->rows_pad, lora->cols, GBK, GBM);

@@ -9,14 +9,10 @@
 #include <atomic>
 #include <type_traits>
 
-#include <cooperative_groups.h>
-
 #include "common.cuh"
 #include "lora.h"
 
 namespace wanb200 {
-
-namespace cg = cooperative_groups;
 
 constexpr int LD_THREADS = 192;  // TMA, MMA, 4 epilogue warps
 constexpr int LD_BM = 128, LD_BK = 64, LD_GROUP = 4;  // chunks of one pass: N = 256
@@ -33,6 +29,7 @@ struct LoraDownArgs {
   int adapters, rank, cols, planes, kblocks_per_rank;
   int64_t rows_pad;
   uint32_t* step_mask;
+  int* mixed;
   __nv_bfloat16* h;
   int* err;
 };
@@ -79,7 +76,6 @@ __global__ void __launch_bounds__(LD_THREADS, 1)
   __shared__ int chunks[LORA_MAX_COLS / LORA_CHUNK];
   __shared__ int num_chunks;
   pdl_launch();  // the GEMM behind starts its own K loop; it waits for this kernel before it reads h
-  cg::cluster_group cluster = cg::this_cluster();
   const int krank = blockIdx.x, ksize = gridDim.x, m0 = blockIdx.y * LD_BM;
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sbase = smem_u32(smem);
@@ -126,6 +122,9 @@ __global__ void __launch_bounds__(LD_THREADS, 1)
   tc_fence_after();
   if (threadIdx.x < LORA_MASK_WORDS && krank == 0)
     a.step_mask[blockIdx.y * LORA_MASK_WORDS + threadIdx.x] = bits[threadIdx.x];
+  const int differs = threadIdx.x < LD_BM && m0 + (int)threadIdx.x < a.M && ids[threadIdx.x] != ids[0];
+  if (__syncthreads_or(differs) && threadIdx.x == 0 && krank == 0) a.mixed[blockIdx.y] = 1;
+  else if (threadIdx.x == 0 && krank == 0) a.mixed[blockIdx.y] = 0;
   if (threadIdx.x == 0) {
     int n = 0;
     for (int c = 0; c < a.cols / LORA_CHUNK; ++c)
@@ -141,40 +140,43 @@ __global__ void __launch_bounds__(LD_THREADS, 1)
 
   for (int pass = 0; pass < passes; ++pass) {
     const int c0 = pass * LD_GROUP, nc = min(LD_GROUP, num_chunks - c0);
+    // (the whole warp walks the issue loops: see elect_one)
     if (warp == 0) {
-      if (lane == 0) {
-        for (int kb = 0; kb < kblocks; ++kb) {
-          if (!mbar_wait(empty0 + 8 * stage, ph ^ 1, abort_flag, err, kErrTimeoutGemmProducer)) break;
-          const uint32_t dst = sbase + stage * LD_STAGE_BYTES;
+      for (int kb = 0; kb < kblocks; ++kb) {
+        if (!mbar_wait_warp(empty0 + 8 * stage, ph ^ 1, abort_flag, err, kErrTimeoutGemmProducer)) break;
+        const uint32_t dst = sbase + stage * LD_STAGE_BYTES;
+        if (elect_one()) {
           mbar_expect_tx(full0 + 8 * stage, LD_BM * LD_BK * 2 + nc * LORA_CHUNK * LD_BK * 2);
           tma_load_2d(dst, &tmX, full0 + 8 * stage, (kb0 + kb) * LD_BK, m0);
           for (int c = 0; c < nc; ++c)
             tma_load_2d(dst + LD_BM * LD_BK * 2 + c * LORA_CHUNK * LD_BK * 2, &tmD, full0 + 8 * stage, (kb0 + kb) * LD_BK,
                         chunks[c0 + c] * LORA_CHUNK);
-          issued |= 1u << stage;
-          last_ph = (last_ph & ~(1u << stage)) | (ph << stage);
-          if (++stage == LD_STAGES) stage = 0, ph ^= 1;
         }
+        __syncwarp();
+        issued |= 1u << stage;
+        last_ph = (last_ph & ~(1u << stage)) | (ph << stage);
+        if (++stage == LD_STAGES) stage = 0, ph ^= 1;
       }
     } else if (warp == 1) {
-      if (lane == 0) {
-        const uint32_t idesc = idesc_bf16_f32(LD_BM, nc * LORA_CHUNK, false, false);
-        bool ok = mbar_wait(tempty, (pass & 1) ^ 1, abort_flag, err, kErrTimeoutGemmMma);
+      const uint32_t idesc = idesc_bf16_f32(LD_BM, nc * LORA_CHUNK, false, false);
+      bool ok = mbar_wait_warp(tempty, (pass & 1) ^ 1, abort_flag, err, kErrTimeoutGemmMma);
+      tc_fence_after();
+      for (int kb = 0; ok && kb < kblocks; ++kb) {
+        ok = mbar_wait_warp(full0 + 8 * stage, ph, abort_flag, err, kErrTimeoutGemmMma);
+        if (!ok) break;
         tc_fence_after();
-        for (int kb = 0; ok && kb < kblocks; ++kb) {
-          ok = mbar_wait(full0 + 8 * stage, ph, abort_flag, err, kErrTimeoutGemmMma);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t x_addr = sbase + stage * LD_STAGE_BYTES, d_addr = x_addr + LD_BM * LD_BK * 2;
+        const uint32_t x_lo = sw128_lo(sbase, 16) + stage * (LD_STAGE_BYTES >> 4), d_lo = x_lo + (LD_BM * LD_BK * 2 >> 4);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < LD_BK / 16; ++kk)
-            umma_bf16(tmem_base, sw128_desc(x_addr + kk * 32, 16, 1024), sw128_desc(d_addr + kk * 32, 16, 1024), idesc,
-                      (kb | kk) != 0);
+            umma_bf16_w(tmem_base, x_lo + kk * 2, d_lo + kk * 2, sw128_hi(1024), idesc, (kb | kk) != 0);
           umma_commit(empty0 + 8 * stage);
-          if (++stage == LD_STAGES) stage = 0, ph ^= 1;
         }
-        if (ok) umma_commit(tfull);
+        __syncwarp();
+        if (++stage == LD_STAGES) stage = 0, ph ^= 1;
       }
+      if (ok && elect_one()) umma_commit(tfull);
+      __syncwarp();
     } else {
       const int quad = warp & 3, r = quad * 32 + lane, row = m0 + r;
       const int id = ids[r];
@@ -205,31 +207,48 @@ __global__ void __launch_bounds__(LD_THREADS, 1)
       mbar_arrive(tempty);
     }
     if (ksize > 1) {
-      __syncwarp();
-      cluster.sync();
-      const int per = LD_BM / ksize, groups = nc * LORA_CHUNK / 4;
+      cluster_sync_all();
+      // Each block takes its share of the rows.  Reads from the other SMs are slow (12 bytes a clock were
+      // measured), so of a row only its own adapter's columns are read; the others are zero.
+      const int per = LD_BM / ksize, own = a.rank / 4;
+      for (int i = threadIdx.x; i < per * own; i += LD_THREADS) {
+        const int r = krank * per + i / own, row = m0 + r, id = ids[r];
+        if (row >= a.M || id < 0) continue;
+        const int first = id * a.rank, col = first + i % own * 4;
+        int g = -1;
+        for (int c = 0; c < nc; ++c)
+          if (chunks[c0 + c] == col / LORA_CHUNK) g = c;
+        if (g < 0) continue;  // another pass has these columns
+        const uint32_t at = sbase + (r * LD_RED_LD + g * LORA_CHUNK + col % LORA_CHUNK) * 4;
+        float4 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < ksize) x[k] = ld_cluster16(at, k);
+        float4 sum = x[0];
+#pragma unroll
+        for (int k = 1; k < 8; ++k)  // in order, so that the sum is the same in every run
+          if (k < ksize) sum.x += x[k].x, sum.y += x[k].y, sum.z += x[k].z, sum.w += x[k].w;
+        lora_store_h(a, row, col, sum, first, first + a.rank, a.scales ? __ldg(a.scales + id) : 1.f);
+      }
+      const int groups = nc * LORA_CHUNK / 8;
       for (int i = threadIdx.x; i < per * groups; i += LD_THREADS) {
-        const int r = krank * per + i / groups, g = i % groups, row = m0 + r;
-        if (row >= a.M) continue;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = 0; k < ksize; ++k) {  // in order, so that the sum is the same in every run
-          const float4 v = *cluster.map_shared_rank(reinterpret_cast<float4*>(smem + (r * LD_RED_LD + g * 4) * 4), k);
-          sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-        }
-        const int id = ids[r];
-        lora_store_h(a, row, chunks[c0 + (g >> 4)] * LORA_CHUNK + (g & 15) * 4, sum, id < 0 ? 0 : id * a.rank,
-                     id < 0 ? 0 : (id + 1) * a.rank, id >= 0 && a.scales ? __ldg(a.scales + id) : 1.f);
+        const int r = krank * per + i / groups, g = i % groups, row = m0 + r, id = ids[r];
+        const int col = chunks[c0 + g / 8] * LORA_CHUNK + g % 8 * 8;
+        if (row >= a.M || (id >= 0 && col >= id * a.rank && col < (id + 1) * a.rank)) continue;
+        for (int pl = 0; pl < a.planes; ++pl)
+          *reinterpret_cast<uint4*>(a.h + (pl * a.rows_pad + row) * a.cols + col) = make_uint4(0u, 0u, 0u, 0u);
       }
       fence_proxy_async_smem();  // the next pass's loads overwrite what was read and written here
-      cluster.sync();
+      cluster_sync_all();
     }
   }
   if (warp == 0 && lane == 0 && *abort_flag) {  // let every load in flight land
     for (int s = 0; s < LD_STAGES; ++s)
       if ((issued >> s) & 1) mbar_drain(full0 + 8 * s, (last_ph >> s) & 1, err);
   }
-  if (warp == 1 && lane == 0) {
-    umma_commit(done_bar);
+  if (warp == 1) {
+    if (elect_one()) umma_commit(done_bar);
+    __syncwarp();
     mbar_drain(done_bar, 0, err);
   }
   tc_fence_before();
@@ -466,7 +485,7 @@ static int lora_few(const wanb200_lora_params* p, float* h, int* err, cudaStream
 
 // ------------------------------------------------------------------ host launcher
 struct LoraLayout {
-  int64_t rows_pad, num_m, h_off, bytes;
+  int64_t rows_pad, num_m, mixed_off, h_off, bytes;
   int cols, planes;
 };
 
@@ -481,7 +500,8 @@ static LoraLayout lora_layout(int64_t M, int adapters, int rank, int out_f32) {
   l.rows_pad = l.num_m * LD_BM;
   l.cols = (adapters * rank + LORA_CHUNK - 1) / LORA_CHUNK * LORA_CHUNK;
   l.planes = out_f32 ? 2 : 1;
-  l.h_off = (l.num_m * LORA_MASK_WORDS * 4 + 255) / 256 * 256;
+  l.mixed_off = l.num_m * LORA_MASK_WORDS * 4;
+  l.h_off = (l.mixed_off + l.num_m * 4 + 255) / 256 * 256;
   l.bytes = l.h_off + l.planes * l.rows_pad * l.cols * 2;
   return l;
 }
@@ -493,6 +513,48 @@ static bool lora_sizes_ok(int64_t M, int adapters, int rank) {
 
 int64_t lora_workspace_bytes(int64_t M, int adapters, int rank, int out_f32) {
   return lora_sizes_ok(M, adapters, rank) ? lora_layout(M, adapters, rank, out_f32).bytes : 0;
+}
+
+// Blocks per row tile of the down-projection, and the GEMM's tile width, K split and grid, by a cost
+// model in which a K block of 64 costs max(200, width) of a tile (the loads into an SM bound narrow
+// tiles, the tensor pipe 256-wide ones: about 215 and 280 ns) and 300 in the down-projection, whose
+// fixed part weighs 3000.
+// The two kernels run side by side where the SMs beside the down-projection's suffice for the GEMM
+// (it waits for h only at the end of its first K loop), else one after the other.  Few tiles
+// share K over a cluster; its join reads (ks - 1) / ks of a tile from other SMs.
+struct LoraLaunch {
+  int down_ksize, bn, ksplit, grid;
+};
+
+static LoraLaunch lora_plan_launch(int64_t M, int64_t N, int kblocks, int tile_n, int sms) {
+  const int64_t num_m = (M + LD_BM - 1) / LD_BM;
+  LoraLaunch best = {};
+  double best_t = 1e300;
+  auto shares = [&](int k) { return (kblocks + k - 1) / k; };
+  for (int ds = 1; ds <= 8; ds *= 2) {
+    if (ds > 1 && ((int64_t)(ds - 1) * shares(ds) >= kblocks || shares(ds) < 4 || num_m * ds > sms)) break;
+    const int64_t down_blocks = num_m * ds;
+    const double down = (double)((down_blocks + sms - 1) / sms) * (shares(ds) * 300.0 + 3000.0);
+    for (int bn = tile_n ? tile_n : 256; bn >= (tile_n ? tile_n : 128); bn -= 32) {
+      const int64_t tiles = num_m * ((N + bn - 1) / bn);
+      const double kb = std::max(200, bn);
+      for (int ks = 1; ks <= 4; ks *= 2) {
+        if (ks > 1 && ((int64_t)(ks - 1) * shares(ks) >= kblocks || shares(ks) < 4 || tiles * ks > sms)) break;
+        const double tile = shares(ks) * kb + (ks > 1 ? 40.0 * bn * (ks - 1) / ks : 0.0) + 64.0 * shares(ks);
+        for (int beside = 0; beside < 2; ++beside) {
+          const int64_t room = beside ? sms - down_blocks : sms;
+          if (room < ks || (ks > 1 && tiles * ks > room)) continue;
+          const double t = beside ? std::max((double)((tiles + room - 1) / room) * tile, down + 1600.0)
+                                  : down + (double)((tiles + sms - 1) / sms) * tile;
+          if (t < best_t - 1e-9) {
+            best_t = t;
+            best = {ds, bn, ks, (int)(ks > 1 ? tiles * ks : std::min<int64_t>(tiles, room))};
+          }
+        }
+      }
+    }
+  }
+  return best;
 }
 
 int gemm_lora(const wanb200_lora_params* p, cudaStream_t st) {
@@ -530,17 +592,12 @@ int gemm_lora(const wanb200_lora_params* p, cudaStream_t st) {
   a.planes = l.planes;
   a.rows_pad = l.rows_pad;
   a.step_mask = reinterpret_cast<uint32_t*>(ws);
+  a.mixed = reinterpret_cast<int*>(ws + l.mixed_off);
   a.h = reinterpret_cast<__nv_bfloat16*>(ws + l.h_off);
   a.err = err;
-  // blocks along K: as many as bring the row tiles to the SM count, at least 4 K blocks each
-  const int kblocks = a.K / LD_BK;
-  int ksize = 1;
-  while (ksize < 8 && l.num_m * ksize * 2 <= num_sms() && kblocks >= ksize * 2 * 4) ksize *= 2;
-  a.kblocks_per_rank = (kblocks + ksize - 1) / ksize;
-  while ((ksize - 1) * a.kblocks_per_rank >= kblocks) {  // no block without work
-    ksize /= 2;
-    a.kblocks_per_rank = (kblocks + ksize - 1) / ksize;
-  }
+  const LoraLaunch pl = lora_plan_launch(g->M, g->N, a.K / LD_BK, g->tile_n, num_sms());
+  const int ksize = pl.down_ksize;
+  a.kblocks_per_rank = (a.K / LD_BK + ksize - 1) / ksize;
   static std::atomic<bool> attr_set[kMaxDevices] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -566,6 +623,7 @@ int gemm_lora(const wanb200_lora_params* p, cudaStream_t st) {
   if (e != cudaSuccess) return set_cuda_error("lora_down_kernel launch", e);
   LoraPlan plan;
   plan.step_mask = a.step_mask;
+  plan.mixed = a.mixed;
   plan.h = a.h;
   plan.up = reinterpret_cast<const __nv_bfloat16*>(p->up);
   plan.ids = a.ids;
@@ -574,6 +632,9 @@ int gemm_lora(const wanb200_lora_params* p, cudaStream_t st) {
   plan.cols = a.cols;
   plan.planes = a.planes;
   plan.rows_pad = a.rows_pad;
+  plan.bn = pl.bn;
+  plan.ksplit = pl.ksplit;
+  plan.grid = pl.grid;
   return gemm_launch(g, &plan, err, st);
 }
 

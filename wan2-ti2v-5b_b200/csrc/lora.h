@@ -11,14 +11,16 @@ namespace wanb200 {
 constexpr int LORA_STEP = 16, LORA_CHUNK = 64, LORA_MAX_COLS = 4096;
 constexpr int LORA_MASK_WORDS = LORA_MAX_COLS / LORA_STEP / 32;  // 8 words of step bits per row tile
 
-// Workspace of one call: [row tiles][8] step bits | h planes.
+// Workspace of one call: [row tiles][8] step bits | [row tiles] mixed | h planes.
 struct LoraPlan {
   const uint32_t* step_mask;  // steps that some row of the tile uses
+  const int* mixed;           // the tile's rows do not all use one adapter
   const __nv_bfloat16* h;     // [planes][rows_pad][cols]: scale * (x . down^T) in bf16 planes that add up
   const __nv_bfloat16* up;    // [N][adapters * rank]
   const int32_t* ids;
   int adapters, rank, cols, planes;
   int64_t rows_pad;
+  int bn, ksplit, grid;  // the GEMM's tile width, blocks that share a tile's K (a cluster), blocks
 };
 
 }  // namespace wanb200
