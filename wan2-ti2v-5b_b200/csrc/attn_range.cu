@@ -16,14 +16,10 @@
 // added one by one to the rows that do see them (never with finite values).
 #include <atomic>
 
-#include <cooperative_groups.h>
-
 #include "common.cuh"
 #include "internal.h"
 
 namespace wanb200 {
-
-namespace cg = cooperative_groups;
 
 constexpr float RA_LOG2E = 1.4426950408889634f;
 constexpr float RA_RESCALE = 8.f;  // log2 units by which a maximum must grow before sums are rescaled
@@ -43,6 +39,17 @@ struct RangeArgs {
   const float* slopes;  // [heads]
   const float* table;   // [heads, 2 * reach + 1]
   int reach;
+};
+
+// Unnormalised results of the key splits, to be merged by range_combine_kernel: slot i holds one
+// split's [slot_rows][D] outputs and [slot_rows] (maximum in log2 units, sum; sum = -1 and no output
+// where the split saw no key tile).  The splits of row group x (slot_rows rows of one batch element and
+// key head) are the slots first[x].x + k * first[x].z for k < first[x].y.
+struct RangeParts {
+  float* o;
+  float2* ml;
+  int4* first;   // written by the few-rows kernel; null: (x, splits, groups) for every x
+  int slot_rows, groups, splits;
 };
 
 __device__ __forceinline__ void row_range(const RangeArgs& a, int b, int i, int& lo, int& hi) {
@@ -82,199 +89,265 @@ __device__ __forceinline__ float score_log2(const RangeArgs& a, float s, int h, 
 }
 
 // ================================================================== few rows: one pass over K and V
-// One cluster of blocks per (key head, batch element); the warps of a cluster take blocks of 16 keys in
-// turn and keep their own running maximum, sum and output, merged at the end over the block's
-// shared memory and then over the cluster's.  K and V pass through a ring of asynchronous copies,
-// each lane's own 16-byte pieces, to the operand registers of mma.sync m16n8k16 (16 rows x 16
-// keys): a dot product does not care about the order of its channels, so a lane's piece is taken as
-// the operand of two K steps, q permuted alike, and the output channels come out permuted the same
-// way.  The tensor work is far below the bandwidth bound, so the warp-level MMA is enough here.
-constexpr int RD_WARPS = 4, RD_KEYS = 16, RD_STAGES = 2, RD_BLOCKS = 3;
+// Several blocks per (key head, batch element) take tiles of 64 keys in turn: one warp feeds a ring of
+// K and V tiles by TMA, four warps take 16 keys of each tile and keep their own running maximum, sum
+// and output, merged at the end over the block's shared memory, and over the blocks by
+// range_combine_kernel.  The batch elements' key counts differ, so every block reads them all and
+// the blocks are dealt out in equal shares of keys.  (With cp.async or plain loads by the warps
+// themselves the reads stopped at 4.1 TB/s whatever the depth of the ring.)  The operands of mma.sync
+// m16n8k16 are transposed: S^T (16 keys x 8 rows) = K Q^T and O^T (16 channels x 8 rows) += V^T P^T, so
+// that up to 8 rows cost one MMA column tile and nothing of it is wasted.  A dot product does not
+// care about the order of its channels: a lane's 16 bytes of K are taken as the operand of two K
+// steps, q permuted alike, and the output channels come out permuted as the pieces of V lie.  The
+// tensor work is far below the bandwidth bound, so the warp-level MMA is enough; what counts is few
+// instructions for each 16 keys (about 200; with rows as the MMA's 16-row side it was 565).
+constexpr int RD_WARPS = 4, RD_KEYS = 16, RD_TILE = RD_WARPS * RD_KEYS;
+constexpr int RD_THREADS = (RD_WARPS + 1) * 32;
+constexpr int RD_SHARE = 2;   // key tiles of a block at least
+constexpr int RD_BLOCKS = 3;  // blocks an SM holds (by shared memory; two with 9 to 16 rows, by registers)
 
 template <int D>
 struct RangeDecodeCfg {
-  static constexpr int KC = D / 32, VC = D / 64;     // 16-byte pieces per K row, per V row
-  static constexpr int PIECES = 2 * KC + 4 * VC;     // of a lane in one stage: 2 K rows, 4 V rows
-  static constexpr int RING = RD_WARPS * RD_STAGES * PIECES * 512;
+  static constexpr int HALF = RD_TILE * 128;               // 64 channels of a tile: 128-byte swizzled rows
+  static constexpr int STAGE = 2 * (D / 64) * HALF;        // K, then V
+  static constexpr int STAGES = D == 128 ? 2 : 4;
+  static constexpr int RING = STAGES * STAGE;              // 64 KB
+  static constexpr int SMEM = RING + 1024;
 };
 
-template <int D, bool TWO, bool CAP, int BIAS>  // TWO: 9 to 16 rows (the second half of the MMA's rows is used)
-__global__ void __launch_bounds__(RD_WARPS * 32, RD_BLOCKS) range_decode_kernel(const RangeArgs a) {
-  constexpr int KC = RangeDecodeCfg<D>::KC, VC = RangeDecodeCfg<D>::VC, PIECES = RangeDecodeCfg<D>::PIECES;
-  constexpr int HR = TWO ? 2 : 1;          // rows held by a lane: lane / 4 and, with TWO, lane / 4 + 8
-  constexpr int ROWS = TWO ? 16 : 8;
-  // the ring [warp][stage][piece][lane], and after it the warps' outputs
-  extern __shared__ uint4 ring[];
-  float(*o_sh)[ROWS][D + 4] = reinterpret_cast<float(*)[ROWS][D + 4]>(ring);
-  static_assert(RD_WARPS * ROWS * (D + 4) * 4 <= RangeDecodeCfg<D>::RING, "the outputs reuse the ring");
+__device__ __forceinline__ int decode_key_tiles(const RangeArgs& a, int b) {
+  int from = INT32_MAX, to = 0;
+  for (int t = 0; t < a.q_len; ++t) {
+    int lo, hi;
+    row_range(a, b, t, lo, hi);
+    if (lo < hi) from = min(from, lo), to = max(to, hi);
+  }
+  return from < to ? (to - from + RD_TILE - 1) / RD_TILE : 0;
+}
+
+template <int D, bool TWO, bool CAP, int BIAS>  // TWO: 9 to 16 rows, two column tiles
+__global__ void __launch_bounds__(RD_THREADS, TWO ? 2 : RD_BLOCKS)
+    range_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                        const __grid_constant__ RangeArgs a, const __grid_constant__ RangeParts out, const int slots, int* err) {
+  using C = RangeDecodeCfg<D>;
+  constexpr int KC = D / 32, VC = D / 64;         // 16-byte pieces per K row, per V row of a lane
+  constexpr int NR = TWO ? 2 : 1, ROWS = 8 * NR;  // a lane holds rows 8 x + 2 q4 + y (x < NR, y < 2)
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // the ring, after it the warps' outputs
+  const uint32_t sbase = smem_u32(smem);
+  float(*o_sh)[ROWS][D + 4] = reinterpret_cast<float(*)[ROWS][D + 4]>(smem);
+  static_assert(RD_WARPS * ROWS * (D + 4) * 4 <= C::RING, "the outputs reuse the ring");
   __shared__ float2 ml_sh[RD_WARPS][ROWS];
-  __shared__ float o_cta[ROWS][D];
-  __shared__ float2 ml_cta[ROWS];
-  cg::cluster_group cluster = cg::this_cluster();
+  __shared__ uint64_t bars[2 * C::STAGES];
+  __shared__ int abort_word;
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * C::STAGES;
+  volatile int* abort_flag = &abort_word;
+  pdl_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, q4 = lane & 3;
-  const int b = blockIdx.z, kh = blockIdx.y, csize = gridDim.x, crank = blockIdx.x;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::STAGES; ++i) {
+      mbar_init(full0 + 8 * i, 1);
+      mbar_init(empty0 + 8 * i, RD_WARPS);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
   const int rows = a.q_len * a.group;
+  int b = (int)blockIdx.x / a.kv_heads, kh = (int)blockIdx.x % a.kv_heads, csize = 1, crank = 0;
+  if (slots > 0) {  // else one block for each (key head, batch element)
+    __shared__ int deal[4];  // batch element, its first block, its blocks of each head; -1 = none left
+    if (threadIdx.x < 32) {
+      // tiles of every batch element (all heads alike), then the share of one block
+      const int mine = lane < a.batch ? decode_key_tiles(a, lane) : 0;
+      int total = mine;
+      for (int i = lane + 32; i < a.batch; i += 32) total += decode_key_tiles(a, i);
+      total = __reduce_add_sync(0xffffffffu, total);
+      const int64_t all = (int64_t)total * a.kv_heads;
+      const int each = (int)max((all + slots - 1) / slots, (int64_t)RD_SHARE);
+      int before = 0;
+      if (lane == 0) deal[0] = -1;
+      __syncwarp();
+      for (int i0 = 0; i0 < a.batch; i0 += 32) {
+        const int i = i0 + lane;
+        const int n = i < a.batch ? max(1, ((i0 ? decode_key_tiles(a, i) : mine) + each - 1) / each) : 0;
+        int sum = n;
+#pragma unroll
+        for (int w = 1; w < 32; w *= 2) {
+          const int v = __shfl_up_sync(0xffffffffu, sum, w);
+          if (lane >= w) sum += v;
+        }
+        const int first = (before + sum - n) * a.kv_heads;
+        if (n > 0 && (int)blockIdx.x >= first && (int)blockIdx.x < first + n * a.kv_heads)
+          deal[0] = i, deal[1] = first, deal[2] = n;
+        before += __shfl_sync(0xffffffffu, sum, 31);
+      }
+    }
+    __syncthreads();
+    b = deal[0];
+    if (b < 0) return;  // more blocks were launched than there are shares
+    csize = deal[2];
+    const int x = (int)blockIdx.x - deal[1];
+    kh = x % a.kv_heads;
+    crank = x / a.kv_heads;
+    if (crank == 0 && threadIdx.x == 0) out.first[b * a.kv_heads + kh] = make_int4((int)blockIdx.x, csize, a.kv_heads, 0);
+  } else {
+    __syncthreads();  // the barriers are set up
+  }
 
   // the rows' ranges: each lane's own, and over all rows what any and what all of them see
-  int lo[HR], hi[HR], pos[HR], head[HR];
+  int lo[NR][2], hi[NR][2], pos[NR][2], head[NR][2];
   int all_lo = 0, all_hi = INT32_MAX, any_lo = INT32_MAX, any_hi = 0;
 #pragma unroll
-  for (int x = 0; x < HR; ++x) {
-    const int r = g4 + 8 * x;
-    lo[x] = hi[x] = pos[x] = head[x] = 0;
-    if (r < rows) {
-      const int tok = r / a.group;
-      row_range(a, b, tok, lo[x], hi[x]);
-      pos[x] = row_pos(a, b, tok);
-      head[x] = kh * a.group + r % a.group;
-      if (lo[x] < hi[x]) {
-        any_lo = min(any_lo, lo[x]);
-        any_hi = max(any_hi, hi[x]);
+  for (int x = 0; x < NR; ++x)
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int r = 8 * x + 2 * q4 + y;
+      lo[x][y] = hi[x][y] = pos[x][y] = head[x][y] = 0;
+      if (r < rows) {
+        const int tok = r / a.group;
+        row_range(a, b, tok, lo[x][y], hi[x][y]);
+        pos[x][y] = BIAS == kBiasNone ? 0 : row_pos(a, b, tok);
+        head[x][y] = kh * a.group + r % a.group;
+        if (lo[x][y] < hi[x][y]) {
+          any_lo = min(any_lo, lo[x][y]);
+          any_hi = max(any_hi, hi[x][y]);
+        }
+        all_lo = max(all_lo, lo[x][y]);
+        all_hi = min(all_hi, hi[x][y]);
       }
-      all_lo = max(all_lo, lo[x]);
-      all_hi = min(all_hi, hi[x]);
     }
-  }
   all_lo = __reduce_max_sync(0xffffffffu, all_lo);
   all_hi = __reduce_min_sync(0xffffffffu, all_hi);
   any_lo = __reduce_min_sync(0xffffffffu, any_lo);
   any_hi = __reduce_max_sync(0xffffffffu, any_hi);
 
-  uint32_t qa[HR][2 * KC][2];  // A operand: [row half][K step][the two k pairs]
+  const int tiles = any_lo < any_hi ? (any_hi - any_lo + RD_TILE - 1) / RD_TILE : 0;
+  if (warp == RD_WARPS) {  // the whole warp walks the loop: see elect_one
+    int n = 0;
+    bool ok = true;
+    for (int t = crank; t < tiles; t += csize, ++n) {
+      const int stage = n % C::STAGES, key0 = any_lo + t * RD_TILE;
+      ok = mbar_wait_warp(empty0 + 8 * stage, ((n / C::STAGES) & 1) ^ 1, abort_flag, err, kErrTimeoutAttnProducer);
+      if (!ok) break;
+      if (elect_one()) {
+        const uint32_t dst = sbase + stage * C::STAGE;
+        mbar_expect_tx(full0 + 8 * stage, C::STAGE);
+        for (int h = 0; h < VC; ++h) {
+          tma_load_4d(dst + h * C::HALF, &tmK, full0 + 8 * stage, 64 * h, kh, key0, b);
+          tma_load_4d(dst + (VC + h) * C::HALF, &tmV, full0 + 8 * stage, 64 * h, kh, key0, b);
+        }
+      }
+      __syncwarp();
+    }
+    if (!ok)  // let every load in flight land before the block's shared memory goes away
+      for (int i = max(0, n - C::STAGES); i < n; ++i) mbar_drain(full0 + 8 * (i % C::STAGES), (i / C::STAGES) & 1, err);
+    __syncthreads();
+    __syncthreads();
+    return;
+  }
+
+  uint32_t qb[NR][2 * KC][2];  // B operand of S^T: row 8 x + g4, [K step][the two k pairs]
 #pragma unroll
-  for (int x = 0; x < HR; ++x) {
-    const int r = g4 + 8 * x;
+  for (int x = 0; x < NR; ++x) {
+    const int r = 8 * x + g4;
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
       uint4 u = make_uint4(0u, 0u, 0u, 0u);
       if (r < rows)
         u = __ldg(reinterpret_cast<const uint4*>(a.q + b * a.q_batch + (int64_t)(r / a.group) * a.q_tok +
                                                  (int64_t)(kh * a.group + r % a.group) * D + 32 * c + 8 * q4));
-      qa[x][2 * c][0] = u.x;
-      qa[x][2 * c][1] = u.y;
-      qa[x][2 * c + 1][0] = u.z;
-      qa[x][2 * c + 1][1] = u.w;
+      qb[x][2 * c][0] = u.x;
+      qb[x][2 * c][1] = u.y;
+      qb[x][2 * c + 1][0] = u.z;
+      qb[x][2 * c + 1][1] = u.w;
     }
   }
+  // o[x][4 c + p][2 e + y]: channel 64 c + 8 g4 + 2 p + e of row 8 x + 2 q4 + y
+  float o[NR][4 * VC][4], m[NR][2], l[NR][2];
+#pragma unroll
+  for (int x = 0; x < NR; ++x) {
+#pragma unroll
+    for (int n = 0; n < 4 * VC; ++n) o[x][n][0] = o[x][n][1] = o[x][n][2] = o[x][n][3] = 0.f;
+    m[x][0] = m[x][1] = -INFINITY;
+    l[x][0] = l[x][1] = 0.f;
+  }
 
-  const int step = csize * RD_WARPS * RD_KEYS;
-  const bool some = any_lo < any_hi;
-  int key0 = (some ? any_lo : 0) + (crank * RD_WARPS + warp) * RD_KEYS, fkey = key0, stage = 0;
-  // this lane's rows of the block of keys to be asked for next: K rows g4, g4 + 8; V rows 2 q4 + {0, 1}, + 8
-  const __nv_bfloat16* kp = a.k + b * a.k_batch + (int64_t)kh * D + 8 * q4 + (key0 + g4) * a.k_tok;
-  const __nv_bfloat16* vp = a.v + b * a.v_batch + (int64_t)kh * D + 8 * g4 + (key0 + 2 * q4) * a.v_tok;
-  const int64_t k8 = 8 * a.k_tok, v8 = 8 * a.v_tok, kstep = step * a.k_tok, vstep = step * a.v_tok;
-  const __nv_bfloat16 *k_any = a.k, *v_any = a.v;  // a valid address for the copies that write zeros
-  const uint32_t base = smem_u32(ring + warp * (RD_STAGES * PIECES * 32) + lane);
-  auto fetch = [&](int stg) {  // keys behind the last seen one are not read
-    const uint32_t dst = base + stg * PIECES * 512;
-    if (fkey < any_hi) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const bool in = fkey + 8 * t + g4 < any_hi;
-        const __nv_bfloat16* src = in ? kp + t * k8 : k_any;
-#pragma unroll
-        for (int c = 0; c < KC; ++c) cp_async16(dst + (t * KC + c) * 512, src + 32 * c, in);
-      }
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const bool in = fkey + (t >> 1) * 8 + 2 * q4 + (t & 1) < any_hi;
-        const __nv_bfloat16* src = in ? vp + (t >> 1) * v8 + (t & 1) * a.v_tok : v_any;
-#pragma unroll
-        for (int c = 0; c < VC; ++c) cp_async16(dst + (2 * KC + t * VC + c) * 512, src + 64 * c, in);
-      }
-    }
-    cp_async_commit();
-    fkey += step;
-    kp += kstep;
-    vp += vstep;
+  // 16 bytes of this lane: K row g4 (+ 8), channels 32 c + 8 q4; V row 2 q4 + t % 2 (+ 8), channels 64 c + 8 g4
+  const uint32_t krow = sbase + (warp * RD_KEYS + g4) * 128, vrow = sbase + VC * C::HALF + (warp * RD_KEYS + 2 * q4) * 128;
+  auto k_piece = [&](int stage, int t, int c) {
+    return ld_shared16(krow + stage * C::STAGE + (c >> 1) * C::HALF + t * 1024 + ((((c & 1) * 4 + q4) ^ g4) << 4));
   };
-
-  float o[VC * 8][2 * HR];  // n tile 8 c + i: channels 64 c + 8 (2 q4 + {0, 1}) + i of the lane's rows
+  auto v_piece = [&](int stage, int t, int c) {
+    return ld_shared16(vrow + stage * C::STAGE + c * C::HALF + (t >> 1) * 1024 + (t & 1) * 128 + ((g4 ^ (2 * q4 + (t & 1))) << 4));
+  };
+  int n = 0;
+  for (int tile = crank; tile < tiles; tile += csize, ++n) {
+    const int stage = n % C::STAGES, key0 = any_lo + tile * RD_TILE + warp * RD_KEYS;
+    if (!mbar_wait_warp(full0 + 8 * stage, (n / C::STAGES) & 1, abort_flag, err, kErrTimeoutAttnSoftmax)) break;
+    float s[NR][2][4];  // two chains of products, half as long; keys g4 + 8 (e / 2), rows 2 q4 + e % 2
 #pragma unroll
-  for (int n = 0; n < VC * 8; ++n)
+    for (int x = 0; x < NR; ++x)
 #pragma unroll
-    for (int e = 0; e < 2 * HR; ++e) o[n][e] = 0.f;
-  float m[HR], l[HR];
+      for (int e = 0; e < 4; ++e) s[x][0][e] = s[x][1][e] = 0.f;
 #pragma unroll
-  for (int x = 0; x < HR; ++x) m[x] = -INFINITY, l[x] = 0.f;
-
+    for (int c = 0; c < KC; ++c) {
+      const uint4 k0 = k_piece(stage, 0, c), k1 = k_piece(stage, 1, c);
 #pragma unroll
-  for (int i = 0; i < RD_STAGES - 1; ++i) fetch(i);
-  for (; some && key0 < any_hi; key0 += step) {
-    fetch(stage == 0 ? RD_STAGES - 1 : stage - 1);  // the stage used last
-    cp_async_wait<RD_STAGES - 1>();
-    const uint32_t src = base + stage * PIECES * 512;
-    if (++stage == RD_STAGES) stage = 0;
-    float s[2][4];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      float odd[4] = {0.f, 0.f, 0.f, 0.f};  // two chains of products, half as long
-      s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-#pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        const uint4 k = ld_shared16(src + (t * KC + c) * 512);
-        mma_16816(s[t], qa[0][2 * c][0], TWO ? qa[HR - 1][2 * c][0] : 0u, qa[0][2 * c][1], TWO ? qa[HR - 1][2 * c][1] : 0u, k.x,
-                  k.y);
-        mma_16816(odd, qa[0][2 * c + 1][0], TWO ? qa[HR - 1][2 * c + 1][0] : 0u, qa[0][2 * c + 1][1],
-                  TWO ? qa[HR - 1][2 * c + 1][1] : 0u, k.z, k.w);
+      for (int x = 0; x < NR; ++x) {
+        mma_16816(s[x][0], k0.x, k1.x, k0.y, k1.y, qb[x][2 * c][0], qb[x][2 * c][1]);
+        mma_16816(s[x][1], k0.z, k1.z, k0.w, k1.w, qb[x][2 * c + 1][0], qb[x][2 * c + 1][1]);
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[t][e] += odd[e];
     }
-
-    // the lane's scores: rows g4 (+ 8), keys key0 + 8 t + 2 q4 + e
-    float p[HR][4];
+    const bool full = key0 >= all_lo && key0 + RD_KEYS <= all_hi;  // every row sees every key of this block
+    float p[NR][4];
     bool raise = false;
-    float mx[HR];
 #pragma unroll
-    for (int x = 0; x < HR; ++x) {
-      mx[x] = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int j = key0 + 8 * t + 2 * q4 + e;
-          const float v = score_log2<CAP, BIAS>(a, s[t][2 * x + e], head[x], j - pos[x]);
-          p[x][2 * t + e] = j >= lo[x] && j < hi[x] ? v : -INFINITY;
-          mx[x] = fmaxf(mx[x], p[x][2 * t + e]);
-        }
-      mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
-      mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
-      raise |= mx[x] > m[x] + RA_RESCALE;
-    }
-    if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-      for (int x = 0; x < HR; ++x) {
-        const float mn = mx[x] > m[x] + RA_RESCALE ? mx[x] : m[x];
-        const float alpha = mn == m[x] ? 1.f : ex2_approx(m[x] - mn);
-        m[x] = mn;
-        l[x] *= alpha;
-#pragma unroll
-        for (int n = 0; n < VC * 8; ++n) {
-          o[n][2 * x] *= alpha;
-          o[n][2 * x + 1] *= alpha;
-        }
-      }
-    }
-    uint32_t pa[HR][2];
-#pragma unroll
-    for (int x = 0; x < HR; ++x) {
-      const float neg = m[x] == -INFINITY ? 0.f : -m[x];
+    for (int x = 0; x < NR; ++x)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        p[x][e] = ex2_approx(p[x][e] + neg);
-        l[x] += p[x][e];
+        const int j = key0 + g4 + 8 * (e >> 1), y = e & 1;
+        const float v = score_log2<CAP, BIAS>(a, s[x][0][e] + s[x][1][e], head[x][y], j - pos[x][y]);
+        p[x][e] = full || (j >= lo[x][y] && j < hi[x][y]) ? v : -INFINITY;
+        raise |= p[x][e] > m[x][y] + RA_RESCALE;
       }
-      pa[x][0] = pack_bf16x2(p[x][0], p[x][1]);  // weights in bf16, the MMA's operand type; the sum keeps fp32
-      pa[x][1] = pack_bf16x2(p[x][2], p[x][3]);
+    // the running maximum moves only when a score passes it by 2^8 (exact all the same)
+    if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+      for (int x = 0; x < NR; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          float mx = fmaxf(p[x][y], p[x][2 + y]);
+#pragma unroll
+          for (int w = 4; w < 32; w *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+          const float mn = mx > m[x][y] + RA_RESCALE ? mx : m[x][y];
+          const float alpha = mn == m[x][y] ? 1.f : ex2_approx(m[x][y] - mn);
+          m[x][y] = mn;
+          l[x][y] *= alpha;
+#pragma unroll
+          for (int n = 0; n < 4 * VC; ++n) o[x][n][y] *= alpha, o[x][n][2 + y] *= alpha;
+        }
+    }
+    uint32_t pb[NR][2];
+#pragma unroll
+    for (int x = 0; x < NR; ++x) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float mm = m[x][e & 1];
+        p[x][e] = ex2_approx(p[x][e] - (mm == -INFINITY ? 0.f : mm));
+        l[x][e & 1] += p[x][e];
+      }
+      // weights in bf16, the MMA's operand type; the sum keeps fp32
+      pb[x][0] = transpose_8x8(pack_bf16x2(p[x][0], p[x][1]));
+      pb[x][1] = transpose_8x8(pack_bf16x2(p[x][2], p[x][3]));
     }
     uint4 vr[4][VC];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int c = 0; c < VC; ++c) vr[t][c] = ld_shared16(src + (2 * KC + t * VC + c) * 512);
-    if (key0 < all_lo || key0 + RD_KEYS > all_hi) {  // some row does not see some key of this block
+      for (int c = 0; c < VC; ++c) vr[t][c] = v_piece(stage, t, c);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty0 + 8 * stage);  // K and V of this stage are in registers
+    if (!full) {
       uint32_t bad = 0;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
@@ -289,23 +362,23 @@ __global__ void __launch_bounds__(RD_WARPS * 32, RD_BLOCKS) range_decode_kernel(
                                   zero_nonfinite(vr[t][c].w));
 #pragma unroll 1
         for (int kk = 0; kk < RD_KEYS; ++kk) {
-          const int j = key0 + kk, src = (lane & ~3) | ((kk & 7) >> 1), e = (kk >> 3) * 2 + (kk & 1);
+          const int j = key0 + kk, from = (kk & 7) * 4 + q4;
 #pragma unroll
-          for (int x = 0; x < HR; ++x) {
-            const float p0 = __shfl_sync(0xffffffffu, p[x][0], src), p1 = __shfl_sync(0xffffffffu, p[x][1], src);
-            const float p2 = __shfl_sync(0xffffffffu, p[x][2], src), p3 = __shfl_sync(0xffffffffu, p[x][3], src);
-            const float pj = e == 0 ? p0 : e == 1 ? p1 : e == 2 ? p2 : p3;
-            if (j >= lo[x] && j < hi[x]) {
-              const __nv_bfloat16* vp = a.v + b * a.v_batch + j * a.v_tok + (int64_t)kh * D;
+          for (int x = 0; x < NR; ++x)
 #pragma unroll
-              for (int n = 0; n < VC * 8; ++n)
+            for (int y = 0; y < 2; ++y) {
+              const float pa = __shfl_sync(0xffffffffu, p[x][y], from), pc = __shfl_sync(0xffffffffu, p[x][2 + y], from);
+              if (j >= lo[x][y] && j < hi[x][y]) {
+                const __nv_bfloat16* row = a.v + b * a.v_batch + j * a.v_tok + (int64_t)kh * D + 8 * g4;
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                  const __nv_bfloat16 vv = vp[64 * (n >> 3) + 8 * (2 * q4 + y) + (n & 7)];
-                  if (nonfinite_bf16(vv)) o[n][2 * x + y] += pj * __bfloat162float(vv);
-                }
+                for (int n = 0; n < 4 * VC; ++n)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    const __nv_bfloat16 vv = row[64 * (n >> 2) + 2 * (n & 3) + e];
+                    if (nonfinite_bf16(vv)) o[x][n][2 * e + y] += (kk < 8 ? pa : pc) * __bfloat162float(vv);
+                  }
+              }
             }
-          }
         }
       }
     }
@@ -316,74 +389,56 @@ __global__ void __launch_bounds__(RD_WARPS * 32, RD_BLOCKS) range_decode_kernel(
       const uint32_t w2[4] = {vr[2][c].x, vr[2][c].y, vr[2][c].z, vr[2][c].w};
       const uint32_t w3[4] = {vr[3][c].x, vr[3][c].y, vr[3][c].z, vr[3][c].w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t sel = i & 1 ? 0x7632u : 0x5410u;
-        float acc[4] = {o[8 * c + i][0], o[8 * c + i][1], TWO ? o[8 * c + i][2 * HR - 2] : 0.f,
-                        TWO ? o[8 * c + i][2 * HR - 1] : 0.f};
-        mma_16816(acc, pa[0][0], TWO ? pa[HR - 1][0] : 0u, pa[0][1], TWO ? pa[HR - 1][1] : 0u,
-                  __byte_perm(w0[i >> 1], w1[i >> 1], sel), __byte_perm(w2[i >> 1], w3[i >> 1], sel));
-        o[8 * c + i][0] = acc[0];
-        o[8 * c + i][1] = acc[1];
-        if constexpr (TWO) {
-          o[8 * c + i][2] = acc[2];
-          o[8 * c + i][3] = acc[3];
-        }
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a0 = __byte_perm(w0[i], w1[i], 0x5410u), a1 = __byte_perm(w0[i], w1[i], 0x7632u);
+        const uint32_t a2 = __byte_perm(w2[i], w3[i], 0x5410u), a3 = __byte_perm(w2[i], w3[i], 0x7632u);
+#pragma unroll
+        for (int x = 0; x < NR; ++x) mma_16816(o[x][4 * c + i], a0, a1, a2, a3, pb[x][0], pb[x][1]);
       }
     }
   }
-  cp_async_wait<0>();
   __syncthreads();  // the ring becomes the merge buffer
-
-  // merge: warps of the block, then blocks of the cluster (row r of the result by rank r % csize)
 #pragma unroll
-  for (int x = 0; x < HR; ++x) {
-    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-    const int r = g4 + 8 * x;
-    if (q4 == 0) ml_sh[warp][r] = make_float2(m[x], l[x]);
+  for (int x = 0; x < NR; ++x)
 #pragma unroll
-    for (int n = 0; n < VC * 8; ++n)
+    for (int y = 0; y < 2; ++y) {
+      const int r = 8 * x + 2 * q4 + y;
 #pragma unroll
-      for (int y = 0; y < 2; ++y) o_sh[warp][r][64 * (n >> 3) + 8 * (2 * q4 + y) + (n & 7)] = o[n][2 * x + y];
-  }
+      for (int w = 4; w < 32; w *= 2) l[x][y] += __shfl_xor_sync(0xffffffffu, l[x][y], w);
+      if (g4 == 0) ml_sh[warp][r] = make_float2(m[x][y], l[x][y]);
+#pragma unroll
+      for (int n = 0; n < 4 * VC; ++n)
+        *reinterpret_cast<float2*>(&o_sh[warp][r][64 * (n >> 2) + 8 * g4 + 2 * (n & 3)]) = make_float2(o[x][n][y], o[x][n][2 + y]);
+    }
   __syncthreads();
-  for (int i = threadIdx.x; i < rows * D; i += RD_WARPS * 32) {
-    const int r = i / D, d = i % D;
+  for (int i = threadIdx.x; i < rows * (D / 4); i += RD_WARPS * 32) {  // four channels a thread
+    const int r = i / (D / 4), d = i % (D / 4) * 4, tok = r / a.group;
     float mm = -INFINITY;
 #pragma unroll
     for (int w = 0; w < RD_WARPS; ++w) mm = fmaxf(mm, ml_sh[w][r].x);
-    float ll = 0.f, oo = 0.f;
+    float ll = 0.f;
+    float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < RD_WARPS; ++w) {
       const float2 ml = ml_sh[w][r];
+      const float4 x = *reinterpret_cast<const float4*>(&o_sh[w][r][d]);
       // a warp that saw nothing, or only scores of minus infinity: its sums are 0, or NaN to be kept
       const float f = ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - mm);
       ll = fmaf(f, ml.y, ll);
-      oo = fmaf(f, o_sh[w][r][d], oo);
+      oo.x = fmaf(f, x.x, oo.x), oo.y = fmaf(f, x.y, oo.y), oo.z = fmaf(f, x.z, oo.z), oo.w = fmaf(f, x.w, oo.w);
     }
-    o_cta[r][d] = oo;
-    if (d == 0) ml_cta[r] = make_float2(mm, ll);
-  }
-  cluster.sync();
-  for (int r = crank; r < rows; r += csize) {
-    const int tok = r / a.group;
-    int rlo, rhi;
-    row_range(a, b, tok, rlo, rhi);
-    float mm = -INFINITY;
-    for (int c = 0; c < csize; ++c) mm = fmaxf(mm, cluster.map_shared_rank(ml_cta, c)[r].x);
-    for (int d = threadIdx.x; d < D; d += RD_WARPS * 32) {
-      float ll = 0.f, oo = 0.f;
-      for (int c = 0; c < csize; ++c) {
-        const float2 ml = cluster.map_shared_rank(ml_cta, c)[r];
-        const float f = ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - mm);
-        ll = fmaf(f, ml.y, ll);
-        oo = fmaf(f, cluster.map_shared_rank(&o_cta[0][0], c)[r * D + d], oo);
-      }
-      a.o[b * a.o_batch + (int64_t)tok * a.o_tok + (int64_t)(kh * a.group + r % a.group) * D + d] =
-          __float2bfloat16(rlo < rhi ? oo / ll : 0.f);
+    if (csize > 1) {
+      const int64_t prow = (int64_t)blockIdx.x * rows + r;
+      *reinterpret_cast<float4*>(out.o + prow * D + d) = oo;
+      if (d == 0) out.ml[prow] = make_float2(mm, ll);
+    } else {
+      int rlo, rhi;
+      row_range(a, b, tok, rlo, rhi);
+      const float inv = 1.f / ll;
+      *reinterpret_cast<uint2*>(a.o + b * a.o_batch + (int64_t)tok * a.o_tok + (int64_t)(kh * a.group + r % a.group) * D + d) =
+          rlo < rhi ? make_uint2(pack_bf16x2(oo.x * inv, oo.y * inv), pack_bf16x2(oo.z * inv, oo.w * inv)) : make_uint2(0u, 0u);
     }
   }
-  cluster.sync();  // a block's shared memory stays until all have read it
 }
 
 // ================================================================== many rows: tcgen05 tiles
@@ -405,7 +460,8 @@ constexpr int RT_THREADS = 384;
 constexpr int RT_BLK = 16384;  // 128 rows of one 128-byte swizzle row
 constexpr int RT_P_SPLIT = 96;
 constexpr int RT_QUEUE = 2;
-constexpr int RT_SORT_MAX = 2048;  // pairs that the plan kernel sorts
+constexpr int RT_SORT_MAX = 1024;  // pairs that the plan kernel sorts
+constexpr int RT_REACH_MAX = 8192;  // of a bias table (it is copied with padded ends at every call)
 
 template <int D>
 struct RangeTileCfg {
@@ -430,11 +486,14 @@ struct RangeTileArgs {
   const RangePair* pairs;
   const int* order;
   int* counter;
-  float* o_part;   // [splits][batch * kv_heads * q_len * group][D]
-  float2* ml_part;
-  int64_t part_rows;
+  RangeParts parts;
+  const float* padded;  // the bias table in log2 units, its ends repeated RT_N times
+  float cap_scale;      // softmax_scale / softcap
   int* err;
 };
+
+// Entry RT_N + reach + d of a padded row is table[clamp(d, -reach, reach)] log2(e), -reach - RT_N <= d < reach + RT_N.
+__host__ __device__ constexpr int range_padded(int reach) { return 2 * (reach + RT_N); }
 
 struct PlanArgs {
   RangeArgs a;
@@ -442,65 +501,75 @@ struct PlanArgs {
   RangePair* pairs;
   int* order;
   int* counter;
+  float* padded;
 };
 
-// The key ranges of every tile pair (one warp each), and the pairs from the most key tiles to the
-// fewest (bitonic sort, up to RT_SORT_MAX pairs; more are taken from the last to the first).
+// Block 0: the key ranges of every tile pair (one warp each) and the pairs from the most key tiles to
+// the fewest (each counts those in front of it, up to RT_SORT_MAX pairs; more are spread over the
+// blocks and taken from the last to the first).  The other blocks: the padded bias table.
 __global__ void __launch_bounds__(1024) range_plan_kernel(const PlanArgs p) {
-  __shared__ uint32_t key[RT_SORT_MAX];
+  __shared__ __align__(16) int tiles_of[RT_SORT_MAX];
+  pdl_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int n2 = 1;
-  while (n2 < p.entries) n2 *= 2;
-  const bool sort = n2 <= RT_SORT_MAX;
+  const bool sort = p.entries <= RT_SORT_MAX;
+  if (p.padded) {
+    const int row = range_padded(p.a.reach), n = p.a.kv_heads * p.a.group * row;
+    for (int i = blockIdx.x * 1024 + threadIdx.x; i < n; i += gridDim.x * 1024) {
+      const int h = i / row, d = min(max(i - h * row - RT_N - p.a.reach, -p.a.reach), p.a.reach);
+      p.padded[i] = RA_LOG2E * __ldg(p.a.table + (int64_t)h * (2 * p.a.reach + 1) + d + p.a.reach);
+    }
+  }
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.counter = 0;
-  if (sort)
-    for (int i = threadIdx.x; i < n2; i += 1024) key[i] = 0u;
-  __syncthreads();
+  if (sort && blockIdx.x != 0) return;
   const int warps = sort ? 32 : gridDim.x * 32;
   for (int e = (sort ? 0 : blockIdx.x * 32) + warp; e < p.entries; e += warps) {
     const int b = e / p.nqp, tok0 = e % p.nqp * 2 * p.tpt;
+    int any_lo[2], any_hi[2], all_lo[2], all_hi[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) any_lo[t] = INT32_MAX, any_hi[t] = 0, all_lo[t] = 0, all_hi[t] = INT32_MAX;
+#pragma unroll 4
+    for (int i = lane; i < 2 * p.tpt; i += 32) {
+      if (tok0 + i >= p.a.q_len) break;
+      const int t = i >= p.tpt;
+      int lo, hi;
+      row_range(p.a, b, tok0 + i, lo, hi);
+      const bool some = lo < hi;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        if (x == t) {
+          any_lo[x] = some ? min(any_lo[x], lo) : any_lo[x];
+          any_hi[x] = some ? max(any_hi[x], hi) : any_hi[x];
+          all_lo[x] = max(all_lo[x], lo);
+          all_hi[x] = min(all_hi[x], hi);
+        }
+    }
     RangePair r;
     int tiles = 0;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      int any_lo = INT32_MAX, any_hi = 0, all_lo = 0, all_hi = INT32_MAX;
-      for (int i = tok0 + t * p.tpt + lane; i < min(tok0 + (t + 1) * p.tpt, p.a.q_len); i += 32) {
-        int lo, hi;
-        row_range(p.a, b, i, lo, hi);
-        if (lo < hi) any_lo = min(any_lo, lo), any_hi = max(any_hi, hi);
-        all_lo = max(all_lo, lo);
-        all_hi = min(all_hi, hi);
-      }
-      r.any_lo[t] = __reduce_min_sync(0xffffffffu, any_lo);
-      r.any_hi[t] = __reduce_max_sync(0xffffffffu, any_hi);
-      r.all_lo[t] = __reduce_max_sync(0xffffffffu, all_lo);
-      r.all_hi[t] = __reduce_min_sync(0xffffffffu, all_hi);
+      r.any_lo[t] = __reduce_min_sync(0xffffffffu, any_lo[t]);
+      r.any_hi[t] = __reduce_max_sync(0xffffffffu, any_hi[t]);
+      r.all_lo[t] = __reduce_max_sync(0xffffffffu, all_lo[t]);
+      r.all_hi[t] = __reduce_min_sync(0xffffffffu, all_hi[t]);
       if (r.any_lo[t] >= r.any_hi[t]) r.any_lo[t] = r.any_hi[t] = 0;
       tiles += (r.any_hi[t] + RT_N - 1) / RT_N - r.any_lo[t] / RT_N;
     }
     if (lane == 0) {
       p.pairs[e] = r;
       if (sort)
-        key[e] = (uint32_t)min(tiles, (1 << 20) - 1) << 11 | (uint32_t)e;
+        tiles_of[e] = tiles;
       else
         p.order[e] = p.entries - 1 - e;
     }
   }
   if (!sort) return;
   __syncthreads();
-  for (int k = 2; k <= n2; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int i = threadIdx.x; i < n2; i += 1024) {
-        const int x = i ^ j;
-        if (x > i) {
-          const uint32_t u = key[i], v = key[x];
-          if (((i & k) == 0) ? u < v : u > v) key[i] = v, key[x] = u;  // descending
-        }
-      }
-      __syncthreads();
-    }
-  // the padding keys are 0, and so is that of entry 0 without any keys: it may end up among them
-  for (int i = threadIdx.x; i < p.entries; i += 1024) p.order[i] = (int)(key[i] & (RT_SORT_MAX - 1));
+  for (int e = threadIdx.x; e < p.entries; e += 1024) {  // entries <= 1024: one each
+    const int mine = tiles_of[e];
+    int place = 0;
+    for (int i = 0; i < p.entries; ++i) place += tiles_of[i] > mine || (tiles_of[i] == mine && i < e);
+    p.order[place] = e;
+  }
 }
 
 struct RangeUnit {
@@ -644,6 +713,7 @@ __global__ void __maxnreg__(160)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();  // the plan; its launch ran beside the set-up above
 
   // The next unit for a consuming warp (or its one lane): -1 = no more, -2 = aborted.
   int un = 0;
@@ -887,6 +957,9 @@ __global__ void __maxnreg__(160)
       const RangeUnit w = range_unit(g, u);
       __syncwarp();
       if (lane == 0) release_unit();
+      // this tile's bounds as scalars (indexing the unit by t would put it into local memory)
+      const int a_t = t ? w.a[1] : w.a[0], z_t = t ? w.z[1] : w.z[0];
+      const int flo_t = t ? w.full_lo[1] : w.full_lo[0], fhi_t = t ? w.full_hi[1] : w.full_hi[0];
       const int tok = w.tok0 + t * g.tpt + rtok;
       const bool live = rtok < g.tpt && tok < a.q_len;
       const int head = w.kh * a.group + rhead;
@@ -898,7 +971,7 @@ __global__ void __maxnreg__(160)
       float slope2 = 0.f;
       const float* trow = nullptr;
       if constexpr (BIAS == kBiasSlopes) slope2 = live ? RA_LOG2E * __ldg(a.slopes + head) : 0.f;
-      if constexpr (BIAS == kBiasTable) trow = a.table + (live ? (int64_t)head * (2 * a.reach + 1) : 0) + a.reach;
+      if constexpr (BIAS == kBiasTable) trow = g.padded + (live ? (int64_t)head * range_padded(a.reach) : 0) + a.reach + RT_N;
       float m_used = -INFINITY, l_run = 0.f;
       bool any_tile = false;
       for (int j = w.k0; j < w.k1; ++j) {
@@ -906,7 +979,7 @@ __global__ void __maxnreg__(160)
         const int slot = (gk + 1) % RING;
         const bool partial = unit_partial(w, j);
         gk += 2;
-        if (!unit_has(w, t, j)) {
+        if (j < a_t || j >= z_t) {
           if (partial) ok_ph ^= 1u << slot;
           continue;
         }
@@ -922,7 +995,7 @@ __global__ void __maxnreg__(160)
         tmem_wait_ld();
         float* s = reinterpret_cast<float*>(sr);
         const int kbase = j * RT_N;
-        const bool masked = !unit_full(w, t, j);
+        const bool masked = kbase < flo_t || kbase + RT_N > fhi_t;
         uint32_t mask[4];
         if (masked) {
 #pragma unroll
@@ -937,20 +1010,53 @@ __global__ void __maxnreg__(160)
               if (!((mask[k >> 5] >> (k & 31)) & 1u)) s[k] = 0.f;
           }
         }
+        float mx = -INFINITY;
         if constexpr (CAP) {
-          // cap2 tanh = cap2 - 2 cap2 / (1 + 2^x); four reciprocals from one (MUFU is what bounds this form)
-          const float n2c = -2.f * a.cap2;
+          float hi8[4], lo8[4];
 #pragma unroll
-          for (int k = 0; k < RT_N; k += 4) {
-            const float d0 = 1.f + ex2_approx(min30(s[k] * a.sl2)), d1 = 1.f + ex2_approx(min30(s[k + 1] * a.sl2));
-            const float d2 = 1.f + ex2_approx(min30(s[k + 2] * a.sl2)), d3 = 1.f + ex2_approx(min30(s[k + 3] * a.sl2));
-            const float p01 = d0 * d1, p23 = d2 * d3;
-            const float rc = n2c * rcp_approx(p01 * p23);
-            const float r01 = rc * p23, r23 = rc * p01;
-            s[k] = fmaf(r01, d1, a.cap2);
-            s[k + 1] = fmaf(r01, d0, a.cap2);
-            s[k + 2] = fmaf(r23, d3, a.cap2);
-            s[k + 3] = fmaf(r23, d2, a.cap2);
+          for (int c = 0; c < 4; ++c) hi8[c] = fmaxf(s[2 * c], s[2 * c + 1]), lo8[c] = fminf(s[2 * c], s[2 * c + 1]);
+#pragma unroll
+          for (int q = 1; q < RT_N / 8; ++q)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              hi8[c] = fmax3(hi8[c], s[8 * q + 2 * c], s[8 * q + 2 * c + 1]);
+              lo8[c] = fmin3(lo8[c], s[8 * q + 2 * c], s[8 * q + 2 * c + 1]);
+            }
+          const float top_hi = fmax3(hi8[0], hi8[1], fmaxf(hi8[2], hi8[3]));
+          const float top = fmaxf(top_hi, -fmin3(lo8[0], lo8[1], fminf(lo8[2], lo8[3])));
+          if (__all_sync(0xffffffffu, top * g.cap_scale <= 0.6f)) {
+            // |x| = |score| / cap <= 0.6: tanh x = x P(x^2), P fitted to 5.9e-7 (least maximum error of an
+            // odd polynomial of degree 7 on [0, 0.6]): 3e-5 of a score capped at 50, far below the bf16
+            // rounding of its weight, and no MUFU, which bounds the general form
+            const float2 kx = make_float2(g.cap_scale, g.cap_scale);
+            const float c0 = 0.999991018f * a.cap2, c1 = -0.332989737f * a.cap2, c2 = 0.129745518f * a.cap2, c3 = -0.0396112428f * a.cap2;
+            const float2 p0 = make_float2(c0, c0), p1 = make_float2(c1, c1), p2 = make_float2(c2, c2), p3 = make_float2(c3, c3);
+#pragma unroll
+            for (int k = 0; k < RT_N; k += 2) {
+              const float2 x = __fmul2_rn(make_float2(s[k], s[k + 1]), kx);
+              const float2 x2 = __fmul2_rn(x, x);
+              const float2 y = __fmul2_rn(x, __ffma2_rn(x2, __ffma2_rn(x2, __ffma2_rn(x2, p3, p2), p1), p0));
+              s[k] = y.x;
+              s[k + 1] = y.y;
+            }
+            const float x = top_hi * g.cap_scale, x2 = x * x;
+            mx = x * fmaf(x2, fmaf(x2, fmaf(x2, c3, c2), c1), c0);
+          } else {
+            // cap2 tanh = cap2 - 2 cap2 / (1 + 2^x); four reciprocals from one (MUFU bounds this form)
+            const float n2c = -2.f * a.cap2;
+#pragma unroll
+            for (int k = 0; k < RT_N; k += 4) {
+              const float d0 = 1.f + ex2_approx(min30(s[k] * a.sl2)), d1 = 1.f + ex2_approx(min30(s[k + 1] * a.sl2));
+              const float d2 = 1.f + ex2_approx(min30(s[k + 2] * a.sl2)), d3 = 1.f + ex2_approx(min30(s[k + 3] * a.sl2));
+              const float p01 = d0 * d1, p23 = d2 * d3;
+              const float rc = n2c * rcp_approx(p01 * p23);
+              const float r01 = rc * p23, r23 = rc * p01;
+              s[k] = fmaf(r01, d1, a.cap2);
+              s[k + 1] = fmaf(r01, d0, a.cap2);
+              s[k + 2] = fmaf(r23, d3, a.cap2);
+              s[k + 3] = fmaf(r23, d2, a.cap2);
+            }
+            mx = fmaf(n2c, rcp_approx(1.f + ex2_approx(min30(top_hi * a.sl2))), a.cap2);
           }
         }
         const float sl2 = CAP ? 1.f : a.sl2;
@@ -959,17 +1065,10 @@ __global__ void __maxnreg__(160)
 #pragma unroll
           for (int k = 0; k < RT_N; ++k) s[k] = fmaf(-slope2, fabsf(d0 + (float)k), CAP ? s[k] : s[k] * sl2);
         }
-        if constexpr (BIAS == kBiasTable) {
-          const int d0 = kbase - pos;
-          if (__all_sync(0xffffffffu, d0 >= a.reach || d0 + RT_N - 1 <= -a.reach)) {
-            const float far = RA_LOG2E * __ldg(trow + (d0 >= a.reach ? a.reach : -a.reach));
+        if constexpr (BIAS == kBiasTable) {  // the padded table: one clamp a row, fixed offsets for its keys
+          const float* tp = trow + min(max(kbase - pos, -a.reach - RT_N), a.reach);
 #pragma unroll
-            for (int k = 0; k < RT_N; ++k) s[k] = CAP ? s[k] + far : fmaf(s[k], sl2, far);
-          } else {
-#pragma unroll
-            for (int k = 0; k < RT_N; ++k)
-              s[k] = fmaf(RA_LOG2E, __ldg(trow + min(max(d0 + k, -a.reach), a.reach)), CAP ? s[k] : s[k] * sl2);
-          }
+          for (int k = 0; k < RT_N; ++k) s[k] = CAP ? s[k] + __ldg(tp + k) : fmaf(s[k], sl2, __ldg(tp + k));
         }
         const float mul = BIAS == kBiasNone && !CAP ? a.sl2 : 1.f;  // what is left to apply in the exponent
         if (masked) {
@@ -977,14 +1076,18 @@ __global__ void __maxnreg__(160)
           for (int k = 0; k < RT_N; ++k)
             if (!((mask[k >> 5] >> (k & 31)) & 1u)) s[k] = -INFINITY;
         }
-        float m8[8];
+        // the capped maximum of a fully seen tile follows from that of the raw scores (tanh grows with
+        // its argument); m only has to be near the true maximum, so the two need not agree to the bit
+        if (!CAP || BIAS != kBiasNone || masked) {
+          float m8[8];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) m8[c] = fmaxf(s[2 * c], s[2 * c + 1]);
+          for (int c = 0; c < 8; ++c) m8[c] = fmaxf(s[2 * c], s[2 * c + 1]);
 #pragma unroll
-        for (int q = 1; q < RT_N / 16; ++q)
+          for (int q = 1; q < RT_N / 16; ++q)
 #pragma unroll
-          for (int c = 0; c < 8; ++c) m8[c] = fmax3(m8[c], s[16 * q + 2 * c], s[16 * q + 2 * c + 1]);
-        const float mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
+            for (int c = 0; c < 8; ++c) m8[c] = fmax3(m8[c], s[16 * q + 2 * c], s[16 * q + 2 * c + 1]);
+          mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
+        }
         const float m_cand = mx * mul;
         const bool need = m_cand > m_used + RA_RESCALE;
         const bool any_need = __any_sync(0xffffffffu, need);
@@ -1055,9 +1158,9 @@ __global__ void __maxnreg__(160)
         tc_fence_after();
       }
       if (g.splits > 1) {
-        const int64_t prow = (int64_t)w.split * g.part_rows +
-                             (((int64_t)w.b * a.kv_heads + w.kh) * a.q_len + tok) * a.group + rhead;
-        float4* dst = reinterpret_cast<float4*>(g.o_part + prow * D);
+        const int64_t prow = ((int64_t)w.split * g.parts.groups + (int64_t)w.b * a.kv_heads + w.kh) * g.parts.slot_rows +
+                             (int64_t)tok * a.group + rhead;
+        float4* dst = reinterpret_cast<float4*>(g.parts.o + prow * D);
         if (any_tile) {  // otherwise the sum and maximum say that this split saw nothing
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
@@ -1069,7 +1172,7 @@ __global__ void __maxnreg__(160)
             }
           }
         }
-        if (live) g.ml_part[prow] = make_float2(any_tile ? m_used : -INFINITY, any_tile ? l_run : -1.f);
+        if (live) g.parts.ml[prow] = make_float2(any_tile ? m_used : -INFINITY, any_tile ? l_run : -1.f);
       } else {
         const float inv_l = lo < hi ? 1.f / l_run : 0.f;
         uint4* dst = reinterpret_cast<uint4*>(a.o + (int64_t)w.b * a.o_batch + (int64_t)tok * a.o_tok + (int64_t)head * D);
@@ -1100,37 +1203,49 @@ __global__ void __maxnreg__(160)
   if (warp == 9) tmem_dealloc(tmem_base, 512);
 }
 
-// Merge of the key splits: one warp per packed row.  A split that saw no key tile left l = -1 and no O.
+// Merge of the key splits: one block per packed row, its warps taking the splits in turn.
+constexpr int RC_WARPS = 4;
+
 template <int D>
-__global__ void __launch_bounds__(256) range_combine_kernel(const RangeTileArgs g) {
+__global__ void __launch_bounds__(RC_WARPS * 32) range_combine_kernel(const RangeArgs a, const RangeParts in) {
   constexpr int E = D / 32;
-  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (w >= g.part_rows) return;
-  const RangeArgs& a = g.a;
-  const int hg = (int)(w % a.group);
-  int64_t x = w / a.group;
-  const int tok = (int)(x % a.q_len);
-  x /= a.q_len;
-  const int kh = (int)(x % a.kv_heads), b = (int)(x / a.kv_heads);
+  __shared__ float l_sh[RC_WARPS], o_sh[RC_WARPS][D];
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int x = (int)(blockIdx.x / in.slot_rows), r = (int)(blockIdx.x - (int64_t)x * in.slot_rows);
+  const int hg = r % a.group, tok = r / a.group, kh = x % a.kv_heads, b = x / a.kv_heads;
+  const int4 f4 = in.first ? in.first[x] : make_int4(x, in.splits, in.groups, 0);
+  if (in.first && f4.y == 1) return;  // its one block wrote the output
   int lo, hi;
   row_range(a, b, tok, lo, hi);
+  const int64_t row0 = (int64_t)f4.x * in.slot_rows + r, next = (int64_t)f4.z * in.slot_rows;
   float m = -INFINITY;
-  for (int s = 0; s < g.splits; ++s) m = fmaxf(m, g.ml_part[s * g.part_rows + w].x);
+  for (int s = lane; s < f4.y; s += 32) m = fmaxf(m, in.ml[row0 + s * next].x);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   float l = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int s = 0; s < g.splits; ++s) {
-    const float2 ml = g.ml_part[s * g.part_rows + w];
+#pragma unroll 4
+  for (int s = warp; s < f4.y; s += RC_WARPS) {
+    const float2 ml = in.ml[row0 + s * next];
     if (ml.y == -1.f) continue;
     const float f = ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - m);
     l = fmaf(f, ml.y, l);
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(f, g.o_part[(s * g.part_rows + w) * D + lane * E + e], o[e]);
+    for (int e = 0; e < E; ++e) o[e] = fmaf(f, in.o[(row0 + s * next) * D + lane * E + e], o[e]);
   }
-  __nv_bfloat16* op = a.o + b * a.o_batch + (int64_t)tok * a.o_tok + (int64_t)(kh * a.group + hg) * D + lane * E;
+  if (lane == 0) l_sh[warp] = l;
 #pragma unroll
-  for (int e = 0; e < E; ++e) op[e] = __float2bfloat16(lo < hi ? o[e] / l : 0.f);
+  for (int e = 0; e < E; ++e) o_sh[warp][lane * E + e] = o[e];
+  __syncthreads();
+  if (threadIdx.x < D) {
+    float ll = 0.f, oo = 0.f;
+#pragma unroll
+    for (int w = 0; w < RC_WARPS; ++w) ll += l_sh[w], oo += o_sh[w][threadIdx.x];
+    a.o[b * a.o_batch + (int64_t)tok * a.o_tok + (int64_t)(kh * a.group + hg) * D + threadIdx.x] =
+        __float2bfloat16(lo < hi ? oo / ll : 0.f);
+  }
 }
 
 // ------------------------------------------------------------------ host launcher
@@ -1139,13 +1254,41 @@ constexpr int RD_ROWS = 16;
 
 struct RangeLayout {
   int tpt, nqp, entries, streams, splits;
-  int64_t units, part_rows, order_off, counter_off, part_off, ml_off, bytes;
+  int64_t units, part_rows, order_off, counter_off, pad_off, part_off, ml_off, bytes;
 };
+
+static int64_t range_up(int64_t x) { return (x + 255) / 256 * 256; }
+
+// The few-rows kernel's blocks: as many as the SMs hold at once, less half a block for each (key head,
+// batch element), whose last share is half full on average.  More elements than blocks: one block each.
+static int range_decode_slots(const wanb200_range_attn_params* p) {
+  const int64_t units = p->batch * p->kv_heads, slots = (int64_t)num_sms() * RD_BLOCKS;
+  return units >= slots || p->kv_len <= RD_TILE * RD_SHARE ? 0 : (int)std::max(slots - units / 2, slots / 4);
+}
+
+static int64_t range_decode_blocks(const wanb200_range_attn_params* p) {  // an upper bound: the lengths are on the device
+  const int64_t units = p->batch * p->kv_heads, slots = range_decode_slots(p);
+  const int64_t most = (p->kv_len + RD_TILE * RD_SHARE - 1) / (RD_TILE * RD_SHARE);
+  return slots ? std::min(slots + units, units * most) : units;
+}
 
 static RangeLayout range_layout(const wanb200_range_attn_params* p) {
   RangeLayout l = {};
   const int group = (int)(p->heads / p->kv_heads);
-  if (p->q_len * group <= RD_ROWS) return l;
+  l.part_rows = p->batch * p->heads * p->q_len;
+  auto parts = [&](int64_t at, int64_t rows) {  // rows of all slots
+    l.part_off = at;
+    l.ml_off = at + range_up(rows * p->head_dim * 4);
+    l.bytes = l.ml_off + range_up(rows * 8);
+  };
+  if (p->q_len * group <= RD_ROWS) {
+    l.splits = 1;
+    if (range_decode_slots(p)) {
+      l.splits = 2;  // some element may have several blocks
+      parts(range_up(p->batch * p->kv_heads * 16), range_decode_blocks(p) * p->q_len * group);
+    }
+    return l;
+  }
   const bool per_batch = p->range_batch_stride > 0;
   l.tpt = RT_M / group;
   l.nqp = (int)((p->q_len + 2 * l.tpt - 1) / (2 * l.tpt));
@@ -1157,13 +1300,11 @@ static RangeLayout range_layout(const wanb200_range_attn_params* p) {
   const int64_t units = entries * streams, tiles = (p->kv_len + RT_N - 1) / RT_N;
   l.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(num_sms() / units, tiles / 2), 32));
   l.units = units * l.splits;
-  l.part_rows = p->batch * p->heads * p->q_len;
-  auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
-  l.order_off = up(entries * (int64_t)sizeof(RangePair));
-  l.counter_off = l.order_off + up(entries * 4);
-  l.part_off = l.counter_off + 256;
-  l.ml_off = l.part_off + (l.splits > 1 ? up(l.splits * l.part_rows * p->head_dim * 4) : 0);
-  l.bytes = l.ml_off + (l.splits > 1 ? up(l.splits * l.part_rows * 8) : 0);
+  l.order_off = range_up(entries * (int64_t)sizeof(RangePair));
+  l.counter_off = l.order_off + range_up(entries * 4);
+  l.pad_off = l.counter_off + 256;
+  parts(l.pad_off + (p->dist_bias ? range_up(p->heads * (int64_t)range_padded(p->reach) * 4) : 0),
+        l.splits > 1 ? l.splits * l.part_rows : 0);
   return l;
 }
 
@@ -1193,8 +1334,8 @@ static int range_validate(const wanb200_range_attn_params* p) {
   if (!(p->softcap >= 0.f) || !(p->softcap < INFINITY))
     return set_error(WANB200_EINVAL, "range_attn: softcap must be >= 0 (0 = none)");
   if (p->slopes && p->dist_bias) return set_error(WANB200_EINVAL, "range_attn: slopes or dist_bias, not both");
-  if (p->dist_bias && (p->reach < 0 || p->reach > (1 << 24)))
-    return set_error(WANB200_EINVAL, "range_attn: dist_bias needs 0 <= reach <= 2^24");
+  if (p->dist_bias && (p->reach < 0 || p->reach > RT_REACH_MAX))
+    return set_error(WANB200_EINVAL, "range_attn: dist_bias needs 0 <= reach <= 8192");
   if (p->range_batch_stride < 0) return set_error(WANB200_EINVAL, "range_attn: negative range_batch_stride");
   return WANB200_OK;
 }
@@ -1202,53 +1343,57 @@ static int range_validate(const wanb200_range_attn_params* p) {
 int64_t range_attn_workspace_bytes(const wanb200_range_attn_params* p) {
   if (!p || p->batch <= 0 || p->heads <= 0 || p->kv_heads <= 0 || p->heads % p->kv_heads || p->heads / p->kv_heads > RT_M ||
       p->q_len <= 0 || p->kv_len <= 0 || p->q_len > INT32_MAX / 2 || p->batch > 65535 || p->heads > 65535 ||
-      (p->head_dim != 64 && p->head_dim != 128))
+      (p->head_dim != 64 && p->head_dim != 128) || p->reach < 0 || p->reach > RT_REACH_MAX)
     return 0;
   return range_layout(p).bytes;
 }
 
+template <int D>
+static int launch_range_combine(const RangeArgs& a, const RangeParts& parts, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(parts.groups * parts.slot_rows));
+  cfg.blockDim = dim3(RC_WARPS * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, range_combine_kernel<D>, a, parts);
+  if (e != cudaSuccess) return set_cuda_error("range_combine_kernel launch", e);
+  return WANB200_OK;
+}
+
+struct DecodeLaunch {
+  RangeParts parts;
+  CUtensorMap k, v;
+  int rows, blocks, slots;
+  int* err;
+};
+
 template <int D, bool TWO, bool CAP, int BIAS>
-static cudaError_t launch_range_decode(const RangeArgs& a, const cudaLaunchConfig_t& cfg, int dev) {
+static cudaError_t launch_range_decode(const RangeArgs& a, const DecodeLaunch& d, int dev, cudaStream_t st) {
   static std::atomic<bool> attr_set[kMaxDevices] = {};
   if (!attr_set[dev].load(std::memory_order_acquire)) {
     const cudaError_t e = cudaFuncSetAttribute(range_decode_kernel<D, TWO, CAP, BIAS>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, RangeDecodeCfg<D>::RING);
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, RangeDecodeCfg<D>::SMEM);
     if (e != cudaSuccess) return e;
     attr_set[dev].store(true, std::memory_order_release);
   }
-  return cudaLaunchKernelEx(&cfg, range_decode_kernel<D, TWO, CAP, BIAS>, a);
+  range_decode_kernel<D, TWO, CAP, BIAS><<<(unsigned)d.blocks, RD_THREADS, RangeDecodeCfg<D>::SMEM, st>>>(d.k, d.v, a, d.parts,
+                                                                                                          d.slots, d.err);
+  return cudaGetLastError();
 }
 
 template <int D, bool CAP, int BIAS>
-static int launch_range_decode(const RangeArgs& a, int rows, cudaStream_t st) {
-  // Blocks of a cluster share one (key head, batch element).  The cluster size is the one with the
-  // smallest waves x (keys of a block + 160): the block's fixed costs (start, merges) weigh about as much
-  // as 160 keys.
+static int launch_range_decode(const RangeArgs& a, const DecodeLaunch& d, cudaStream_t st) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= kMaxDevices) return set_error(WANB200_EINVAL, "device index out of range");
-  const int64_t units = (int64_t)a.batch * a.kv_heads, slots = (int64_t)num_sms() * RD_BLOCKS;
-  int best = 1;
-  double best_t = 1e300;
-  for (int c = 1; c <= 8; c *= 2) {
-    const double t = (double)((units * c + slots - 1) / slots) * ((double)a.kv_len / c + 160.0);
-    if (t < best_t - 1e-9) best_t = t, best = c;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)best, (unsigned)a.kv_heads, (unsigned)a.batch);
-  cfg.blockDim = dim3(RD_WARPS * 32);
-  cfg.dynamicSmemBytes = RangeDecodeCfg<D>::RING;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)best;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = rows > 8 ? launch_range_decode<D, true, CAP, BIAS>(a, cfg, dev)
-                                 : launch_range_decode<D, false, CAP, BIAS>(a, cfg, dev);
+  const cudaError_t e = d.rows > 8 ? launch_range_decode<D, true, CAP, BIAS>(a, d, dev, st)
+                                   : launch_range_decode<D, false, CAP, BIAS>(a, d, dev, st);
   if (e != cudaSuccess) return set_cuda_error("range_decode_kernel launch", e);
-  return WANB200_OK;
+  return d.parts.splits > 1 ? launch_range_combine<D>(a, d.parts, st) : WANB200_OK;
 }
 
 template <int D, bool CAP, int BIAS>
@@ -1272,21 +1417,33 @@ static int launch_range_tiles(const CUtensorMap& tq, const CUtensorMap& tk, cons
   pl.pairs = const_cast<RangePair*>(g.pairs);
   pl.order = const_cast<int*>(g.order);
   pl.counter = g.counter;
-  const int plan_blocks = g.entries <= RT_SORT_MAX ? 1 : std::min((g.entries + 31) / 32, num_sms());
+  pl.padded = const_cast<float*>(g.padded);
+  int plan_blocks = g.entries <= RT_SORT_MAX ? 1 : std::min((g.entries + 31) / 32, num_sms());
+  if (BIAS == kBiasTable)
+    plan_blocks = std::max(plan_blocks, std::min(1 + g.a.kv_heads * g.a.group * range_padded(g.a.reach) / 4096, num_sms()));
   range_plan_kernel<<<plan_blocks, 1024, 0, st>>>(pl);
-  const unsigned grid = (unsigned)std::min<int64_t>(g.units, num_sms());
-  range_attn_kernel<D, CAP, BIAS><<<grid, RT_THREADS, RangeTileCfg<D>::SMEM, st>>>(tq, tk, tv, g);
-  if (g.splits > 1) range_combine_kernel<D><<<(unsigned)((g.part_rows + 7) / 8), 256, 0, st>>>(g);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return set_cuda_error("range attention launch", e);
-  return WANB200_OK;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>(g.units, num_sms()));
+  cfg.blockDim = dim3(RT_THREADS);
+  cfg.dynamicSmemBytes = RangeTileCfg<D>::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, range_attn_kernel<D, CAP, BIAS>, tq, tk, tv, g);
+  if (e != cudaSuccess) return set_cuda_error("range_attn_kernel launch", e);
+  return g.splits > 1 ? launch_range_combine<D>(g.a, g.parts, st) : WANB200_OK;
 }
 
+// The few-rows kernel (d) or the tiles (g with the maps of q, k and v).
 template <int D>
-static int range_dispatch(const RangeArgs& a, const RangeTileArgs* g, const CUtensorMap* maps, int rows, cudaStream_t st) {
+static int range_dispatch(const RangeArgs& a, const DecodeLaunch* d, const RangeTileArgs* g, const CUtensorMap* maps,
+                          cudaStream_t st) {
   const int bias = a.slopes ? kBiasSlopes : a.table ? kBiasTable : kBiasNone;
 #define WANB200_RANGE_CASE(cap, bs) \
-  return g ? launch_range_tiles<D, cap, bs>(maps[0], maps[1], maps[2], *g, st) : launch_range_decode<D, cap, bs>(a, rows, st)
+  return g ? launch_range_tiles<D, cap, bs>(maps[0], maps[1], maps[2], *g, st) : launch_range_decode<D, cap, bs>(a, *d, st)
   if (a.cap2 > 0.f) {
     if (bias == kBiasSlopes) WANB200_RANGE_CASE(true, kBiasSlopes);
     if (bias == kBiasTable) WANB200_RANGE_CASE(true, kBiasTable);
@@ -1325,30 +1482,50 @@ int range_attn_fwd(const wanb200_range_attn_params* p, cudaStream_t st) {
   a.table = p->dist_bias;
   a.reach = p->reach;
   const int64_t rows = p->q_len * a.group;
-  if (rows <= RD_ROWS) {
-    return p->head_dim == 64 ? range_dispatch<64>(a, nullptr, nullptr, (int)rows, st)
-                             : range_dispatch<128>(a, nullptr, nullptr, (int)rows, st);
-  }
+  const bool few = rows <= RD_ROWS;
   const RangeLayout l = range_layout(p);
-  if (l.units <= 0 || l.units > INT32_MAX / 2 || (l.part_rows + 7) / 8 > INT32_MAX)
+  if ((!few && l.units <= 0) || l.units > INT32_MAX / 2 || l.part_rows > INT32_MAX)
     return set_error(WANB200_EINVAL, "range_attn: too many rows");
-  if (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255u) || p->workspace_bytes < l.bytes)
+  if (l.bytes > 0 &&
+      (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255u) || p->workspace_bytes < l.bytes))
     return set_error(WANB200_EINVAL, "range_attn: need a 256-byte aligned workspace of wanb200_range_attn_workspace_bytes()");
+  uint8_t* ws = static_cast<uint8_t*>(p->workspace);
+  RangeParts parts;
+  parts.o = reinterpret_cast<float*>(ws + l.part_off);
+  parts.ml = reinterpret_cast<float2*>(ws + l.ml_off);
+  parts.first = few ? reinterpret_cast<int4*>(ws) : nullptr;
+  parts.slot_rows = (int)rows;
+  parts.groups = (int)(p->batch * p->kv_heads);
+  parts.splits = l.splits;
   int* err = device_error_word();
   if (!err) return WANB200_ECUDA;
   CUtensorMap maps[3];
   const int D = (int)p->head_dim;
-  const int64_t dq[4] = {D, p->heads, p->q_len, p->batch}, sq[4] = {1, D, p->q_tok_stride, p->q_batch_stride};
-  const int boxq[4] = {64, a.group, l.tpt, 1}, boxk[4] = {64, 1, RT_N, 1};
-  rc = make_tmap_4d(&maps[0], p->q, dq, sq, boxq);
-  if (rc) return rc;
+  const int boxk[4] = {64, 1, few ? RD_TILE : RT_N, 1};
   const int64_t dk[4] = {D, p->kv_heads, p->kv_len, p->batch}, sk[4] = {1, D, p->k_tok_stride, p->k_batch_stride};
   rc = make_tmap_4d(&maps[1], p->k, dk, sk, boxk);
   if (rc) return rc;
   const int64_t sv[4] = {1, D, p->v_tok_stride, p->v_batch_stride};
   rc = make_tmap_4d(&maps[2], p->v, dk, sv, boxk);
   if (rc) return rc;
-  uint8_t* ws = static_cast<uint8_t*>(p->workspace);
+  if (few) {
+    const int64_t blocks = range_decode_blocks(p);
+    if (blocks > INT32_MAX) return set_error(WANB200_EINVAL, "range_attn: too many rows");
+    DecodeLaunch d;
+    d.parts = parts;
+    d.k = maps[1];
+    d.v = maps[2];
+    d.rows = (int)rows;
+    d.blocks = (int)blocks;
+    d.slots = range_decode_slots(p);
+    d.err = err;
+    return D == 64 ? range_dispatch<64>(a, &d, nullptr, nullptr, st) : range_dispatch<128>(a, &d, nullptr, nullptr, st);
+  }
+  if (rows > INT32_MAX || p->batch * p->kv_heads > INT32_MAX) return set_error(WANB200_EINVAL, "range_attn: too many rows");
+  const int64_t dq[4] = {D, p->heads, p->q_len, p->batch}, sq[4] = {1, D, p->q_tok_stride, p->q_batch_stride};
+  const int boxq[4] = {64, a.group, l.tpt, 1};
+  rc = make_tmap_4d(&maps[0], p->q, dq, sq, boxq);
+  if (rc) return rc;
   RangeTileArgs g;
   g.a = a;
   g.tpt = l.tpt;
@@ -1362,11 +1539,11 @@ int range_attn_fwd(const wanb200_range_attn_params* p, cudaStream_t st) {
   g.pairs = reinterpret_cast<const RangePair*>(ws);
   g.order = reinterpret_cast<const int*>(ws + l.order_off);
   g.counter = reinterpret_cast<int*>(ws + l.counter_off);
-  g.o_part = reinterpret_cast<float*>(ws + l.part_off);
-  g.ml_part = reinterpret_cast<float2*>(ws + l.ml_off);
-  g.part_rows = l.part_rows;
+  g.parts = parts;
+  g.padded = p->dist_bias ? reinterpret_cast<const float*>(ws + l.pad_off) : nullptr;
+  g.cap_scale = p->softcap > 0.f ? p->softmax_scale / p->softcap : 0.f;
   g.err = err;
-  return D == 64 ? range_dispatch<64>(a, &g, maps, 0, st) : range_dispatch<128>(a, &g, maps, 0, st);
+  return D == 64 ? range_dispatch<64>(a, nullptr, &g, maps, st) : range_dispatch<128>(a, nullptr, &g, maps, st);
 }
 
 }  // namespace wanb200

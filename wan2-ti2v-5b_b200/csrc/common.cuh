@@ -279,6 +279,12 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return m;
 }
 
+__device__ __forceinline__ float fmin3(float a, float b, float c) {
+  float m;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+
 // UMMA instruction descriptor, kind::f16 with bf16 A/B and fp32 D.
 // Bits: [4,6) D fmt (1=f32), [7,10) A fmt (1=bf16), [10,13) B fmt, 15 A MN-major, 16 B MN-major,
 // [17,23) N>>3, [24,29) M>>4.
@@ -436,17 +442,6 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {
   return v;
 }
 
-// Asynchronous 16-byte copies to shared memory, counted in groups per thread; zeros, without a read,
-// where !in.  A thread that reads back only what it copied itself needs no barrier, only the wait:
-// a prefetch that takes no registers.
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {  // all but the newest N groups have landed
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
@@ -460,6 +455,14 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Transposes an 8 x 8 matrix of 16-bit values over a warp (fragment layout of mma: lane / 4 = row, the two
+// values of lane % 4 its columns).
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
 }
 
 // Hardware tanh (one MUFU op; PTX tanh.approx.f32, max relative error 2^-11, far below the bf16

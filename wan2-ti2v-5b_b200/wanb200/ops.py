@@ -481,7 +481,7 @@ def range_attention(q, k, v, lo, hi, *, pos=None, out=None, softmax_scale=None, 
     with H a multiple of Hkv (query head h reads key head h // (H / Hkv)), D 64 or 128, head stride
     D.  lo, hi (and pos): int32 [Lq] for every batch element or [B, Lq]; a row with no keys gives
     zeros.  softcap c > 0: scores c tanh(s / c).  slopes [H] fp32: bias -slopes[h] |j - pos|;
-    dist_bias [H, 2R + 1] fp32: bias dist_bias[h, clamp(j - pos, -R, R) + R]; pos defaults to the
+    dist_bias [H, 2R + 1] fp32, R <= 8192: bias dist_bias[h, clamp(j - pos, -R, R) + R]; pos defaults to the
     row index.  lo, hi and pos are read on the device at every call, so a captured graph follows
     them.  wanb200.ranges has the common masks (packed documents, caches)."""
     dev = _device_index(q, k, v, lo, hi, pos, out, slopes, dist_bias)
@@ -539,7 +539,7 @@ def range_attention(q, k, v, lo, hi, *, pos=None, out=None, softmax_scale=None, 
                           hi.data_ptr(), _p(pos), Lq if B > 1 and len(shape) == 2 and shape[0] == B else 0, _p(slopes),
                           _p(dist_bias), reach)
     lib = L.load()
-    nbytes = lib.wanb200_range_attn_workspace_bytes(p) if Lq * (H // Hkv) > 16 else 0
+    nbytes = lib.wanb200_range_attn_workspace_bytes(p)
     if nbytes:  # from torch's allocator: ordered on this stream, and a captured graph's own
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
