@@ -28,9 +28,15 @@ struct HeadNormArgs {
 // passes of one row, all loads in flight before the first use.  Sums and the norm are fp32 over
 // the head's lanes (a butterfly inside the lane group); the lane's angles are read once per row
 // and serve all its heads.  Interleaved pairs live inside a lane; half-split pairs (i, i + rot/2)
-// are exchanged with the partner lane by shuffles.  One rounding, to bf16, at the store.
+// are exchanged with the partner lane by shuffles.  One rounding, to bf16, at the store.  x and the
+// output go past the L1 (streaming hints), which keeps the angles that a row's warps share.
+//
+// NV by a sweep at 15708 x 48 heads of 128 (390 MB): 1 124 us, 2 116, 4 96, 6 91, 8 95 without hints, and
+// 111, 98, 83, 78 (4980 GB/s, 0.77 of the measured copy rate), 83 with them; more registers than
+// four blocks an SM leave cost more than the loads in flight gain.  A single row of 48 heads: 2.4,
+// 2.7, 3.5, 4.0 us.
 template <int LPH, int NV, bool INTER>
-__global__ void __launch_bounds__(256) head_norm_rope_kernel(const HeadNormArgs a) {
+__global__ void __launch_bounds__(256, 4) head_norm_rope_kernel(const HeadNormArgs a) {
   constexpr int HP = 32 / LPH, D = LPH * 8;
   const int lane = threadIdx.x & 31;
   const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -45,8 +51,8 @@ __global__ void __launch_bounds__(256) head_norm_rope_kernel(const HeadNormArgs 
     raw[i] = make_uint4(0u, 0u, 0u, 0u);
     if (h < a.heads) {
       const int s = h >= a.heads0;
-      raw[i] = *reinterpret_cast<const uint4*>(a.x + row * a.ldx + (s ? a.col0[1] : a.col0[0]) +
-                                               (int64_t)(h - (s ? a.heads0 : 0)) * D + 8 * c);
+      raw[i] = __ldcs(reinterpret_cast<const uint4*>(a.x + row * a.ldx + (s ? a.col0[1] : a.col0[0]) +
+                                                     (int64_t)(h - (s ? a.heads0 : 0)) * D + 8 * c));
     }
   }
   const int half = a.rot >> 4;  // lanes of one half of the rotated channels (half-split pairs)
@@ -114,8 +120,9 @@ __global__ void __launch_bounds__(256) head_norm_rope_kernel(const HeadNormArgs 
       u.y = pack_bf16x2(x[2], x[3]);
       u.z = pack_bf16x2(x[4], x[5]);
       u.w = pack_bf16x2(x[6], x[7]);
-      *reinterpret_cast<uint4*>(a.out + row * a.ldo + (s ? a.col0[1] : a.col0[0]) +
-                                (int64_t)(h - (s ? a.heads0 : 0)) * D + 8 * c) = u;
+      __stcs(reinterpret_cast<uint4*>(a.out + row * a.ldo + (s ? a.col0[1] : a.col0[0]) +
+                                      (int64_t)(h - (s ? a.heads0 : 0)) * D + 8 * c),
+             u);
     }
   }
 }
@@ -132,8 +139,10 @@ template <int LPH>
 static void launch_head_norm(const HeadNormArgs& a, int nv, bool inter, unsigned blocks, cudaStream_t st) {
   if (nv == 1)
     launch_head_norm<LPH, 1>(a, inter, blocks, st);
+  else if (nv == 2)
+    launch_head_norm<LPH, 2>(a, inter, blocks, st);
   else
-    launch_head_norm<LPH, 4>(a, inter, blocks, st);
+    launch_head_norm<LPH, 6>(a, inter, blocks, st);
 }
 
 int head_norm_rope(const wanb200_headnorm_params* p, cudaStream_t st) {
@@ -190,7 +199,10 @@ int head_norm_rope(const wanb200_headnorm_params* p, cudaStream_t st) {
   a.table_rows = p->cos ? p->table_rows : 1;
   a.err = err;
   const int lph = p->head_dim / 8, hp = 32 / lph;
-  const int nv = 4;
+  // the most passes a warp that still leave every SM its 32 warps; few rows: one each, for latency
+  // (1999 rows of 40 heads of 64: 10.6, 10.3, 10.7 us with 1, 2, 6)
+  const int64_t passes = (heads + hp - 1) / hp, fill = (int64_t)num_sms() * 32;
+  const int nv = p->rows * ((passes + 5) / 6) >= fill ? 6 : p->rows * ((passes + 1) / 2) >= fill / 2 ? 2 : 1;
   a.groups = (int)((heads + hp * nv - 1) / (hp * nv));
   const int64_t blocks = (p->rows * a.groups + 7) / 8;
   if (p->rows > INT32_MAX || blocks > INT32_MAX) return set_error(WANB200_EINVAL, "head_norm_rope: too many rows");
