@@ -105,7 +105,9 @@ int wanb200_gemm_bf16(const wanb200_gemm_params* p, void* stream);
  * the accumulators before the epilogue (bias, GELU, gate, residual); all epilogues but SUMSQ and
  * SCATTER.  The rank-wide intermediate is held in bf16, or for fp32 outputs in two bf16 planes
  * (16 significant bits).  NaN or infinite weights of an adapter reach the rows that use it only.
- * An id >= adapters counts as none and sets the device error word to 502.
+ * An id >= adapters counts as none and sets the device error word to 502.  d must not overlap a (it
+ * may alias residual); tile_n does not act on calls of up to 16 rows, which read w once with other
+ * kernels and keep the intermediate in fp32.
  * Limits: rank % 8 == 0, adapters * rank <= 4096, 16-byte aligned down and up, and the GEMM's. */
 typedef struct wanb200_lora_params {
   wanb200_gemm_params gemm;
@@ -272,7 +274,7 @@ int wanb200_head_norm_rope(const wanb200_headnorm_params* p, void* stream);
  *   lo, hi    [q_len] int32 per batch element (range_batch_stride elements apart, 0 = shared); the
  *             range is clipped to 0 .. kv_len; a row with an empty range gives zeros.  Documents,
  *             causal and frame-causal order, a prefix, a window and padding all are such ranges
- *   softcap   cap(s) = softcap * tanh(s / softcap); 0 = none
+ *   softcap   cap(s) = softcap * tanh(s / softcap), 1e-6 .. 1e6; 0 = none
  *   slopes    bias = -slopes[h] * |j - pos|, [heads] fp32
  *   dist_bias bias = dist_bias[h][clamp(j - pos, -reach, reach) + reach], [heads, 2 reach + 1] fp32
  *             (a relative-position table, reach <= 8192; at most one of the two)

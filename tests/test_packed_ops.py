@@ -126,7 +126,8 @@ def _range_params():
     ("q", None, "null"), ("lo", None, "null"), ("head_dim", 96, "head_dim"), ("q_len", 0, "positive"),
     ("kv_len", 0, "positive"), ("kv_heads", 3, "multiple"), ("k_tok_stride", 100, "multiples of 8"),
     ("k_tok_stride", 64, "token stride"), ("v", 4104, "aligned"), ("softmax_scale", 0.0, "softmax_scale"),
-    ("softmax_scale", float("nan"), "softmax_scale"), ("softcap", -1.0, "softcap"), ("softcap", float("inf"), "softcap"),
+    ("softmax_scale", float("nan"), "softmax_scale"), ("softmax_scale", float("inf"), "softmax_scale"),
+    ("softcap", -1.0, "softcap"), ("softcap", 1e-20, "softcap"), ("softcap", float("nan"), "softcap"), ("softcap", float("inf"), "softcap"),
     ("range_batch_stride", -1, "range_batch_stride"), ("kv_len", 2 ** 31, "too large")])
 def test_range_attention_refuses_on_host(field, value, word):
     p = _range_params()
@@ -138,8 +139,10 @@ def test_range_attention_refuses_two_biases_and_bad_reach_on_host():
     p = _range_params()
     p.slopes = p.dist_bias = 4096
     _refused(L.load().wanb200_range_attn_fwd, p, "not both")
-    p.slopes, p.reach = None, -1
-    _refused(L.load().wanb200_range_attn_fwd, p, "reach")
+    for reach in (-1, 8193):
+        p.slopes, p.reach = None, reach
+        _refused(L.load().wanb200_range_attn_fwd, p, "reach")
+        assert L.load().wanb200_range_attn_workspace_bytes(ctypes.byref(p)) == 0
 
 
 def _lora_params():
@@ -396,6 +399,41 @@ def test_range_attention_many_units_a_block(lengths, block, prefix, H, Hkv, D, w
 
 
 @pytest.mark.gpu
+def test_range_attention_many_short_sequences(word):
+    """More tile pairs than the plan sorts, and more (key head, batch element) pairs than the few-rows
+    kernel deals out."""
+    for B, Lq, H, Hkv in ((1100, 17, 2, 2), (500, 2, 4, 2)):
+        q, k, v = randn(B, Lq, H, 64, seed=1), randn(B, 40, Hkv, 64, seed=2), randn(B, 40, Hkv, 64, seed=3)
+        check_attn(q, k, v, *random_ranges(B, Lq, 40, 5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,Hkv", [(10, 1), (7, 1), (96, 1), (24, 2)])
+def test_range_attention_groups_that_do_not_fill_a_tile(H, Hkv, word):
+    """Key heads shared by numbers of query heads that leave rows of the 128-row tile unused."""
+    for Lq in (1, 3, 150):
+        q, k, v = randn(1, Lq, H, 128, seed=1), randn(1, 300, Hkv, 128, seed=2), randn(1, 300, Hkv, 128, seed=3)
+        lo, hi = random_ranges(1, Lq, 300, 6)
+        check_attn(q, k, v, lo, hi, cap=20.0)
+        check_attn(q, k, v, lo, hi, slopes=torch.rand(H, device=DEV))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Lq", [1, 4, 130])
+def test_range_attention_long_cache_of_unequal_lengths(Lq, word):
+    """Caches from nothing to 5000 keys in one batch, views of a larger cache."""
+    B, H, Hkv, D = 7, 8, 4, 64
+    cache = randn(2, B, 5100, Hkv, D, seed=7)
+    k, v = cache[0, :, 50:5050], cache[1, :, 50:5050]
+    q = randn(B, Lq, H, D, seed=8)
+    lens = torch.tensor([0, 1, 5000, 77, 64, 4097, 2048], dtype=torch.int32, device=DEV)
+    lo, hi, pos = ranges.cache_ranges(lens, Lq)
+    check_attn(q, k, v, lo, hi, pos=pos, slopes=torch.rand(H, device=DEV) * 0.1)
+    lo, hi, pos = ranges.cache_ranges(lens, Lq, window=100)
+    check_attn(q, k, v, lo, hi, pos=pos)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("cap", [0.0, 5.0, 50.0])
 @pytest.mark.parametrize("bias", ["none", "slopes", "table", "short_table", "flat_table"])
@@ -537,7 +575,8 @@ def lora_case(M, K, N, n, r, seed, order="mixed"):
 @pytest.mark.parametrize("M,K,N,n,r,order", [
     (1, 64, 32, 1, 8, "mixed"), (1, 512, 96, 5, 16, "mixed"), (4, 1024, 256, 8, 16, "mixed"), (13, 256, 160, 3, 24, "mixed"),
     (16, 2048, 64, 20, 64, "mixed"), (17, 128, 64, 2, 8, "sorted"), (100, 320, 544, 9, 40, "mixed"), (129, 64, 64, 16, 16, "sorted"),
-    (300, 704, 256, 4, 64, "sorted"), (400, 256, 1056, 32, 128, "mixed"), (1000, 192, 96, 3, 8, "sorted")])
+    (300, 704, 256, 4, 64, "sorted"), (400, 256, 1056, 32, 128, "mixed"), (1000, 192, 96, 3, 8, "sorted"),
+    (509, 2048, 512, 16, 16, "mixed"), (60, 4096, 320, 7, 40, "mixed"), (2500, 512, 1024, 2, 64, "sorted")])
 def test_lora_linear(M, K, N, n, r, order, word):
     x, w, b, down, up, ids, scales = lora_case(M, K, N, n, r, 21, order)
     got = ops.lora_linear(x, w, b, down, up, ids, scales=scales)

@@ -1023,7 +1023,8 @@ __global__ void __maxnreg__(160)
               lo8[c] = fmin3(lo8[c], s[8 * q + 2 * c], s[8 * q + 2 * c + 1]);
             }
           const float top_hi = fmax3(hi8[0], hi8[1], fmaxf(hi8[2], hi8[3]));
-          const float top = fmaxf(top_hi, -fmin3(lo8[0], lo8[1], fminf(lo8[2], lo8[3])));
+          // rows that are not stored do not hold the others back from the short form
+          const float top = live ? fmaxf(top_hi, -fmin3(lo8[0], lo8[1], fminf(lo8[2], lo8[3]))) : 0.f;
           if (__all_sync(0xffffffffu, top * g.cap_scale <= 0.6f)) {
             // |x| = |score| / cap <= 0.6: tanh x = x P(x^2), P fitted to 5.9e-7 (least maximum error of an
             // odd polynomial of degree 7 on [0, 0.6]): 3e-5 of a score capped at 50, far below the bf16
@@ -1329,10 +1330,10 @@ static int range_validate(const wanb200_range_attn_params* p) {
     return set_error(WANB200_EINVAL, "range_attn: token stride smaller than heads * head_dim");
   if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) || !aligned16(p->o))
     return set_error(WANB200_EINVAL, "range_attn: q/k/v/o must be 16-byte aligned");
-  if (!(p->softmax_scale > 0.f) || !(p->softmax_scale < INFINITY))
-    return set_error(WANB200_EINVAL, "range_attn: softmax_scale must be positive");
-  if (!(p->softcap >= 0.f) || !(p->softcap < INFINITY))
-    return set_error(WANB200_EINVAL, "range_attn: softcap must be >= 0 (0 = none)");
+  if (!(p->softmax_scale >= 1e-12f && p->softmax_scale <= 1e12f))
+    return set_error(WANB200_EINVAL, "range_attn: softmax_scale must lie in 1e-12 .. 1e12");
+  if (p->softcap != 0.f && !(p->softcap >= 1e-6f && p->softcap <= 1e6f))
+    return set_error(WANB200_EINVAL, "range_attn: softcap must be 0 (none) or in 1e-6 .. 1e6");
   if (p->slopes && p->dist_bias) return set_error(WANB200_EINVAL, "range_attn: slopes or dist_bias, not both");
   if (p->dist_bias && (p->reach < 0 || p->reach > RT_REACH_MAX))
     return set_error(WANB200_EINVAL, "range_attn: dist_bias needs 0 <= reach <= 8192");

@@ -255,10 +255,44 @@ __device__ __noinline__ float lora_slow_value(const LoraPlan* lo, int row, int c
   return v;
 }
 
-__device__ __forceinline__ void lora_add_slow(const LoraPlan* lo, float* v, int row, int col0, int M) {
-  if (row >= M) return;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] += lora_slow_value(lo, row, col0 + i);
+// The whole epilogue of a tile that has such weights, value by value, for the warp on lane quarter
+// `quad` that takes the 32-column chunks half, half + 2, ...  A function of its own, so that nothing
+// of it burdens the registers of the ordinary epilogue.
+template <int EPI>
+__device__ __noinline__ void lora_slow_tile(const GemmArgs* ap, const LoraPlan* lo, uint32_t t_row, int m0, int n0, int quad,
+                                            int half, int lane) {
+  const GemmArgs& a = *ap;
+  const int row = m0 + quad * 32 + lane;
+  for (int c = half; c < a.bn / 32; c += 2) {
+    if (n0 + c * 32 >= a.N) break;  // warp-uniform
+    float v[32];
+    __syncwarp();
+    tmem_ld32(t_row + c * 32, v);
+    if (row >= a.M) continue;
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i) {
+      const int n = n0 + c * 32 + i;
+      float x = v[i] + lora_slow_value(lo, row, n);
+      if constexpr (EPI != WANB200_EPI_NONE) x += __bfloat162float(a.bias[n]);
+      if constexpr (EPI == WANB200_EPI_BIAS_GELU) x = gelu_tanh(x);
+      if constexpr (EPI == WANB200_EPI_BIAS_SILU) x = silu(x);
+      if constexpr (epi_has_residual(EPI)) {
+        const int64_t at = (int64_t)row * a.ldr + n;
+        const float r = a.res_f32 ? static_cast<const float*>(a.residual)[at]
+                                  : __bfloat162float(static_cast<const __nv_bfloat16*>(a.residual)[at]);
+        if constexpr (EPI == WANB200_EPI_BIAS_GATE_RES) {
+          const int64_t f = frame_of_row(row, a.rows_per_seq, a.row_offset, a.seq_len, a.tokens_per_frame);
+          x = r + x * (__bfloat162float(a.gate_mod[n]) + a.gate_e0[f * a.gate_frame_stride + n]);
+        } else {
+          x += r;
+        }
+      }
+      if (a.out_f32)
+        static_cast<float*>(a.d)[(int64_t)row * a.ldd + n] = x;
+      else
+        static_cast<__nv_bfloat16*>(a.d)[(int64_t)row * a.ldd + n] = __float2bfloat16(x);
+    }
+  }
 }
 
 // A tile whose K is shared by the blocks of a cluster.  Every block leaves its fp32 sums in its
@@ -348,9 +382,9 @@ __device__ __forceinline__ void lora_join_rows(const GemmArgs& a, const LoraPlan
 // swizzled by the row's low three bits: the row-per-lane writes and the row-segment reads are
 // both free of bank conflicts.  The arithmetic per element is gemm_epilogue_chunk's (bias add,
 // then r + v * g for GATE_RES, v + r for RES), so both paths give the same bits.
-template <int EPI, bool LORA>
-__device__ __forceinline__ void residual_tile_staged(const GemmArgs& a, const LoraPlan* lora, bool slow, float* stg,
-                                                     uint32_t t_row, int m0, int n0, int quad, int half, int lane) {
+template <int EPI>
+__device__ __forceinline__ void residual_tile_staged(const GemmArgs& a, float* stg, uint32_t t_row, int m0, int n0,
+                                                     int quad, int half, int lane) {
   const int sub = lane >> 3, cg = lane & 7;
   const int rbase = m0 + quad * 32 + sub;  // the row of i = 0; a lane's rows step by 4
   int fr[8];
@@ -382,9 +416,6 @@ __device__ __forceinline__ void residual_tile_staged(const GemmArgs& a, const Lo
     const bool more = c + 2 < nchunks && col0 + 64 < a.N;
     float v[32];
     tmem_ld32(t_row + c * 32, v);
-    if constexpr (LORA) {
-      if (slow) lora_add_slow(lora, v, m0 + quad * 32 + lane, col0, a.M);
-    }
 #pragma unroll
     for (int q = 0; q < 8; ++q)
       *reinterpret_cast<float4*>(stg + lane * 32 + ((q ^ (lane & 7)) << 2)) =
@@ -733,8 +764,12 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       tile_origin(tile, num_m, num_n, bn, m0, n0);
       const int row = m0 + r;
       bool slow = false;
-      if constexpr (LORA) slow = *reinterpret_cast<volatile int*>(lora_tile_bad + acc) != 0;
-      if constexpr (EPI == WANB200_EPI_SCATTER) {
+      if constexpr (LORA) {
+        slow = *reinterpret_cast<volatile int*>(lora_tile_bad + acc) != 0;
+        if (slow) lora_slow_tile<EPI>(&args, lora, t_row, m0, n0, quad, half, lane);
+      }
+      if (slow) {  // done above
+      } else if constexpr (EPI == WANB200_EPI_SCATTER) {
         // stage this warp's 32 rows (lane = row), then write each row as one 512-byte segment
         // (the first warp of each lane quarter does the whole tile; the second only arrives)
         constexpr int SR = GemmCfg<EPI>::STAGING_ROW;
@@ -762,7 +797,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       } else if (epi_has_residual(EPI) && args.res_staging) {
         if constexpr (epi_has_residual(EPI)) {
           float* stg = reinterpret_cast<float*>(smem + args.tiles_bytes + GemmCfg<EPI>::STAGING) + (warp - 2) * 1024;
-          residual_tile_staged<EPI, LORA>(args, lora, slow, stg, t_row, m0, n0, quad, half, lane);
+          residual_tile_staged<EPI>(args, stg, t_row, m0, n0, quad, half, lane);
         }
       } else {
         uint4 res_next[8] = {}, res_cur[8];
@@ -786,9 +821,6 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
           }
           float v[32];
           tmem_ld32(t_row + c * 32, v);
-          if constexpr (LORA) {
-            if (slow) lora_add_slow(lora, v, row, col0, args.M);
-          }
           gemm_epilogue_chunk<EPI>(args, v, row, col0, res_cur, gate_row);
         }
       }
@@ -822,7 +854,7 @@ template <int EPI>
 __global__ void __launch_bounds__(G_LORA_THREADS, 1)
     gemm_lora_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmU,
-                     const GemmArgs args, const __grid_constant__ LoraPlan lora) {
+                     const __grid_constant__ GemmArgs args, const __grid_constant__ LoraPlan lora) {
   gemm_body<EPI, true>(tmA, tmB, &tmH, &tmU, args, &lora);
 }
 
