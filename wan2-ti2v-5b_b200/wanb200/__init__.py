@@ -6,7 +6,7 @@ sequence-parallel block of `WanSelfAttentionSP`), `FastBlockSP` (= `_FastBlockSP
 `FastCrossKV` (= `_FastCrossKV`), `FastWanDiT`; the device-side sampler and denoise loop
 (`FlowUniPC`, `denoise`); the checkpoint reader (`load_wan_checkpoint`,
 `FastWanDiT.from_checkpoint`); process-group layouts in `wanb200.parallel`; kernel ops in
-`wanb200.ops`.
+`wanb200.ops`, the key ranges of its masked attention in `wanb200.ranges`.
 """
 from ._lib import LIB_PATH, WanB200Error, device_error, load  # noqa: F401
 from .block import FastBlock, FastBlockSP, FastCrossKV  # noqa: F401

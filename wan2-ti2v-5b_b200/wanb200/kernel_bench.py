@@ -5,6 +5,10 @@
     python -m wanb200.kernel_bench ln --M 15708 --C 3072 [--f32]
     python -m wanb200.kernel_bench qknorm --M 15708 --C 3072
     python -m wanb200.kernel_bench gemm --M 15708 --N 3072 --K 3072 --epi gate_res --f32
+    python -m wanb200.kernel_bench headnorm --M 15708 --H 24 --Hkv 24
+    python -m wanb200.kernel_bench range --B 16 --H 24 --Hkv 8 --Lq 1 --Lk 4096
+    python -m wanb200.kernel_bench range --B 1 --H 24 --Hkv 24 --Lq 7854 --Lk 7854 --block 374 [--softcap 30]
+    python -m wanb200.kernel_bench lora --M 15708 --N 4096 --K 4096 --adapters 4 --rank 64 [--mixed]
 
 (run from wan2-ti2v-5b_b200/ or with it on sys.path).  Prints one JSON line with the mean
 time per launch and the algorithmic TFLOP/s or GB/s.  Used for sweeps and as the small-case
@@ -18,7 +22,7 @@ import json
 import torch
 
 from . import _lib as L
-from . import ops
+from . import ops, ranges
 
 EPIS = {"none": L.EPI_NONE, "bias": L.EPI_BIAS, "gelu": L.EPI_BIAS_GELU, "gate_res": L.EPI_BIAS_GATE_RES,
         "res": L.EPI_BIAS_RES, "sumsq": L.EPI_BIAS_SUMSQ}
@@ -127,9 +131,59 @@ def bench_qknorm(a):
     return {"kernel": "qk_norm_rope", "M": M, "C": C, "ss": a.ss, "ms": ms, "gbs": nbytes / ms / 1e6}
 
 
+def bench_headnorm(a):
+    """Per-head norm and rotation of the q and k sections of a fused projection's output, out of place."""
+    D, cols = a.D, (a.H + 2 * a.Hkv) * a.D
+    x = torch.randn(a.M, cols, device="cuda").to(torch.bfloat16)
+    out = torch.empty_like(x)
+    g = torch.ones(D, device="cuda", dtype=torch.bfloat16)
+    ang = torch.rand(a.M, D // 2, device="cuda")
+    cos, sin = ang.cos(), ang.sin()
+    pos = torch.arange(a.M, device="cuda", dtype=torch.int32)
+    secs = [(0, a.H, g), (a.H * D, a.Hkv, g)]
+    ms = _time(lambda: ops.head_norm_rope(x, secs, D, out=out, cos=cos, sin=sin, positions=pos), a.iters)
+    nbytes = 4 * a.M * (a.H + a.Hkv) * D + 4 * a.M * D
+    return {"kernel": "head_norm_rope", "M": a.M, "H": a.H, "Hkv": a.Hkv, "D": D, "ms": ms, "gbs": nbytes / ms / 1e6}
+
+
+def bench_range(a):
+    """Attention over key ranges: Lq == Lk packs two documents of half the rows each (--block n: block-
+    causal), Lq < Lk are the last Lq tokens of full caches; FLOPs and bytes of the visible keys."""
+    D, B, Lq, Lk = a.D, a.B, a.Lq, a.Lk
+    q = torch.randn(B, Lq, a.H, D, device="cuda").to(torch.bfloat16)
+    k, v = (torch.randn(B, Lk, a.Hkv, D, device="cuda").to(torch.bfloat16) for _ in range(2))
+    pos = None
+    if Lq == Lk:
+        lo, hi = ranges.document_ranges([Lk - Lk // 2, Lk // 2], "cuda", block=a.block)
+    else:
+        lo, hi, pos = ranges.cache_ranges(torch.full((B,), Lk, dtype=torch.int32, device="cuda"), Lq)
+    out = torch.empty_like(q)
+    ms = _time(lambda: ops.range_attention(q, k, v, lo, hi, pos=pos, out=out, softcap=a.softcap), a.iters)
+    pairs = float((hi - lo).sum()) * (1 if lo.dim() == 2 else B) * a.H
+    nbytes = 4 * B * Lq * a.H * D + 4 * B * Lk * a.Hkv * D
+    return {"kernel": "range_attention", "B": B, "H": a.H, "Hkv": a.Hkv, "D": D, "Lq": Lq, "Lk": Lk, "block": a.block,
+            "softcap": a.softcap, "ms": ms, "tflops": 4 * pairs * D / ms / 1e9, "gbs": nbytes / ms / 1e6}
+
+
+def bench_lora(a):
+    """The projection with per-row adapters (requests one after the other, or --mixed), and without."""
+    bf = torch.bfloat16
+    x, w = torch.randn(a.M, a.K, device="cuda").to(bf), (torch.randn(a.N, a.K, device="cuda") * 0.02).to(bf)
+    b = torch.zeros(a.N, device="cuda", dtype=bf)
+    down, up = (torch.randn(a.adapters, a.rank, a.K, device="cuda") * 0.02).to(bf), torch.randn(a.N, a.adapters, a.rank, device="cuda").to(bf)
+    ids = torch.arange(a.M, device="cuda") % a.adapters
+    ids = (ids if a.mixed else ids.sort().values).to(torch.int32)
+    out = torch.empty(a.M, a.N, device="cuda", dtype=bf)
+    ms = _time(lambda: ops.lora_linear(x, w, b, down, up, ids, out=out), a.iters)
+    base = _time(lambda: ops.linear(x, w, b, out=out), a.iters)
+    fl = 2 * a.M * a.N * a.K + 2 * a.M * a.rank * (a.K + a.N)
+    return {"kernel": "lora_linear", "M": a.M, "N": a.N, "K": a.K, "adapters": a.adapters, "rank": a.rank, "mixed": a.mixed,
+            "ms": ms, "ms_without": base, "tflops": fl / ms / 1e9}
+
+
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("kind", choices=["gemm", "attn", "ln", "qknorm"])
+    ap.add_argument("kind", choices=["gemm", "attn", "ln", "qknorm", "headnorm", "range", "lora"])
     ap.add_argument("--M", type=int, default=15708)
     ap.add_argument("--N", type=int, default=14336)
     ap.add_argument("--K", type=int, default=3072)
@@ -137,6 +191,13 @@ def main():
     ap.add_argument("--epi", default="gelu", choices=sorted(EPIS))
     ap.add_argument("--B", type=int, default=2)
     ap.add_argument("--H", type=int, default=24)
+    ap.add_argument("--Hkv", type=int, default=24, help="headnorm / range: key heads")
+    ap.add_argument("--D", type=int, default=128, help="headnorm / range: head dim")
+    ap.add_argument("--block", type=int, default=0, help="range: tokens of a causal block (0 = whole documents)")
+    ap.add_argument("--softcap", type=float, default=0.0, help="range: tanh cap of the scores")
+    ap.add_argument("--adapters", type=int, default=4, help="lora: adapters")
+    ap.add_argument("--rank", type=int, default=64, help="lora: rank")
+    ap.add_argument("--mixed", action="store_true", help="lora: rows of all adapters interleaved")
     ap.add_argument("--Lq", type=int, default=7854)
     ap.add_argument("--Lk", type=int, default=7854)
     ap.add_argument("--iters", type=int, default=20)
@@ -149,7 +210,8 @@ def main():
     ap.add_argument("--ss", default="self", choices=["self", "partials", "sums"], help="qknorm: where the sums of squares come from")
     a = ap.parse_args()
     torch.cuda.set_device(0)
-    r = {"gemm": bench_gemm, "attn": bench_attn, "ln": bench_ln, "qknorm": bench_qknorm}[a.kind](a)
+    r = {"gemm": bench_gemm, "attn": bench_attn, "ln": bench_ln, "qknorm": bench_qknorm,
+         "headnorm": bench_headnorm, "range": bench_range, "lora": bench_lora}[a.kind](a)
     r["device_error"] = L.device_error(reset=True)
     print(json.dumps(r), flush=True)
 
