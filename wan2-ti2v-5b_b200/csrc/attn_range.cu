@@ -563,11 +563,18 @@ __global__ void __launch_bounds__(1024) range_plan_kernel(const PlanArgs p) {
     }
   }
   if (!sort) return;
+  if (threadIdx.x < 4 && p.entries + threadIdx.x < RT_SORT_MAX) tiles_of[p.entries + threadIdx.x] = -1;  // behind the last
   __syncthreads();
-  for (int e = threadIdx.x; e < p.entries; e += 1024) {  // entries <= 1024: one each
+  const int e = threadIdx.x;  // entries <= 1024: one each
+  if (e < p.entries) {
     const int mine = tiles_of[e];
     int place = 0;
-    for (int i = 0; i < p.entries; ++i) place += tiles_of[i] > mine || (tiles_of[i] == mine && i < e);
+#pragma unroll 4
+    for (int i = 0; i < p.entries; i += 4) {
+      const int4 v = *reinterpret_cast<const int4*>(tiles_of + i);
+      place += (v.x > mine || (v.x == mine && i < e)) + (v.y > mine || (v.y == mine && i + 1 < e)) +
+               (v.z > mine || (v.z == mine && i + 2 < e)) + (v.w > mine || (v.w == mine && i + 3 < e));
+    }
     p.order[place] = e;
   }
 }

@@ -12,7 +12,7 @@ struct HeadNormArgs {
   __nv_bfloat16* out;
   int64_t ldx, ldo, rows;
   int64_t col0[2];
-  int heads0, heads;  // heads of section 0, of all sections
+  int heads0, heads1;
   const __nv_bfloat16* gamma[2];
   float eps;
   int rot;
@@ -20,21 +20,21 @@ struct HeadNormArgs {
   const float* sin;
   const int32_t* positions;
   int64_t table_rows;
-  int groups;  // warps per row
+  int groups0, groups;  // warps per row: of section 0, of both
   int* err;
 };
 
 // A head is LPH = D / 8 lanes of 16 bytes, so a warp holds 32 / LPH heads at once and takes NV such
-// passes of one row, all loads in flight before the first use.  Sums and the norm are fp32 over
-// the head's lanes (a butterfly inside the lane group); the lane's angles are read once per row
-// and serve all its heads.  Interleaved pairs live inside a lane; half-split pairs (i, i + rot/2)
-// are exchanged with the partner lane by shuffles.  One rounding, to bf16, at the store.  x and the
-// output go past the L1 (streaming hints), which keeps the angles that a row's warps share.
+// passes over heads of one section of one row, all loads in flight before the first use.  Sums and the
+// norm are fp32 over the head's lanes (a butterfly inside the lane group).  Gains and angles are the
+// same for all heads of the warp, so their products are formed once: a pair becomes
+//   a' = r (a (g_a c) - b (g_b s)),  b' = r (a (g_a s) + b (g_b c)),  r = rsqrt(mean + eps).
+// Interleaved pairs live inside a lane; half-split pairs (i, i + rot/2) are exchanged with the partner
+// lane by shuffles.  One rounding, to bf16, at the store.  x and the output go past the L1 (streaming
+// hints), which keeps the angles that a row's warps share.
 //
-// NV by a sweep at 15708 x 48 heads of 128 (390 MB): 1 124 us, 2 116, 4 96, 6 91, 8 95 without hints, and
-// 111, 98, 83, 78 (4980 GB/s, 0.77 of the measured copy rate), 83 with them; more registers than
-// four blocks an SM leave cost more than the loads in flight gain.  A single row of 48 heads: 2.4,
-// 2.7, 3.5, 4.0 us.
+// With gains and angles applied head by head the kernel issued 21 instructions a value and stood at
+// 78 us for 15708 rows of 48 heads of 128 (390 MB) with its issue slots 68% busy, DRAM 46%.
 template <int LPH, int NV, bool INTER>
 __global__ void __launch_bounds__(256, 4) head_norm_rope_kernel(const HeadNormArgs a) {
   constexpr int HP = 32 / LPH, D = LPH * 8;
@@ -42,87 +42,97 @@ __global__ void __launch_bounds__(256, 4) head_norm_rope_kernel(const HeadNormAr
   const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int64_t row = w / a.groups;
   if (row >= a.rows) return;  // warp-uniform
-  const int h0 = (int)(w - row * a.groups) * (HP * NV) + lane / LPH;
+  int grp = (int)(w - row * a.groups);
+  const int sec = grp >= a.groups0;  // warp-uniform
+  grp -= sec ? a.groups0 : 0;
+  const int heads = sec ? a.heads1 : a.heads0;
+  const int h0 = grp * (HP * NV) + lane / LPH;
   const int c = lane % LPH;  // this lane's 8 channels: 8c .. 8c + 7
+  const int64_t col = (sec ? a.col0[1] : a.col0[0]) + 8 * c;
+  const __nv_bfloat16* xr = a.x + row * a.ldx + col;
   uint4 raw[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int h = h0 + i * HP;
-    raw[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (h < a.heads) {
-      const int s = h >= a.heads0;
-      raw[i] = __ldcs(reinterpret_cast<const uint4*>(a.x + row * a.ldx + (s ? a.col0[1] : a.col0[0]) +
-                                                     (int64_t)(h - (s ? a.heads0 : 0)) * D + 8 * c));
-    }
+    raw[i] = h < heads ? __ldcs(reinterpret_cast<const uint4*>(xr + h * D)) : make_uint4(0u, 0u, 0u, 0u);
   }
   const int half = a.rot >> 4;  // lanes of one half of the rotated channels (half-split pairs)
-  const bool turned = 8 * c < a.rot;
-  float cs[8], sn[8];
+  const bool turned = a.cos && 8 * c < a.rot;
+  const int partner = (lane + (c < half ? half : -half)) & 31;
+  const __nv_bfloat16* gamma = sec ? a.gamma[1] : a.gamma[0];
+  // own[k], other[k]: factors of the value itself and of its pair's other value
+  float own[8], other[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) own[k] = 1.f, other[k] = 0.f;
+  if (gamma) unpack_bf16x8(__ldg(reinterpret_cast<const uint4*>(gamma) + c), own);
   if (a.cos) {
     const int64_t pos = a.positions ? (int64_t)__ldg(a.positions + row) : row % a.table_rows;
     if (pos < 0 || pos >= a.table_rows) {  // warp-uniform: the row is left as it was
       if (lane == 0) atomicCAS(a.err, 0, kErrBadPosition);
       return;
     }
+    float g2[8];  // the gains of the pairs' other values
+#pragma unroll
+    for (int k = 0; k < 8; ++k) g2[k] = INTER ? own[k ^ 1] : __shfl_sync(0xffffffffu, own[k], partner);
     if (turned) {
       const int p0 = INTER ? 4 * c : 8 * (c < half ? c : c - half);
       const float4* cp = reinterpret_cast<const float4*>(a.cos + pos * (a.rot >> 1) + p0);
       const float4* sp = reinterpret_cast<const float4*>(a.sin + pos * (a.rot >> 1) + p0);
+      float cs[8], sn[8];
 #pragma unroll
       for (int q = 0; q < (INTER ? 1 : 2); ++q) {
         const float4 cv = __ldg(cp + q), sv = __ldg(sp + q);
         cs[4 * q] = cv.x; cs[4 * q + 1] = cv.y; cs[4 * q + 2] = cv.z; cs[4 * q + 3] = cv.w;
         sn[4 * q] = sv.x; sn[4 * q + 1] = sv.y; sn[4 * q + 2] = sv.z; sn[4 * q + 3] = sv.w;
       }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const bool first = INTER ? (k & 1) == 0 : c < half;
+        const int p = INTER ? k >> 1 : k;
+        own[k] *= cs[p];
+        other[k] = first ? -g2[k] * sn[p] : g2[k] * sn[p];
+      }
     }
   }
+  __nv_bfloat16* outr = a.out + row * a.ldo + col;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int h = h0 + i * HP;
-    const int s = h >= a.heads0;
     float x[8];
     unpack_bf16x8(raw[i], x);
-    float q = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) q = fmaf(x[k], x[k], q);
-#pragma unroll
-    for (int o = LPH / 2; o; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
-    const __nv_bfloat16* gamma = s ? a.gamma[1] : a.gamma[0];
+    float r = 1.f;
     if (gamma) {
-      const float rs = rsqrtf(q * (1.f / D) + a.eps);
-      float g[8];
-      unpack_bf16x8(__ldg(reinterpret_cast<const uint4*>(gamma) + c), g);
+      float q = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] *= rs * g[k];
+      for (int k = 0; k < 8; ++k) q = fmaf(x[k], x[k], q);
+#pragma unroll
+      for (int o = LPH / 2; o; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+      r = rsqrtf(q * (1.f / D) + a.eps);
     }
+    float y[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y[k] = x[k] * own[k];
     if (a.cos) {
       if constexpr (INTER) {
         if (turned) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float u = x[2 * k], v = x[2 * k + 1];
-            x[2 * k] = u * cs[k] - v * sn[k];
-            x[2 * k + 1] = u * sn[k] + v * cs[k];
-          }
+          for (int k = 0; k < 8; ++k) y[k] = fmaf(x[k ^ 1], other[k], y[k]);
         }
       } else {
-        const int partner = lane + (c < half ? half : -half);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float o = __shfl_sync(0xffffffffu, x[k], partner & 31);
-          if (turned) x[k] = c < half ? x[k] * cs[k] - o * sn[k] : o * sn[k] + x[k] * cs[k];
+          const float o = __shfl_sync(0xffffffffu, x[k], partner);
+          if (turned) y[k] = fmaf(o, other[k], y[k]);
         }
       }
     }
-    if (h < a.heads) {
+    if (h < heads) {
       uint4 u;
-      u.x = pack_bf16x2(x[0], x[1]);
-      u.y = pack_bf16x2(x[2], x[3]);
-      u.z = pack_bf16x2(x[4], x[5]);
-      u.w = pack_bf16x2(x[6], x[7]);
-      __stcs(reinterpret_cast<uint4*>(a.out + row * a.ldo + (s ? a.col0[1] : a.col0[0]) +
-                                      (int64_t)(h - (s ? a.heads0 : 0)) * D + 8 * c),
-             u);
+      u.x = pack_bf16x2(y[0] * r, y[1] * r);
+      u.y = pack_bf16x2(y[2] * r, y[3] * r);
+      u.z = pack_bf16x2(y[4] * r, y[5] * r);
+      u.w = pack_bf16x2(y[6] * r, y[7] * r);
+      __stcs(reinterpret_cast<uint4*>(outr + h * D), u);
     }
   }
 }
@@ -188,7 +198,7 @@ int head_norm_rope(const wanb200_headnorm_params* p, cudaStream_t st) {
   a.col0[0] = p->col0[0];
   a.col0[1] = p->nsections > 1 ? p->col0[1] : 0;
   a.heads0 = p->heads[0];
-  a.heads = (int)heads;
+  a.heads1 = p->nsections > 1 ? p->heads[1] : 0;
   a.gamma[0] = reinterpret_cast<const __nv_bfloat16*>(p->gamma[0]);
   a.gamma[1] = p->nsections > 1 ? reinterpret_cast<const __nv_bfloat16*>(p->gamma[1]) : nullptr;
   a.eps = p->eps;
@@ -200,10 +210,10 @@ int head_norm_rope(const wanb200_headnorm_params* p, cudaStream_t st) {
   a.err = err;
   const int lph = p->head_dim / 8, hp = 32 / lph;
   // the most passes a warp that still leave every SM its 32 warps; few rows: one each, for latency
-  // (1999 rows of 40 heads of 64: 10.6, 10.3, 10.7 us with 1, 2, 6)
   const int64_t passes = (heads + hp - 1) / hp, fill = (int64_t)num_sms() * 32;
   const int nv = p->rows * ((passes + 5) / 6) >= fill ? 6 : p->rows * ((passes + 1) / 2) >= fill / 2 ? 2 : 1;
-  a.groups = (int)((heads + hp * nv - 1) / (hp * nv));
+  a.groups0 = (a.heads0 + hp * nv - 1) / (hp * nv);
+  a.groups = a.groups0 + (a.heads1 + hp * nv - 1) / (hp * nv);
   const int64_t blocks = (p->rows * a.groups + 7) / 8;
   if (p->rows > INT32_MAX || blocks > INT32_MAX) return set_error(WANB200_EINVAL, "head_norm_rope: too many rows");
   if (lph == 8)

@@ -287,34 +287,60 @@ __device__ __forceinline__ int few_id(const LoraFewArgs& a, int row) {
   return id >= 0 && id < a.adapters ? id : -1;
 }
 
-// h[row][i] = scale * x[row] . down[id][i] in fp32, one warp per (row, i).
+// h[row][i] = scale * x[row] . down[id][i] in fp32.  A block has one row and LF_RANKS values i; its 256
+// threads share K, so that (up to K = 4096) every load is in flight at once: the GEMM behind waits for
+// this latency.
+constexpr int LF_RANKS = 4;
+
 __global__ void __launch_bounds__(256) lora_few_down_kernel(const LoraFewArgs a) {
+  __shared__ float part[8][LF_RANKS];
   pdl_launch();
-  const int w = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int row = w / a.rank, i = w - row * a.rank;
-  if (row >= a.M) return;  // warp-uniform
+  const int per = a.rank / LF_RANKS, row = blockIdx.x / per, i0 = (blockIdx.x - row * per) * LF_RANKS;
   const int id = few_id(a, row);
   if (id < 0) {
-    if (lane == 0 && i == 0 && __ldg(a.ids + row) >= a.adapters) atomicCAS(a.err, 0, kErrBadAdapter);
+    if (threadIdx.x == 0 && i0 == 0 && __ldg(a.ids + row) >= a.adapters) atomicCAS(a.err, 0, kErrBadAdapter);
     return;
   }
-  const uint4* xp = reinterpret_cast<const uint4*>(a.x + row * a.ldx) + lane;
-  const uint4* dp = reinterpret_cast<const uint4*>(a.down + ((int64_t)id * a.rank + i) * a.K) + lane;
-  float v = 0.f;
+  const uint4* xp = reinterpret_cast<const uint4*>(a.x + row * a.ldx);
+  const uint4* dp = reinterpret_cast<const uint4*>(a.down + ((int64_t)id * a.rank + i0) * a.K);
   const int n = a.K / 8;
-#pragma unroll 8
-  for (int k = 0; k < n; k += 32) {
-    if (k + lane < n) {
-      float f[8], g[8];
-      unpack_bf16x8(__ldg(xp + k), f);
-      unpack_bf16x8(__ldg(dp + k), g);
+  float v[LF_RANKS] = {};
+  for (int k0 = threadIdx.x; k0 < n; k0 += 512) {
+    const bool second = k0 + 256 < n;
+    uint4 x[2], d[2][LF_RANKS];
+    x[0] = __ldg(xp + k0);
+    x[1] = second ? __ldg(xp + k0 + 256) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v = fmaf(f[e], g[e], v);
+    for (int r = 0; r < LF_RANKS; ++r) {
+      d[0][r] = __ldg(dp + r * n + k0);
+      d[1][r] = second ? __ldg(dp + r * n + k0 + 256) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      float f[8];
+      unpack_bf16x8(x[y], f);
+#pragma unroll
+      for (int r = 0; r < LF_RANKS; ++r) {
+        float g[8];
+        unpack_bf16x8(d[y][r], g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[r] = fmaf(f[e], g[e], v[r]);
+      }
     }
   }
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (lane == 0) a.h[row * a.rank + i] = v * (a.scales ? __ldg(a.scales + id) : 1.f);
+  for (int r = 0; r < LF_RANKS; ++r) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v[r] += __shfl_xor_sync(0xffffffffu, v[r], o);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5][r] = v[r];
+  }
+  __syncthreads();
+  if (threadIdx.x < LF_RANKS) {
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) t += part[w][threadIdx.x];
+    a.h[row * a.rank + i0 + threadIdx.x] = t * (a.scales ? __ldg(a.scales + id) : 1.f);
+  }
 }
 
 // 8 columns of the output a block (16 or 32 were slower up to N = 14336: fewer blocks to hide a block's
@@ -460,7 +486,7 @@ static int lora_few(const wanb200_lora_params* p, float* h, int* err, cudaStream
   a.rank = p->rank;
   a.h = h;
   a.err = err;
-  lora_few_down_kernel<<<(unsigned)((a.M * a.rank + 7) / 8), 256, 0, st>>>(a);
+  lora_few_down_kernel<<<(unsigned)(a.M * (a.rank / LF_RANKS)), 256, 0, st>>>(a);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.N / 8));
   cfg.blockDim = dim3(LF_WARPS * 32);
