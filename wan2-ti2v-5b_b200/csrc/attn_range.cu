@@ -524,24 +524,28 @@ __global__ void __launch_bounds__(1024) range_plan_kernel(const PlanArgs p) {
   const int warps = sort ? 32 : gridDim.x * 32;
   for (int e = (sort ? 0 : blockIdx.x * 32) + warp; e < p.entries; e += warps) {
     const int b = e / p.nqp, tok0 = e % p.nqp * 2 * p.tpt;
+    // a tile's rows four a lane, all loads first; lanes behind the last row repeat it
+    int lo[2][4], hi[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = min(p.tpt, p.a.q_len - (tok0 + t * p.tpt));
+        lo[t][q] = hi[t][q] = 0;
+        if (n > 0) row_range(p.a, b, tok0 + t * p.tpt + min(lane + 32 * q, n - 1), lo[t][q], hi[t][q]);
+      }
     int any_lo[2], any_hi[2], all_lo[2], all_hi[2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) any_lo[t] = INT32_MAX, any_hi[t] = 0, all_lo[t] = 0, all_hi[t] = INT32_MAX;
-#pragma unroll 4
-    for (int i = lane; i < 2 * p.tpt; i += 32) {
-      if (tok0 + i >= p.a.q_len) break;
-      const int t = i >= p.tpt;
-      int lo, hi;
-      row_range(p.a, b, tok0 + i, lo, hi);
-      const bool some = lo < hi;
+    for (int t = 0; t < 2; ++t) {
+      any_lo[t] = INT32_MAX, any_hi[t] = 0, all_lo[t] = 0, all_hi[t] = INT32_MAX;
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-        if (x == t) {
-          any_lo[x] = some ? min(any_lo[x], lo) : any_lo[x];
-          any_hi[x] = some ? max(any_hi[x], hi) : any_hi[x];
-          all_lo[x] = max(all_lo[x], lo);
-          all_hi[x] = min(all_hi[x], hi);
-        }
+      for (int q = 0; q < 4; ++q) {
+        const bool some = lo[t][q] < hi[t][q];
+        any_lo[t] = some ? min(any_lo[t], lo[t][q]) : any_lo[t];
+        any_hi[t] = some ? max(any_hi[t], hi[t][q]) : any_hi[t];
+        all_lo[t] = max(all_lo[t], lo[t][q]);
+        all_hi[t] = min(all_hi[t], hi[t][q]);
+      }
     }
     RangePair r;
     int tiles = 0;
