@@ -34,7 +34,8 @@ struct HeadNormArgs {
 // hints), which keeps the angles that a row's warps share.
 //
 // With gains and angles applied head by head the kernel issued 21 instructions a value and stood at
-// 78 us for 15708 rows of 48 heads of 128 (390 MB) with its issue slots 68% busy, DRAM 46%.
+// 78 us for 15708 rows of 48 heads of 128 (390 MB) with its issue slots 68% busy; with the products
+// formed once it is 70 us, 5.56 TB/s, 0.86 of the copy rate, issue 59%.
 template <int LPH, int NV, bool INTER>
 __global__ void __launch_bounds__(256, 4) head_norm_rope_kernel(const HeadNormArgs a) {
   constexpr int HP = 32 / LPH, D = LPH * 8;
@@ -166,13 +167,11 @@ int head_norm_rope(const wanb200_headnorm_params* p, cudaStream_t st) {
     return set_error(WANB200_EINVAL, "head_norm_rope: x / out need 16-byte aligned pointers and row strides % 8 == 0");
   if (p->x == p->out && p->ldx != p->ldo)
     return set_error(WANB200_EINVAL, "head_norm_rope: in place needs equal row strides");
-  int64_t heads = 0;
   for (int s = 0; s < p->nsections; ++s) {
     if (p->heads[s] <= 0 || p->heads[s] > 65535 || p->col0[s] < 0 || p->col0[s] % 8 ||
         p->col0[s] + (int64_t)p->heads[s] * p->head_dim > std::min(p->ldx, p->ldo) || !aligned16(p->gamma[s]))
       return set_error(WANB200_EINVAL, "head_norm_rope: bad section (col0 % 8 == 0, heads * head_dim inside the row, "
                                        "16-byte aligned gamma)");
-    heads += p->heads[s];
   }
   if (p->nsections == 2) {  // a warp may hold heads of both, so they must not share channels
     const int64_t e0 = p->col0[0] + (int64_t)p->heads[0] * p->head_dim, e1 = p->col0[1] + (int64_t)p->heads[1] * p->head_dim;
@@ -209,9 +208,14 @@ int head_norm_rope(const wanb200_headnorm_params* p, cudaStream_t st) {
   a.table_rows = p->cos ? p->table_rows : 1;
   a.err = err;
   const int lph = p->head_dim / 8, hp = 32 / lph;
-  // the most passes a warp that still leave every SM its 32 warps; few rows: one each, for latency
-  const int64_t passes = (heads + hp - 1) / hp, fill = (int64_t)num_sms() * 32;
-  const int nv = p->rows * ((passes + 5) / 6) >= fill ? 6 : p->rows * ((passes + 1) / 2) >= fill / 2 ? 2 : 1;
+  // The passes of a warp: six where that leaves every SM its 32 warps and at most half as many idle
+  // passes again (a section's heads fill whole warps), two where that leaves 16, else one, for latency.
+  // Measured (us, 1 / 2 / 6 passes): 1 row of 48 heads of 128 2.2 / 2.3 / 3.2; 640 rows 6.0 / 4.8 / 5.0;
+  // 15708 rows 109 / 79 / 69, of 32 + 8 heads of 64 (8 + 2 passes in 18 places) 47 / 35 / 41, of 16 + 2
+  // heads of 256 (18 in 24) 83 / 68 / 62.
+  const int64_t p0 = (a.heads0 + hp - 1) / hp, p1 = (a.heads1 + hp - 1) / hp, fill = (int64_t)num_sms() * 32;
+  const int64_t warps6 = (p0 + 5) / 6 + (p1 + 5) / 6, warps2 = (p0 + 1) / 2 + (p1 + 1) / 2;
+  const int nv = p->rows * warps6 >= fill && 4 * warps6 <= p0 + p1 ? 6 : p->rows * warps2 >= fill / 2 ? 2 : 1;
   a.groups0 = (a.heads0 + hp * nv - 1) / (hp * nv);
   a.groups = a.groups0 + (a.heads1 + hp * nv - 1) / (hp * nv);
   const int64_t blocks = (p->rows * a.groups + 7) / 8;
