@@ -104,7 +104,7 @@ __device__ __forceinline__ float score_log2(const RangeArgs& a, float s, int h, 
 constexpr int RD_WARPS = 4, RD_KEYS = 16, RD_TILE = RD_WARPS * RD_KEYS;
 constexpr int RD_THREADS = (RD_WARPS + 1) * 32;
 constexpr int RD_SHARE = 2;   // key tiles of a block at least
-constexpr int RD_BLOCKS = 3;  // blocks an SM holds (by shared memory; two with 9 to 16 rows, by registers)
+constexpr int RD_BLOCKS = 3, RD_BLOCKS_TWO = 2;  // blocks an SM holds: by shared memory; with 9 to 16 rows by registers
 
 template <int D>
 struct RangeDecodeCfg {
@@ -126,7 +126,7 @@ __device__ __forceinline__ int decode_key_tiles(const RangeArgs& a, int b) {
 }
 
 template <int D, bool TWO, bool CAP, int BIAS>  // TWO: 9 to 16 rows, two column tiles
-__global__ void __launch_bounds__(RD_THREADS, TWO ? 2 : RD_BLOCKS)
+__global__ void __launch_bounds__(RD_THREADS, TWO ? RD_BLOCKS_TWO : RD_BLOCKS)
     range_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                         const __grid_constant__ RangeArgs a, const __grid_constant__ RangeParts out, const int slots, int* err) {
   using C = RangeDecodeCfg<D>;
@@ -1261,7 +1261,10 @@ __global__ void __launch_bounds__(RC_WARPS * 32) range_combine_kernel(const Rang
 }
 
 // ------------------------------------------------------------------ host launcher
-// Packed rows up to which the few-rows kernel runs (the 16 rows of its MMA).
+// Packed rows up to which the few-rows kernel runs: two column tiles of 8 rows of its MMA.  Measured at
+// 16 rows, few-rows kernel / tiles (us; batch x 8 key heads of 128, all keys seen): 1 x 1024 keys
+// 11.7 / 13.4, 1 x 16384 26 / 29, 16 x 4096 55 / 64, 16 x 16384 165 / 217, and with lengths between a
+// quarter of that and all of it 124 / 206.  Only many short caches go the other way (16 x 256: 18 / 14).
 constexpr int RD_ROWS = 16;
 
 struct RangeLayout {
@@ -1274,7 +1277,8 @@ static int64_t range_up(int64_t x) { return (x + 255) / 256 * 256; }
 // The few-rows kernel's blocks: as many as the SMs hold at once, less half a block for each (key head,
 // batch element), whose last share is half full on average.  More elements than blocks: one block each.
 static int range_decode_slots(const wanb200_range_attn_params* p) {
-  const int64_t units = p->batch * p->kv_heads, slots = (int64_t)num_sms() * RD_BLOCKS;
+  const bool two = p->q_len * (p->heads / p->kv_heads) > 8;
+  const int64_t units = p->batch * p->kv_heads, slots = (int64_t)num_sms() * (two ? RD_BLOCKS_TWO : RD_BLOCKS);
   return units >= slots || p->kv_len <= RD_TILE * RD_SHARE ? 0 : (int)std::max(slots - units / 2, slots / 4);
 }
 

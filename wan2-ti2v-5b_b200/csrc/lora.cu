@@ -258,6 +258,8 @@ __global__ void __launch_bounds__(LD_THREADS, 1)
 }
 
 // ================================================================== up to 16 rows: W is read once
+// Measured, these kernels / the tiles (us; K = N = 4096, 8 adapters of rank 16): 1 row 9.5 / 20.4, 4 rows
+// 9.8 / 20.7, 16 rows 13.4 / 22.1; K = 8192, N = 2048, 16 rows 18.9 / 19.9, where the gain ends.
 constexpr int LF_ROWS = 16, LF_WARPS = 8;
 
 struct LoraFewArgs {
@@ -548,6 +550,9 @@ int64_t lora_workspace_bytes(int64_t M, int adapters, int rank, int out_f32) {
 // The two kernels run side by side where the SMs beside the down-projection's suffice for the GEMM
 // (it waits for h only at the end of its first K loop), else one after the other.  Few tiles
 // share K over a cluster; its join reads (ks - 1) / ks of a tile from other SMs.
+// Measured (us): 509 x 2048 x 4096, 16 adapters of rank 16: 25 as chosen, 46 without a split of the
+// down-projection, 34 without one of the GEMM; 128 x 4096 x 4096, 4 of rank 64: 23, 45 and 35; 1964 x
+// 8192 x 2048, 3 of rank 32, has tiles enough: 67 whatever is allowed.
 struct LoraLaunch {
   int down_ksize, bn, ksplit, grid;
 };
