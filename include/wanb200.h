@@ -277,7 +277,9 @@ int wanb200_head_norm_rope(const wanb200_headnorm_params* p, void* stream);
  *   softcap   cap(s) = softcap * tanh(s / softcap), 1e-6 .. 1e6; 0 = none
  *   slopes    bias = -slopes[h] * |j - pos|, [heads] fp32
  *   dist_bias bias = dist_bias[h][clamp(j - pos, -reach, reach) + reach], [heads, 2 reach + 1] fp32
- *             (a relative-position table, reach <= 8192; at most one of the two)
+ *             (a relative-position table, reach <= 8192; at most one of the two).  The type's lowest
+ *             value hides a key beside others; keys that all have it weigh alike, and keys that all
+ *             have -inf give NaN: keys that a row shall not see belong outside its range
  *   pos       [q_len] int32 like lo: the row's place among the keys (NULL = i; clipped to +-2^30)
  * What keys outside a row's range hold (NaN, infinities) does not reach the row.  The masked,
  * grouped, single-token companion of wanb200_attn_fwd.

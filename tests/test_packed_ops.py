@@ -477,6 +477,34 @@ def test_range_attention_hidden_keys_do_not_reach_a_row(Lq, Lk, H, Hkv, word):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("low", [torch.finfo(torch.float32).min, -math.inf])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("Lq,Lk,H,Hkv", [(1, 700, 4, 2), (3, 300, 4, 1), (200, 300, 4, 2)])
+def test_range_attention_table_of_lowest_values(Lq, Lk, H, Hkv, cap, low, word):
+    """A table that is 0 near the row and the lowest value, or -inf, from a distance of R on hides the far keys
+    from rows that see a near one.  Where every key has the lowest value all weigh alike (in fp32 no
+    score changes it); where every key has -inf the weights are 0 / 0."""
+    D, R = 64, 20
+    q, k, v = randn(1, Lq, H, D, seed=30), randn(1, Lk, Hkv, D, seed=31), randn(1, Lk, Hkv, D, seed=32)
+    table = torch.zeros(H, 2 * R + 1, device=DEV)
+    table[:, 0] = table[:, -1] = low
+    lo, hi = ints([3] * Lq)[0].contiguous(), ints([Lk - 2] * Lq)[0].contiguous()
+    for first in (5, Lk + 100):  # near keys for every row; none
+        pos = torch.arange(Lq, dtype=torch.int32, device=DEV) + first
+        got = ops.range_attention(q, k, v, lo, hi, pos=pos, softcap=cap, dist_bias=table)
+        if first == 5:
+            ref, tol = attn_ref(q, k, v, torch.maximum(lo, pos - R + 1), torch.minimum(hi, pos + R), cap=cap)
+            within(got, ref, tol)
+        elif low == -math.inf:
+            assert bool(got.isnan().all())
+        else:  # weights of exactly 1, fp32 sums of up to 700 values, one rounding to bf16
+            seen = v[:, 3:Lk - 2].double()
+            ref = seen.mean(1, keepdim=True).repeat_interleave(H // Hkv, 2).expand(1, Lq, H, D)
+            mag = seen.abs().mean(1, keepdim=True).repeat_interleave(H // Hkv, 2).expand(1, Lq, H, D)
+            within(got, ref, HALF * 1.01 * ref.abs() + 2.0 ** -14 * mag)
+
+
+@pytest.mark.gpu
 def test_range_attention_extreme_scores(word):
     """Scores far apart, all equal, and of the largest size: the running maximum keeps the sums finite."""
     D, Lk = 64, 300

@@ -77,6 +77,13 @@ __device__ __forceinline__ float min30(float x) {
 
 __device__ __forceinline__ bool nonfinite_bf16(__nv_bfloat16 x) { return !isfinite(__bfloat162float(x)); }
 
+// A table's bias, such that a finite one stays finite in log2 units: times log2(e) the type's lowest value
+// would become -inf, and a row whose keys all have it 0 / 0 instead of equal weights.  Infinities and NaN
+// stay as they are.  2.3e38 log2(e) = 3.32e38 < 2^128.
+__device__ __forceinline__ float table_bias(float b) {
+  return fabsf(b) < INFINITY ? fminf(fmaxf(b, -2.3e38f), 2.3e38f) : b;
+}
+
 // 2^t-units score of one (row, key) from its raw product, for the forms that take keys one by one.
 template <bool CAP, int BIAS>
 __device__ __forceinline__ float score_log2(const RangeArgs& a, float s, int h, int dist) {
@@ -84,7 +91,7 @@ __device__ __forceinline__ float score_log2(const RangeArgs& a, float s, int h, 
   if constexpr (CAP) t = a.cap2 - 2.f * a.cap2 * rcp_approx(1.f + ex2_approx(t));
   if constexpr (BIAS == kBiasSlopes) t = fmaf(-RA_LOG2E * __ldg(a.slopes + h), fabsf((float)dist), t);
   if constexpr (BIAS == kBiasTable)
-    t = fmaf(RA_LOG2E, __ldg(a.table + (int64_t)h * (2 * a.reach + 1) + min(max(dist, -a.reach), a.reach) + a.reach), t);
+    t = fmaf(RA_LOG2E, table_bias(__ldg(a.table + (int64_t)h * (2 * a.reach + 1) + min(max(dist, -a.reach), a.reach) + a.reach)), t);
   return t;
 }
 
@@ -516,7 +523,7 @@ __global__ void __launch_bounds__(1024) range_plan_kernel(const PlanArgs p) {
     const int row = range_padded(p.a.reach), n = p.a.kv_heads * p.a.group * row;
     for (int i = blockIdx.x * 1024 + threadIdx.x; i < n; i += gridDim.x * 1024) {
       const int h = i / row, d = min(max(i - h * row - RT_N - p.a.reach, -p.a.reach), p.a.reach);
-      p.padded[i] = RA_LOG2E * __ldg(p.a.table + (int64_t)h * (2 * p.a.reach + 1) + d + p.a.reach);
+      p.padded[i] = RA_LOG2E * table_bias(__ldg(p.a.table + (int64_t)h * (2 * p.a.reach + 1) + d + p.a.reach));
     }
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.counter = 0;
