@@ -69,6 +69,12 @@ def test_cache_and_padded_ranges():
         ranges.document_ranges([-1], "cpu")
 
 
+@pytest.mark.parametrize("q_len,window", [(-1, 0), (1, -1)])
+def test_cache_ranges_refuses_negative_sizes(q_len, window):
+    with pytest.raises(ValueError):
+        ranges.cache_ranges(torch.tensor([3], dtype=torch.int32), q_len, window=window)
+
+
 # ---------------------------------------------------------------------------- refusals (CPU)
 def _refused(fn, p, word):
     rc = fn(ctypes.byref(p), None)

@@ -55,6 +55,8 @@ def cache_ranges(kv_lens, q_len, *, window=0):
     """(lo, hi, pos), each [B, q_len], for queries that are the last q_len tokens of caches holding
     kv_lens[b] keys (int32 tensor [B] on the device), in causal order; window w > 0: the last w keys
     only.  All on the tensor's device, without waiting for it."""
+    if q_len < 0 or window < 0:
+        raise ValueError("cache_ranges: q_len and window must be >= 0")
     pos = kv_lens.to(torch.int32)[:, None] - q_len + torch.arange(q_len, dtype=torch.int32, device=kv_lens.device)[None]
     hi = pos + 1
     lo = (hi - window).clamp_min(0) if window else torch.zeros_like(hi)
