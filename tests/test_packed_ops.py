@@ -247,6 +247,21 @@ def test_head_norm_rope(M, hq, hk, d, rot, inter, word):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M,hq,hk,d,rot,inter", [
+    (1300, 24, 24, 128, 128, True), (1701, 21, 11, 128, 96, False), (2400, 23, 21, 64, 64, True), (2401, 6, 5, 256, 80, False),
+    (2500, 32, 8, 64, 48, False), (700, 24, 24, 128, 128, True)])
+def test_head_norm_rope_many_rows(M, hq, hk, d, rot, inter, word):
+    """Rows enough for six passes a warp, with heads that fill them, leave some idle, or too many idle."""
+    x, gq, gk = randn(M, (hq + hk) * d, seed=M), randn(d, seed=1), randn(d, seed=2)
+    ang = torch.rand(M, rot // 2, device=DEV) * 6
+    secs = [(0, hq, gq), (hq * d, hk, gk)]
+    ref, tol = head_norm_ref(x, secs, d, rot, ang.cos(), ang.sin(), torch.arange(M, device=DEV), inter)
+    out = torch.empty_like(x)
+    ops.head_norm_rope(x, secs, d, out=out, cos=ang.cos(), sin=ang.sin(), interleaved=inter)
+    within(out, ref, tol)
+
+
+@pytest.mark.gpu
 def test_head_norm_rope_forms(word):
     M, d = 40, 64
     x = randn(M, 6 * d, seed=3)
@@ -436,6 +451,19 @@ def test_range_attention_long_cache_of_unequal_lengths(Lq, word):
     lo, hi, pos = ranges.cache_ranges(lens, Lq)
     check_attn(q, k, v, lo, hi, pos=pos, slopes=torch.rand(H, device=DEV) * 0.1)
     lo, hi, pos = ranges.cache_ranges(lens, Lq, window=100)
+    check_attn(q, k, v, lo, hi, pos=pos)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,Lq,H,Hkv,D", [(5, 3, 16, 4, 128), (5, 4, 16, 4, 64), (3, 16, 3, 3, 128), (2, 9, 2, 2, 64),
+                                          (40, 5, 16, 8, 64), (60, 2, 64, 8, 64)])
+def test_range_attention_nine_to_sixteen_rows_of_unequal_caches(B, Lq, H, Hkv, D, word):
+    """Two column tiles a block, with one and with several blocks a cache."""
+    Lk = 900 if B > 10 else 4000
+    q, k, v = randn(B, Lq, H, D, seed=40), randn(B, Lk, Hkv, D, seed=41), randn(B, Lk, Hkv, D, seed=42)
+    lens = torch.randint(0, Lk + 1, (B,), dtype=torch.int32, generator=torch.Generator().manual_seed(B))
+    lens[0], lens[1] = Lk, 0
+    lo, hi, pos = ranges.cache_ranges(lens.to(DEV), Lq)
     check_attn(q, k, v, lo, hi, pos=pos)
 
 
@@ -786,3 +814,29 @@ def test_two_streams_at_once(word):
     torch.cuda.synchronize()
     for i in (0, 1):
         assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+@pytest.mark.gpu
+def test_two_captured_graphs_at_once(word):
+    """Two captured graphs of the same layer, replayed at the same time, have workspaces of their own."""
+    P = make_layer(512, 8, 2, 128, 4, 16)
+    sets = []
+    for T, seed in ((700, 104), (3, 106)):  # tiles; the few-rows kernels
+        lo, hi = ranges.document_ranges([T], DEV, block=1)
+        pos = torch.arange(T, device=DEV).to(torch.int32)
+        ids = (torch.arange(T, device=DEV) % 5 - 1).to(torch.int32)
+        for s in (seed, seed + 10):
+            args = (randn(T, 512, seed=s), randn(T, 512, seed=s + 1).float(), P, lo, hi, pos, ids)
+            want = packed_layer(*args).clone()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                out = packed_layer(*args)
+            sets.append((g, out, want, torch.cuda.Stream(), args))  # the graph reads args
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for g, _, _, st, _ in sets:
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for _, out, want, _, _ in sets:
+        assert torch.equal(out, want)
