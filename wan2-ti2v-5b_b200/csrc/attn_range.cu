@@ -48,7 +48,7 @@ struct RangeArgs {
 struct RangeParts {
   float* o;
   float2* ml;
-  int4* first;   // written by the few-rows kernel; null: (x, splits, groups) for every x
+  int4* first;   // written by the few-rows kernel; the tiles' groups all have (x, splits, groups)
   int slot_rows, groups, splits;
 };
 
@@ -468,6 +468,7 @@ constexpr int RT_BLK = 16384;  // 128 rows of one 128-byte swizzle row
 constexpr int RT_P_SPLIT = 96;
 constexpr int RT_QUEUE = 2;
 constexpr int RT_SORT_MAX = 1024;  // pairs that the plan kernel sorts
+constexpr int RT_SPLITS = 32;  // of a tile pair's keys at most: a lane each in range_join_kernel
 constexpr int RT_REACH_MAX = 8192;  // of a bias table (it is copied with padded ends at every call)
 
 template <int D>
@@ -1222,7 +1223,8 @@ __global__ void __maxnreg__(160)
   if (warp == 9) tmem_dealloc(tmem_base, 512);
 }
 
-// Merge of the key splits: one block per packed row, its warps taking the splits in turn.
+// Merge of the few-rows kernel's splits: one block per packed row, its warps taking the splits in turn
+// (few rows with up to hundreds of splits).
 constexpr int RC_WARPS = 4;
 
 template <int D>
@@ -1233,8 +1235,8 @@ __global__ void __launch_bounds__(RC_WARPS * 32) range_combine_kernel(const Rang
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int x = (int)(blockIdx.x / in.slot_rows), r = (int)(blockIdx.x - (int64_t)x * in.slot_rows);
   const int hg = r % a.group, tok = r / a.group, kh = x % a.kv_heads, b = x / a.kv_heads;
-  const int4 f4 = in.first ? in.first[x] : make_int4(x, in.splits, in.groups, 0);
-  if (in.first && f4.y == 1) return;  // its one block wrote the output
+  const int4 f4 = in.first[x];
+  if (f4.y == 1) return;  // its one block wrote the output
   int lo, hi;
   row_range(a, b, tok, lo, hi);
   const int64_t row0 = (int64_t)f4.x * in.slot_rows + r, next = (int64_t)f4.z * in.slot_rows;
@@ -1265,6 +1267,54 @@ __global__ void __launch_bounds__(RC_WARPS * 32) range_combine_kernel(const Rang
     a.o[b * a.o_batch + (int64_t)tok * a.o_tok + (int64_t)(kh * a.group + hg) * D + threadIdx.x] =
         __float2bfloat16(lo < hi ? oo / ll : 0.f);
   }
+}
+
+// Merge of the tiles' splits (at most RT_SPLITS): many rows with few splits, so one warp a row, eight
+// rows a block, the loads of four splits in flight.  With one block a row 15,000 rows of 2 splits took
+// 12 us longer (the whole call 36 against 24).
+constexpr int RJ_WARPS = 8;
+
+template <int D>
+__global__ void __launch_bounds__(RJ_WARPS * 32) range_join_kernel(const RangeArgs a, const RangeParts in) {
+  constexpr int E = D / 32;
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = (int64_t)in.groups * in.slot_rows, row = (int64_t)blockIdx.x * RJ_WARPS + (threadIdx.x >> 5);
+  if (row >= rows) return;  // warp-uniform
+  const int x = (int)(row / in.slot_rows), r = (int)(row - (int64_t)x * in.slot_rows);
+  const int hg = r % a.group, tok = r / a.group, kh = x % a.kv_heads, b = x / a.kv_heads;
+  int lo, hi;
+  row_range(a, b, tok, lo, hi);
+  const float2 ml = lane < in.splits ? in.ml[row + lane * rows] : make_float2(-INFINITY, -1.f);
+  const bool some = ml.y != -1.f;  // this lane's split saw a key tile of the row
+  float m = ml.x;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float f = !some ? 0.f : ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - m);
+  float l = some ? f * ml.y : 0.f, o[E];
+#pragma unroll
+  for (int w = 16; w; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+  const uint32_t has = __ballot_sync(0xffffffffu, some);
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < in.splits; ++s) {
+    const float fs = __shfl_sync(0xffffffffu, f, s);
+    const float* src = in.o + (row + s * rows) * D + lane * E;
+    if ((has >> s) & 1u) {  // else nothing was written there
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(src + e);
+        o[e] = fmaf(fs, v.x, o[e]);
+        o[e + 1] = fmaf(fs, v.y, o[e + 1]);
+      }
+    }
+  }
+  const float inv = lo < hi ? 1.f / l : 0.f;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(a.o + b * a.o_batch + (int64_t)tok * a.o_tok + (int64_t)(kh * a.group + hg) * D) +
+                  lane * (E / 2);
+#pragma unroll
+  for (int e = 0; e < E; e += 2) dst[e / 2] = lo < hi ? pack_bf16x2(o[e] * inv, o[e + 1] * inv) : 0u;
 }
 
 // ------------------------------------------------------------------ host launcher
@@ -1319,9 +1369,12 @@ static RangeLayout range_layout(const wanb200_range_attn_params* p) {
   if (entries > INT32_MAX / 64 || streams > INT32_MAX / 64) return l;
   l.entries = (int)entries;
   l.streams = (int)streams;
-  // split the keys when the units leave SMs idle: at least two key tiles a split
+  // Split the keys when the units leave SMs idle: at least two key tiles a split.  Measured, causal order (us,
+  // 1 split / as chosen): 24 units of up to 47 tiles 93 / 36, 40 of 20 45 / 28, 40 rows against 4 caches of up to
+  // 8000 keys 108 / 40; with 5 tiles 21 / 22.5.  More splits than that, in two rounds of units: 96 units 28.6 as
+  // chosen, 40 with 2 splits; 128 units of up to 32 tiles 70 and 67.
   const int64_t units = entries * streams, tiles = (p->kv_len + RT_N - 1) / RT_N;
-  l.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(num_sms() / units, tiles / 2), 32));
+  l.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(num_sms() / units, tiles / 2), RT_SPLITS));
   l.units = units * l.splits;
   l.order_off = range_up(entries * (int64_t)sizeof(RangePair));
   l.counter_off = l.order_off + range_up(entries * 4);
@@ -1457,7 +1510,14 @@ static int launch_range_tiles(const CUtensorMap& tq, const CUtensorMap& tk, cons
   cfg.numAttrs = 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, range_attn_kernel<D, CAP, BIAS>, tq, tk, tv, g);
   if (e != cudaSuccess) return set_cuda_error("range_attn_kernel launch", e);
-  return g.splits > 1 ? launch_range_combine<D>(g.a, g.parts, st) : WANB200_OK;
+  if (g.splits == 1) return WANB200_OK;
+  const int64_t join_rows = (int64_t)g.parts.groups * g.parts.slot_rows;
+  cfg.gridDim = dim3((unsigned)((join_rows + RJ_WARPS - 1) / RJ_WARPS));
+  cfg.blockDim = dim3(RJ_WARPS * 32);
+  cfg.dynamicSmemBytes = 0;
+  e = cudaLaunchKernelEx(&cfg, range_join_kernel<D>, g.a, g.parts);
+  if (e != cudaSuccess) return set_cuda_error("range_join_kernel launch", e);
+  return WANB200_OK;
 }
 
 // The few-rows kernel (d) or the tiles (g with the maps of q, k and v).
