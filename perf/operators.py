@@ -234,19 +234,13 @@ def _lora_plain(s):
 
 
 # ---------------------------------------------------------------------------- the library's calls
-_ops = None
-
-
 def _library():
-    """wanb200.ops, imported once; the package lies one folder below the repository's root."""
-    global _ops
-    if _ops is None:
-        folder = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "wan2-ti2v-5b_b200")
-        if folder not in sys.path:
-            sys.path.insert(0, folder)
-        from wanb200 import ops
-        _ops = ops
-    return _ops
+    """wanb200.ops; the package lies one folder below the repository's root."""
+    folder = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "wan2-ti2v-5b_b200")
+    if folder not in sys.path:
+        sys.path.insert(0, folder)
+    from wanb200 import ops
+    return ops
 
 
 def _norm_own(s):
