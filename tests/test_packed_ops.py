@@ -695,6 +695,41 @@ def test_lora_linear_broken_adapters_stay_with_their_rows(M, r, word):
     within(torch.where(wrong, torch.zeros_like(got), got), torch.where(wrong, torch.zeros_like(ref), ref), tol.nan_to_num(1.0))
 
 
+def _broken_neighbours(K, N, n, r, M, order, seed=200):
+    """Adapters 0, 2, 4, ... in use (or one of them alone), NaN and infinities in the weights of the others."""
+    x, w, b, down, up, ids, scales = lora_case(M, K, N, n, r, seed)
+    ids = ids.abs() // 2 * 2
+    if order == "sorted":
+        ids = ids.sort().values
+    elif order != "mixed":
+        ids = torch.full_like(ids, order)
+    up[:, 1::2] = math.nan
+    up[3, 1::2, 0] = math.inf
+    up[4, 1::2, -1] = -math.inf
+    down[1::2] = math.inf
+    down[1::2, 0] = math.nan
+    return x, w, b, down, up, ids, scales
+
+
+def _spared(x, w, b, down, up, ids, scales, epi, f32=False, **rf):
+    """(y, bound) of lora_ref, the broken adapters, which no row uses, replaced by zeros."""
+    clean = [torch.where(t.isfinite(), t, torch.zeros_like(t)) for t in (down, up)]
+    return lora_ref(x, w, b, *clean, ids, scales, epi, f32=f32, **rf)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", [0, 2, 4, "sorted", "mixed"])
+@pytest.mark.parametrize("r", [8, 16, 24, 40])
+@pytest.mark.parametrize("M,K", [(9, 128), (17, 128), (260, 128), (700, 128), (260, 2048), (700, 2048)])
+def test_lora_linear_spares_rows_beside_broken_adapters(M, K, r, order, word):
+    """Ranks that are no multiple of 16 put columns of two adapters into one K step, also where all rows of a
+    tile use one adapter; K = 2048 with few tiles shares K over a cluster."""
+    case = _broken_neighbours(K, 96, 6, r, M, order)
+    within(ops.lora_linear(*case[:6], scales=case[6]), *_spared(*case, L.EPI_BIAS))
+    out = torch.empty(M, 96, device=DEV)
+    within(ops.lora_linear(*case[:6], scales=case[6], out=out), *_spared(*case, L.EPI_BIAS, f32=True))
+
+
 @pytest.mark.gpu
 def test_lora_linear_bad_id_counts_as_none():
     L.device_error(reset=True)
