@@ -486,6 +486,64 @@ def test_range_attention_cap_and_bias(B, Lq, Lk, H, Hkv, cap, bias, D, word):
         check_attn(q, k, v, lo, hi, slopes=slopes)  # positions default to the row
 
 
+def capped_ref(q, k, v, lo, hi, cap):
+    """fp64 (o, bound) of capped scores whose error goes with the score itself, whatever the cap: the dot
+    product to 2^-20 of its magnitude (as attn_ref), the cap to 2^-16 of the capped score (its polynomial is
+    9e-6 from tanh, the general form below that where it is used, above 0.6 of the cap)."""
+    B, Lq, H, D = q.shape
+    g, j = H // k.shape[2], torch.arange(k.shape[1], device=q.device)
+    kd, vd = (t.double().repeat_interleave(g, 2) for t in (k, v))
+    s = torch.einsum("bihd,bjhd->bhij", q.double(), kd) / math.sqrt(D)
+    mag = torch.einsum("bihd,bjhd->bhij", q.double().abs(), kd.abs()) / math.sqrt(D)
+    s = cap * torch.tanh(s / cap)
+    seen = ((j >= lo.view(-1, Lq, 1)) & (j < hi.view(-1, Lq, 1)))[:, None]
+    w = torch.softmax(s.masked_fill(~seen, -math.inf), 3).nan_to_num(0.0)
+    o = torch.einsum("bhij,bjhd->bihd", w, vd)
+    av = torch.einsum("bhij,bjhd->bihd", w, vd.abs())
+    e = w * (2.0 ** -20 * (mag + 1) + 2.0 ** -16 * s.abs())  # a score off by e moves w by w e, and the sum by all of them
+    moved = torch.einsum("bhij,bjhd->bihd", e, vd.abs()) + e.sum(3).transpose(1, 2)[..., None] * av
+    return o, HALF * 1.01 * av + moved + HALF * o.abs() + 1e-30
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [10.0, 256.0, 300.0, 1e3, 1e5, 1e6])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv", [(2, 1, 300, 4, 2), (1, 3, 1000, 4, 1), (1, 16, 257, 2, 2), (1, 17, 257, 2, 2),
+                                           (1, 150, 280, 4, 2)])
+def test_range_attention_caps_far_above_the_scores(B, Lq, Lk, H, Hkv, D, cap, word):
+    """A cap that no score comes near changes nothing: the weights are those of the plain scores."""
+    q, k, v = randn(B, Lq, H, D, scale=2.0, seed=60), randn(B, Lk, Hkv, D, scale=1.5, seed=61), randn(B, Lk, Hkv, D, seed=62)
+    lo, hi = random_ranges(B, Lq, Lk, 63)
+    within(ops.range_attention(q, k, v, lo, hi, softcap=cap), *capped_ref(q, k, v, lo, hi, cap))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [30.0, 256.0, 1e4, 1e6])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Lq,Lk", [(2, 300), (12, 300), (150, 300), (300, 300)])
+def test_range_attention_small_scores_beside_scores_above_the_cap(Lq, Lk, D, cap, word):
+    """Rows with scores far above the cap, and single keys far below it, next to rows and keys with small
+    scores, which must not lose their accuracy to them."""
+    H = 2
+    q, k, v = randn(1, Lq, H, D, scale=2.0, seed=64), randn(1, Lk, H, D, scale=1.5, seed=65), randn(1, Lk, H, D, seed=66)
+    lo, hi = torch.zeros(1, Lq, dtype=torch.int32, device=DEV), torch.full((1, Lq), Lk, dtype=torch.int32, device=DEV)
+    hi[0, ::3] -= 7
+    # key 40 scores about -4 cap with the even rows: it points against a channel that only they have, large
+    q[:, :, :, 0], k[:, :, :, 0] = 0, 0
+    far = math.sqrt(4 * cap * math.sqrt(D))
+    q[0, ::2, :, 0], k[0, 40, :, 0] = far, -far
+    # the scores of row 5 are far above the cap on either side, all of the largest size
+    if Lq > 5:
+        q[0, 5] *= 2 * cap
+    got = ops.range_attention(q, k, v, lo, hi, softcap=cap)
+    ref, tol = capped_ref(q, k, v, lo, hi, cap)
+    rows = torch.arange(Lq, device=DEV) != 5
+    within(got[:, rows], ref[:, rows], tol[:, rows])
+    if Lq > 5:
+        # the keys at +cap weigh alike as far as fp32 tells them apart: convex combinations of v
+        assert bool(got[0, 5].isfinite().all()) and bool((got[0, 5].abs() <= v.abs().amax(1)[0] * 1.01).all())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("Lq,Lk,H,Hkv", [(1, 200, 4, 2), (3, 200, 4, 4), (200, 200, 2, 2), (150, 400, 4, 2)])
 def test_range_attention_hidden_keys_do_not_reach_a_row(Lq, Lk, H, Hkv, word):

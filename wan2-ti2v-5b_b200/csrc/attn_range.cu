@@ -84,11 +84,35 @@ __device__ __forceinline__ float table_bias(float b) {
   return fabsf(b) < INFINITY ? fminf(fmaxf(b, -2.3e38f), 2.3e38f) : b;
 }
 
+// The cap's two forms.  cap2 - 2 cap2 / (1 + 2^x) is off by up to 3e-7 of the cap whatever the score: 1e-4
+// log2 units at a cap of 256, a twentieth of a bf16 weight's half step, but 0.2 at 1e6, where it is all of
+// a small score.  The other: where |x| = |score| / cap <= 0.6, tanh x = x P(x^2), P fitted to 5.9e-7 (least
+// maximum error of an odd polynomial of degree 7 on [0, 0.6]), within 9e-6 of the score itself.
+// Caps above 256 take the form that fits each score (kCapLarge).  For the others one form a tile is enough
+// and faster: picking costs 20% where scores pass 0.6 of the cap (4900 rows, 16 heads on 4, 82 -> 98 us)
+// and, by its registers, 3% where none does (70 -> 72), so the two are kernels of their own.
+enum RangeCap : int { kCapNone = 0, kCapSmall = 1, kCapLarge = 2 };
+constexpr float RA_CAP_SMALL = 256.f;
+constexpr float RA_TANH_MAX = 0.6f;
+constexpr float RA_TANH0 = 0.999991018f, RA_TANH1 = -0.332989737f, RA_TANH2 = 0.129745518f, RA_TANH3 = -0.0396112428f;
+
+template <int CAP>
+__device__ __forceinline__ float capped_log2(const RangeArgs& a, float s) {
+  const float t = s * a.sl2, y = a.cap2 - 2.f * a.cap2 * rcp_approx(1.f + ex2_approx(t));
+  if constexpr (CAP == kCapSmall) return y;
+  const float x = t * (0.5f / RA_LOG2E), x2 = x * x;
+  const float near0 = a.cap2 * (x * fmaf(x2, fmaf(x2, fmaf(x2, RA_TANH3, RA_TANH2), RA_TANH1), RA_TANH0));
+  return fabsf(x) <= RA_TANH_MAX ? near0 : y;
+}
+
 // 2^t-units score of one (row, key) from its raw product, for the forms that take keys one by one.
-template <bool CAP, int BIAS>
+template <int CAP, int BIAS>
 __device__ __forceinline__ float score_log2(const RangeArgs& a, float s, int h, int dist) {
-  float t = s * a.sl2;
-  if constexpr (CAP) t = a.cap2 - 2.f * a.cap2 * rcp_approx(1.f + ex2_approx(t));
+  float t;
+  if constexpr (CAP != kCapNone)
+    t = capped_log2<CAP>(a, s);
+  else
+    t = s * a.sl2;
   if constexpr (BIAS == kBiasSlopes) t = fmaf(-RA_LOG2E * __ldg(a.slopes + h), fabsf((float)dist), t);
   if constexpr (BIAS == kBiasTable)
     t = fmaf(RA_LOG2E, table_bias(__ldg(a.table + (int64_t)h * (2 * a.reach + 1) + min(max(dist, -a.reach), a.reach) + a.reach)), t);
@@ -132,7 +156,7 @@ __device__ __forceinline__ int decode_key_tiles(const RangeArgs& a, int b) {
   return from < to ? (to - from + RD_TILE - 1) / RD_TILE : 0;
 }
 
-template <int D, bool TWO, bool CAP, int BIAS>  // TWO: 9 to 16 rows, two column tiles
+template <int D, bool TWO, int CAP, int BIAS>  // TWO: 9 to 16 rows, two column tiles
 __global__ void __launch_bounds__(RD_THREADS, TWO ? RD_BLOCKS_TWO : RD_BLOCKS)
     range_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                         const __grid_constant__ RangeArgs a, const __grid_constant__ RangeParts out, const int slots, int* err) {
@@ -643,7 +667,7 @@ __device__ __forceinline__ bool unit_partial(const RangeUnit& u, int j) {
 
 // The non-finite values of V in the flagged keys of tile j (zeroed in shared memory), added to the
 // rows that see them: o += p v.  Runs in a whole warp; the scores are formed anew.
-template <int D, bool CAP, int BIAS>
+template <int D, int CAP, int BIAS>
 __device__ __noinline__ void range_poison(const RangeArgs* ap, const uint32_t* bad, int b, int kh, int j0, int tok, int head,
                                           int lo, int hi, int pos, float neg, uint32_t t_o) {
   const RangeArgs& a = *ap;
@@ -671,7 +695,7 @@ __device__ __noinline__ void range_poison(const RangeArgs* ap, const uint32_t* b
   }
 }
 
-template <int D, bool CAP, int BIAS>
+template <int D, int CAP, int BIAS>
 __global__ void __maxnreg__(160)
     range_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ RangeTileArgs g) {
@@ -1044,12 +1068,10 @@ __global__ void __maxnreg__(160)
           const float top_hi = fmax3(hi8[0], hi8[1], fmaxf(hi8[2], hi8[3]));
           // rows that are not stored do not hold the others back from the short form
           const float top = live ? fmaxf(top_hi, -fmin3(lo8[0], lo8[1], fminf(lo8[2], lo8[3]))) : 0.f;
-          if (__all_sync(0xffffffffu, top * g.cap_scale <= 0.6f)) {
-            // |x| = |score| / cap <= 0.6: tanh x = x P(x^2), P fitted to 5.9e-7 (least maximum error of an
-            // odd polynomial of degree 7 on [0, 0.6]): 3e-5 of a score capped at 50, far below the bf16
-            // rounding of its weight, and no MUFU, which bounds the general form
+          if (__all_sync(0xffffffffu, top * g.cap_scale <= RA_TANH_MAX)) {
+            // the polynomial alone: no MUFU, which bounds the general form
             const float2 kx = make_float2(g.cap_scale, g.cap_scale);
-            const float c0 = 0.999991018f * a.cap2, c1 = -0.332989737f * a.cap2, c2 = 0.129745518f * a.cap2, c3 = -0.0396112428f * a.cap2;
+            const float c0 = RA_TANH0 * a.cap2, c1 = RA_TANH1 * a.cap2, c2 = RA_TANH2 * a.cap2, c3 = RA_TANH3 * a.cap2;
             const float2 p0 = make_float2(c0, c0), p1 = make_float2(c1, c1), p2 = make_float2(c2, c2), p3 = make_float2(c3, c3);
 #pragma unroll
             for (int k = 0; k < RT_N; k += 2) {
@@ -1061,6 +1083,10 @@ __global__ void __maxnreg__(160)
             }
             const float x = top_hi * g.cap_scale, x2 = x * x;
             mx = x * fmaf(x2, fmaf(x2, fmaf(x2, c3, c2), c1), c0);
+          } else if constexpr (CAP == kCapLarge) {
+#pragma unroll
+            for (int k = 0; k < RT_N; ++k) s[k] = capped_log2<CAP>(a, s[k]);
+            mx = capped_log2<CAP>(a, top_hi);
           } else {
             // cap2 tanh = cap2 - 2 cap2 / (1 + 2^x); four reciprocals from one (MUFU bounds this form)
             const float n2c = -2.f * a.cap2;
@@ -1447,7 +1473,7 @@ struct DecodeLaunch {
   int* err;
 };
 
-template <int D, bool TWO, bool CAP, int BIAS>
+template <int D, bool TWO, int CAP, int BIAS>
 static cudaError_t launch_range_decode(const RangeArgs& a, const DecodeLaunch& d, int dev, cudaStream_t st) {
   static std::atomic<bool> attr_set[kMaxDevices] = {};
   if (!attr_set[dev].load(std::memory_order_acquire)) {
@@ -1461,7 +1487,7 @@ static cudaError_t launch_range_decode(const RangeArgs& a, const DecodeLaunch& d
   return cudaGetLastError();
 }
 
-template <int D, bool CAP, int BIAS>
+template <int D, int CAP, int BIAS>
 static int launch_range_decode(const RangeArgs& a, const DecodeLaunch& d, cudaStream_t st) {
   int dev = 0;
   cudaGetDevice(&dev);
@@ -1472,7 +1498,7 @@ static int launch_range_decode(const RangeArgs& a, const DecodeLaunch& d, cudaSt
   return d.parts.splits > 1 ? launch_range_combine<D>(a, d.parts, st) : WANB200_OK;
 }
 
-template <int D, bool CAP, int BIAS>
+template <int D, int CAP, int BIAS>
 static int launch_range_tiles(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const RangeTileArgs& g,
                               cudaStream_t st) {
   static std::atomic<bool> attr_set[kMaxDevices] = {};
@@ -1527,14 +1553,16 @@ static int range_dispatch(const RangeArgs& a, const DecodeLaunch* d, const Range
   const int bias = a.slopes ? kBiasSlopes : a.table ? kBiasTable : kBiasNone;
 #define WANB200_RANGE_CASE(cap, bs) \
   return g ? launch_range_tiles<D, cap, bs>(maps[0], maps[1], maps[2], *g, st) : launch_range_decode<D, cap, bs>(a, *d, st)
-  if (a.cap2 > 0.f) {
-    if (bias == kBiasSlopes) WANB200_RANGE_CASE(true, kBiasSlopes);
-    if (bias == kBiasTable) WANB200_RANGE_CASE(true, kBiasTable);
-    WANB200_RANGE_CASE(true, kBiasNone);
-  }
-  if (bias == kBiasSlopes) WANB200_RANGE_CASE(false, kBiasSlopes);
-  if (bias == kBiasTable) WANB200_RANGE_CASE(false, kBiasTable);
-  WANB200_RANGE_CASE(false, kBiasNone);
+#define WANB200_RANGE_CAP(cap)                                        \
+  do {                                                                \
+    if (bias == kBiasSlopes) WANB200_RANGE_CASE(cap, kBiasSlopes);    \
+    if (bias == kBiasTable) WANB200_RANGE_CASE(cap, kBiasTable);      \
+    WANB200_RANGE_CASE(cap, kBiasNone);                               \
+  } while (0)
+  if (a.cap2 <= 0.f) WANB200_RANGE_CAP(kCapNone);
+  if (a.cap2 <= RA_CAP_SMALL * RA_LOG2E) WANB200_RANGE_CAP(kCapSmall);
+  WANB200_RANGE_CAP(kCapLarge);
+#undef WANB200_RANGE_CAP
 #undef WANB200_RANGE_CASE
 }
 
