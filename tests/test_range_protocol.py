@@ -4,7 +4,9 @@ On top of the unmasked attention's protocol (test_attn_protocol.py) come a queue
 tiles of a pair that skip key tiles, and two warps that look through the V tiles which are not seen
 by every row before they are multiplied.  The model also notes which load a ring slot holds, so a
 wait that passes a phase too early shows as a wrong load."""
+import os
 import random
+import re
 
 from test_attn_protocol import Bar, _drive
 
@@ -204,3 +206,18 @@ def test_tiles_to_check_must_be_announced():
         units = [((0, 20), (0, 20), {19}) for _ in range(rnd.randint(1, 4))]
         fails += not run(units, 5, seed, announced=False)
     assert fails > 0
+
+
+def test_what_the_launch_before_writes_is_read_with_plain_loads():
+    """The tile attention and the adapter GEMM start beside the launch that plans for them.  The read-only path
+    is for memory that stays as it is over the whole kernel, so it may read a call's inputs only."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "wan2-ti2v-5b_b200", "csrc")
+    inputs = {
+        "attn_range.cu": {"a.lo", "a.hi", "a.pos", "a.slopes", "a.table", "p.a.table", "a.q"},
+        "lora.cu": {"a.ids", "a.scales", "xp", "dp", "x0", "x1", "up"},
+        "gemm.cu": {"a.bias", "a.gate_mod", "a.gate_e0", "lo->ids", "bp", "mp", "ep"},
+    }
+    for name, allowed in inputs.items():
+        with open(os.path.join(csrc, name)) as f:
+            read = re.findall(r"__ldg\((?:reinterpret_cast<[^>]*>\()?\s*([\w.>-]+)", f.read())
+        assert read and not set(read) - allowed, (name, set(read) - allowed)

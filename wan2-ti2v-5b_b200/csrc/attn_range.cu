@@ -621,6 +621,9 @@ struct RangeUnit {
   int full_lo[2], full_hi[2];          // keys that every row of the tile sees
 };
 
+// The plan (order, pairs, padded) is written while this kernel already runs, so it is read with plain loads:
+// the read-only path is for memory that stays as it is over the whole kernel, and its loads may be moved up
+// past the wait for the plan.
 __device__ __forceinline__ RangeUnit range_unit(const RangeTileArgs& g, int u) {
   RangeUnit r;
   const int per_group = g.stream_group * g.entries * g.splits;
@@ -628,13 +631,13 @@ __device__ __forceinline__ RangeUnit range_unit(const RangeTileArgs& g, int u) {
   int x = u - grp * per_group;
   r.split = x % g.splits;
   x /= g.splits;
-  const int stream = first + x % size, e = __ldg(g.order + x / size);
+  const int stream = first + x % size, e = g.order[x / size];
   r.kh = stream % g.a.kv_heads;
   r.mb = e / g.nqp;
   r.b = g.a.range_batch ? r.mb : stream / g.a.kv_heads;
   r.tok0 = e % g.nqp * 2 * g.tpt;
   const int4* pp = reinterpret_cast<const int4*>(g.pairs + e);
-  const int4 any = __ldg(pp), all = __ldg(pp + 1);
+  const int4 any = pp[0], all = pp[1];
   r.a[0] = any.x / RT_N, r.a[1] = any.y / RT_N;
   r.z[0] = (any.z + RT_N - 1) / RT_N, r.z[1] = (any.w + RT_N - 1) / RT_N;
   r.full_lo[0] = all.x, r.full_lo[1] = all.y, r.full_hi[0] = all.z, r.full_hi[1] = all.w;
@@ -1114,7 +1117,7 @@ __global__ void __maxnreg__(160)
         if constexpr (BIAS == kBiasTable) {  // the padded table: one clamp a row, fixed offsets for its keys
           const float* tp = trow + min(max(kbase - pos, -a.reach - RT_N), a.reach);
 #pragma unroll
-          for (int k = 0; k < RT_N; ++k) s[k] = CAP ? s[k] + __ldg(tp + k) : fmaf(s[k], sl2, __ldg(tp + k));
+          for (int k = 0; k < RT_N; ++k) s[k] = CAP ? s[k] + tp[k] : fmaf(s[k], sl2, tp[k]);
         }
         const float mul = BIAS == kBiasNone && !CAP ? a.sl2 : 1.f;  // what is left to apply in the exponent
         if (masked) {

@@ -233,9 +233,11 @@ __device__ __forceinline__ void gemm_epilogue_chunk(const GemmArgs& a, float* v,
 __device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 
-// The steps of chunk c (4 bits) that a row of the tile uses.
+// The steps of chunk c (4 bits) that a row of the tile uses.  The down-projection writes them, `mixed` and h
+// while this kernel already runs: they are read after pdl_wait() with plain loads, not by the read-only path,
+// which is for memory that stays as it is over the whole kernel.
 __device__ __forceinline__ uint32_t lora_chunk_steps(const uint32_t* mask, int c) {
-  return (__ldg(mask + (c >> 3)) >> ((c & 7) * 4)) & 0xfu;
+  return (mask[c >> 3] >> ((c & 7) * 4)) & 0xfu;
 }
 
 // What the non-finite up-projection weights (zeroed in shared memory ahead of the MMA) add to the
@@ -569,7 +571,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
         if constexpr (LORA) {
           pdl_wait();  // h and the step bits come from the launch before, which runs beside this K loop
           const uint32_t* mask = lora->step_mask + m0 / GBM * LORA_MASK_WORDS;
-          const bool mixed = __ldg(lora->mixed + m0 / GBM) != 0;
+          const bool mixed = lora->mixed[m0 / GBM] != 0;
           for (int c = 0, n = 0; ok && c < lora->cols / LORA_CHUNK; ++c) {
             if (!lora_chunk_steps(mask, c) || n++ % lora->ksplit != krank) continue;
             for (int pl = 0; pl < lora->planes; ++pl) {
@@ -636,7 +638,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
           tile_origin(tile, num_m, num_n, bn, m0, n0);
           pdl_wait();
           const uint32_t* mask = lora->step_mask + m0 / GBM * LORA_MASK_WORDS;
-          const bool mixed = __ldg(lora->mixed + m0 / GBM) != 0;
+          const bool mixed = lora->mixed[m0 / GBM] != 0;
           for (int c = 0, n = 0; ok && c < lora->cols / LORA_CHUNK; ++c) {
             const uint32_t steps = lora_chunk_steps(mask, c);
             if (!steps || n++ % lora->ksplit != krank) continue;
@@ -700,7 +702,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
         load += kblocks;
         pdl_wait();
         const uint32_t* mask = lora->step_mask + m0 / GBM * LORA_MASK_WORDS;
-        const bool mixed = __ldg(lora->mixed + m0 / GBM) != 0;
+        const bool mixed = lora->mixed[m0 / GBM] != 0;
         for (int c = 0, n = 0; ok && c < lora->cols / LORA_CHUNK; ++c) {
           if (!lora_chunk_steps(mask, c) || n++ % lora->ksplit != krank) continue;
           if (!mixed) {
