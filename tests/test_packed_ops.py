@@ -789,6 +789,30 @@ def test_lora_linear_spares_rows_beside_broken_adapters(M, K, r, order, word):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("order", ["mixed", "one"])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("M,K,r", [(9, 128, 16), (150, 128, 16), (150, 128, 24), (260, 2048, 16)])
+def test_lora_linear_infinite_weight_in_use(M, K, r, f32, order, word):
+    """An infinite up-projection weight gives its rows an infinity of the intermediate's sign, whoever shares
+    their tile."""
+    x, w, b, down, up, ids, scales = lora_case(M, K, 64, 3, r, 220)
+    if order == "one":
+        ids = torch.full_like(ids, 1)
+    up[5, 1, 3], up[6, 1, 0] = math.inf, -math.inf
+    got = ops.lora_linear(x, w, b, down, up, ids, scales=scales, out=torch.empty(M, 64, dtype=torch.float32 if f32 else BF16, device=DEV))
+    on = ids == 1
+    h = x.double() @ down[1].double().t()
+    sure = on & (h[:, [0, 3]].abs() > 1e-3).all(1)  # the sign of a value near zero is not settled in fp32
+    assert bool(sure.any()) and bool(got[~on].isfinite().all())
+    for col, i, sign in ((5, 3, 1.0), (6, 0, -1.0)):
+        assert torch.equal(got[sure, col].double(), torch.copysign(torch.full_like(h[sure, i], math.inf), sign * h[sure, i]))
+    rest = torch.ones(64, dtype=torch.bool, device=DEV)
+    rest[5] = rest[6] = False
+    ref, tol = lora_ref(x, w, b, down, torch.where(up.isfinite(), up, torch.zeros_like(up)), ids, scales, L.EPI_BIAS, f32=f32)
+    within(got[:, rest], ref[:, rest], tol[:, rest])
+
+
+@pytest.mark.gpu
 def test_lora_linear_bad_id_counts_as_none():
     L.device_error(reset=True)
     for M in (6, 200):

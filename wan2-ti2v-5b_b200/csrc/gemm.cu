@@ -688,7 +688,8 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
   } else if (LORA && warp >= 2 + G_EPI_WARPS) {
     // Two warps look through the up-projection tiles: h = 0 keeps a row clear of another adapter's
     // finite weights, but 0 * NaN does not, so non-finite weights are zeroed before the MMA and added
-    // by the epilogue to the rows whose adapter has them; a tile whose rows all use one adapter, and
+    // by the epilogue to the rows whose adapter has them, as is what the planes of an fp32 output's h
+    // would make of an infinity one by one; a tile with one plane whose rows all use one adapter, and
     // whose steps hold no column of another, needs none of it.  The producer announces each such stage
     // (u_req), so these warps pass over the others without a wait: its phases move only with the
     // stages they handle, and neither they nor `full` can get a phase ahead before u_ok is given.

@@ -123,11 +123,13 @@ __global__ void __launch_bounds__(LD_THREADS, 1)
   if (threadIdx.x < LORA_MASK_WORDS && krank == 0)
     a.step_mask[blockIdx.y * LORA_MASK_WORDS + threadIdx.x] = bits[threadIdx.x];
   // a row is mixed with an adapter that it does not use where the tile's rows differ, or where a step at
-  // either end of its own adapter's columns holds some of the next one's (ranks that are no multiple of 16)
-  int mixed = 0;
+  // either end of its own adapter's columns holds some of the next one's (ranks that are no multiple of 16);
+  // and several planes of h must not meet an infinite weight one by one: its product with a plane that is
+  // zero, or of the other sign, makes a NaN of what is an infinity
+  int mixed = a.planes > 1;
   if (threadIdx.x < LD_BM && m0 + (int)threadIdx.x < a.M) {
     const int id = ids[threadIdx.x], first = id * a.rank, last = first + a.rank;
-    mixed = id != ids[0] || (id >= 0 && (first % LORA_STEP || (last % LORA_STEP && id + 1 < a.adapters)));
+    mixed |= id != ids[0] || (id >= 0 && (first % LORA_STEP || (last % LORA_STEP && id + 1 < a.adapters)));
   }
   mixed = __syncthreads_or(mixed);
   if (threadIdx.x == 0 && krank == 0) a.mixed[blockIdx.y] = mixed != 0;

@@ -14,7 +14,7 @@ constexpr int LORA_MASK_WORDS = LORA_MAX_COLS / LORA_STEP / 32;  // 8 words of s
 // Workspace of one call: [row tiles][8] step bits | [row tiles] mixed | h planes.
 struct LoraPlan {
   const uint32_t* step_mask;  // steps that some row of the tile uses
-  const int* mixed;           // the tile's steps hold columns of an adapter that not all its rows use
+  const int* mixed;           // the tile's steps hold columns of an adapter that not all its rows use, or h has planes
   const __nv_bfloat16* h;     // [planes][rows_pad][cols]: scale * (x . down^T) in bf16 planes that add up
   const __nv_bfloat16* up;    // [N][adapters * rank]
   const int32_t* ids;
