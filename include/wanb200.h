@@ -103,8 +103,8 @@ int wanb200_gemm_bf16(const wanb200_gemm_params* p, void* stream);
  * low-rank update of its own adapter, or none where id < 0 -- the adapters of many requests in one
  * batch, rows in any order (rows of one adapter next to each other cost least).  The update joins
  * the accumulators before the epilogue (bias, GELU, gate, residual); all epilogues but SUMSQ and
- * SCATTER.  The rank-wide intermediate is held in bf16, or for fp32 outputs in two bf16 planes
- * (16 significant bits).  NaN or infinite weights of an adapter reach the rows that use it only.
+ * SCATTER.  The rank-wide intermediate is held in bf16, or for fp32 outputs in three bf16 planes
+ * (24 significant bits, those of fp32).  NaN or infinite weights of an adapter reach the rows that use it only.
  * An id >= adapters counts as none and sets the device error word to 502.  d must not overlap a (it
  * may alias residual); tile_n does not act on calls of up to 16 rows, which read w once with other
  * kernels and keep the intermediate in fp32.

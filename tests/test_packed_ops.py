@@ -789,6 +789,30 @@ def test_lora_linear_spares_rows_beside_broken_adapters(M, K, r, order, word):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("order", ["mixed", "sorted"])
+@pytest.mark.parametrize("M,K,r,N", [(11, 64, 16, 64), (40, 64, 8, 64), (300, 64, 64, 96), (300, 2048, 24, 96), (1000, 192, 40, 64)])
+def test_lora_linear_fp32_output_keeps_the_intermediate(M, K, r, N, order, word):
+    """With w = 0 and one value a row of x the intermediate is a scaled product of two bf16 values, which fp32
+    holds to half a step: an fp32 output is as good, up to the additions of its matrix products (a step of fp32
+    of the sum of magnitudes for each K step of 16 that adds something, and each bf16 plane of h)."""
+    x, w, _, down, up, ids, scales = lora_case(M, K, N, 3, r, 210, order)
+    keep = torch.arange(M, device=DEV) * 7 % K
+    x = torch.zeros_like(x).scatter_(1, keep[:, None], x.gather(1, keep[:, None]))
+    up[:, :, 3:] = 0  # few terms, so that the error of each shows
+    ref = torch.zeros(M, N, dtype=torch.float64, device=DEV)
+    mag = torch.zeros_like(ref)
+    for a in range(3):
+        h = scales[a].double() * (x.double() @ down[a].double().t())
+        on = (ids == a)[:, None]
+        ref += on * (h @ up[:, a].double().t())
+        mag += on * (h.abs() @ up[:, a].double().abs().t())
+    got = ops.lora_linear(x, torch.zeros_like(w), None, down, up, ids, scales=scales, epilogue=L.EPI_NONE,
+                          out=torch.empty(M, N, device=DEV))
+    steps = 3 * 2  # planes x steps of 16 columns that hold an adapter's first three
+    within(got, ref, (steps + 2) * 2.0 ** -23 * mag + 1e-30)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("order", ["mixed", "one"])
 @pytest.mark.parametrize("f32", [False, True])
 @pytest.mark.parametrize("M,K,r", [(9, 128, 16), (150, 128, 16), (150, 128, 24), (260, 2048, 16)])

@@ -38,25 +38,26 @@ __device__ __forceinline__ uint2 bf16x4(const float4& v) { return make_uint2(pac
 
 // Four adjacent columns of a row of h: the row's adapter's columns scaled, zeros elsewhere (selected,
 // so a NaN of another adapter's product goes no further), rounded to bf16 -- the operand type of the
-// MMA that takes them; for an fp32 output a second plane holds what the rounding left.
+// MMA that takes them.  For an fp32 output two more planes hold what the rounding left: 3 x 8 significant
+// bits are those of fp32, and both remainders are exact.
 __device__ __forceinline__ void lora_store_h(const LoraDownArgs& a, int row, int col, float4 v, int first, int last, float scale) {
   v.x = col >= first && col < last ? v.x * scale : 0.f;
   v.y = col + 1 >= first && col + 1 < last ? v.y * scale : 0.f;
   v.z = col + 2 >= first && col + 2 < last ? v.z * scale : 0.f;
   v.w = col + 3 >= first && col + 3 < last ? v.w * scale : 0.f;
   __nv_bfloat16* hp = a.h + (int64_t)row * a.cols + col;
-  const uint2 hi = bf16x4(v);
-  *reinterpret_cast<uint2*>(hp) = hi;
-  if (a.planes > 1) {
-    float4 r;
-    r.x = v.x - __uint_as_float(hi.x << 16);
-    r.y = v.y - __uint_as_float(hi.x & 0xffff0000u);
-    r.z = v.z - __uint_as_float(hi.y << 16);
-    r.w = v.w - __uint_as_float(hi.y & 0xffff0000u);
+  for (int pl = 0;; ) {
+    const uint2 hi = bf16x4(v);
+    *reinterpret_cast<uint2*>(hp) = hi;
+    if (++pl == a.planes) break;
+    v.x -= __uint_as_float(hi.x << 16);
+    v.y -= __uint_as_float(hi.x & 0xffff0000u);
+    v.z -= __uint_as_float(hi.y << 16);
+    v.w -= __uint_as_float(hi.y & 0xffff0000u);
     // an infinite h has no remainder
-    r.x = isfinite(r.x) ? r.x : 0.f, r.y = isfinite(r.y) ? r.y : 0.f;
-    r.z = isfinite(r.z) ? r.z : 0.f, r.w = isfinite(r.w) ? r.w : 0.f;
-    *reinterpret_cast<uint2*>(hp + a.rows_pad * a.cols) = bf16x4(r);
+    v.x = isfinite(v.x) ? v.x : 0.f, v.y = isfinite(v.y) ? v.y : 0.f;
+    v.z = isfinite(v.z) ? v.z : 0.f, v.w = isfinite(v.w) ? v.w : 0.f;
+    hp += a.rows_pad * a.cols;
   }
 }
 
@@ -535,7 +536,7 @@ static LoraLayout lora_layout(int64_t M, int adapters, int rank, int out_f32) {
   l.num_m = (M + LD_BM - 1) / LD_BM;
   l.rows_pad = l.num_m * LD_BM;
   l.cols = (adapters * rank + LORA_CHUNK - 1) / LORA_CHUNK * LORA_CHUNK;
-  l.planes = out_f32 ? 2 : 1;
+  l.planes = out_f32 ? LORA_F32_PLANES : 1;
   l.mixed_off = l.num_m * LORA_MASK_WORDS * 4;
   l.h_off = (l.mixed_off + l.num_m * 4 + 255) / 256 * 256;
   l.bytes = l.h_off + l.planes * l.rows_pad * l.cols * 2;
