@@ -308,6 +308,21 @@ def test_head_norm_rope_refuses_overlap():
                            positions=torch.zeros(8, dtype=torch.int64, device=DEV))
 
 
+@pytest.mark.gpu
+def test_head_norm_rope_offsets_past_32_bits(word):
+    M, hq, d, ld = 700_000, 2, 128, 3200
+    x = torch.zeros(M, ld, dtype=BF16, device=DEV)
+    assert x.numel() > 2 ** 31
+    x[-40:] = randn(40, ld, seed=7)
+    g, ang = randn(d, seed=8), torch.rand(50, d // 2, device=DEV) * 6
+    pos = (torch.arange(M, device=DEV) % 50).to(torch.int32)
+    secs = [(ld - hq * d, hq, g)]
+    ref, tol = head_norm_ref(x[-40:], secs, d, d, ang.cos(), ang.sin(), pos[-40:].long(), True)
+    ops.head_norm_rope(x, secs, d, cos=ang.cos(), sin=ang.sin(), positions=pos)
+    within(x[-40:], ref, tol)
+    assert not bool(x[:-40].any())
+
+
 # ---------------------------------------------------------------------------- range attention
 def attn_ref(q, k, v, lo, hi, pos=None, cap=0.0, slopes=None, table=None, scale=None):
     """fp64 (o, bound).  The kernel rounds the weights to bf16 for the product with v (half a step of
@@ -566,6 +581,77 @@ def test_range_attention_hidden_keys_do_not_reach_a_row(Lq, Lk, H, Hkv, word):
             ref = torch.softmax(s, 0) @ va[:, h // (H // Hkv)]
             assert torch.equal(got[0, r, h].isfinite(), ref.isfinite()), (r, h)
             assert torch.equal(one[h].isfinite(), ref.isfinite()), (r, h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cap", [0.0, 5.0, 1e4])
+@pytest.mark.parametrize("bias", ["none", "slopes", "table"])
+@pytest.mark.parametrize("Lq,Lk,H,Hkv", [(1, 200, 4, 2), (2, 200, 4, 2), (3, 200, 4, 1), (40, 200, 2, 2), (150, 300, 2, 1)])
+def test_range_attention_non_finite_values_seen_and_hidden(Lq, Lk, H, Hkv, bias, cap, D, word):
+    """Rows that do not see a NaN or an infinity keep their values; rows that do have what the formula gives,
+    infinities with their sign, in every form of the score."""
+    q, k, v = randn(1, Lq, H, D, seed=70), randn(1, Lk, Hkv, D, seed=71), randn(1, Lk, Hkv, D, seed=72)
+    i = torch.arange(Lq, device=DEV)
+    hi = (Lk - Lq + i + 1).to(torch.int32)[None]
+    lo = (hi - 70).clamp_min(0)
+    lo[0, ::7], hi[0, ::7] = 0, Lk  # some rows see all keys, the last and the first
+    v[0, 20, :, 5], v[0, Lk - 1, 0, 7], v[0, Lk - 2, 0, 7], v[0, Lk - 40, Hkv - 1, D - 1] = math.nan, math.inf, -math.inf, math.inf
+    k[0, 25], k[0, Lk - 30, 0, 3] = math.nan, math.inf
+    kw = dict(cap=cap)
+    if bias == "slopes":
+        kw["slopes"] = torch.rand(H, device=DEV) * 0.2
+    elif bias == "table":
+        kw["table"] = torch.randn(H, 61, device=DEV)
+    got = ops.range_attention(q, k, v, lo, hi, softcap=cap, slopes=kw.get("slopes"), dist_bias=kw.get("table"))
+    ref, tol = attn_ref(q, k, v, lo, hi, **kw)
+    fine = ref.isfinite()
+    assert Lq == 1 or bool(fine.any())  # a row alone sees all keys
+    assert torch.equal(got.isfinite(), fine) and torch.equal(got.isnan(), ref.isnan())
+    assert torch.equal(got[ref.isinf()].double(), ref[ref.isinf()])
+    within(torch.where(fine, got, torch.zeros_like(got)), torch.where(fine, ref, torch.zeros_like(ref)), tol.nan_to_num(1e-30))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D", [
+    (1, 1, 9000, 24, 1, 128), (1, 40, 9000, 1, 1, 64), (1, 1, 12000, 40, 2, 64), (2, 1, 5000, 128, 1, 128), (1, 17, 20000, 1, 1, 128)])
+def test_range_attention_few_tiles_over_long_caches(B, Lq, Lk, H, Hkv, D, word):
+    """One or two pairs of row tiles over a cache of more key tiles than a pair is split into."""
+    q, k, v = randn(B, Lq, H, D, seed=73), randn(B, Lk, Hkv, D, seed=74), randn(B, Lk, Hkv, D, seed=75)
+    lens = torch.tensor([Lk, Lk // 3][:B], dtype=torch.int32, device=DEV)
+    lo, hi, pos = ranges.cache_ranges(lens, Lq)
+    check_attn(q, k, v, lo, hi, pos=pos)
+    check_attn(q, k, v, lo, hi, pos=pos, slopes=torch.rand(H, device=DEV) * 0.01, cap=20.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Lq", [1, 150])
+def test_range_attention_batch_inside_tokens(Lq, word):
+    """Tensors laid out [L, B, H, D]: the batch stride is the smaller one."""
+    B, Lk, H, Hkv, D = 3, 200, 4, 2, 64
+    q, k, v = (randn(n, B, h, D, seed=s).transpose(0, 1) for n, h, s in ((Lq, H, 76), (Lk, Hkv, 77), (Lk, Hkv, 78)))
+    lo, hi = random_ranges(B, Lq, Lk, 79)
+    ref, tol = attn_ref(q, k, v, lo, hi)
+    out = torch.empty(Lq, B, H, D, dtype=BF16, device=DEV).transpose(0, 1)
+    within(ops.range_attention(q, k, v, lo, hi, out=out), ref, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Lq", [1, 60])
+def test_range_attention_offsets_past_32_bits(Lq, word):
+    """A cache of more than 2^31 values, seen at its start, its end and, in between, by rows with a few keys."""
+    Lk, Hkv, H, D = 2 ** 21 + 1000, 8, 16, 128
+    k, v = torch.zeros(1, Lk, Hkv, D, dtype=BF16, device=DEV), torch.zeros(1, Lk, Hkv, D, dtype=BF16, device=DEV)
+    assert k.numel() > 2 ** 31
+    k[:, -300:], v[:, -300:] = randn(1, 300, Hkv, D, seed=80), randn(1, 300, Hkv, D, seed=81)
+    v[:, -400, :, 3] = math.nan  # a tile that is partly seen, its non-finite value hidden
+    q = randn(1, Lq, H, D, seed=82)
+    pos = (Lk - Lq + torch.arange(Lq, device=DEV)).to(torch.int32)
+    lo, hi = pos - 240, pos + 1
+    got = ops.range_attention(q, k, v, lo, hi, pos=pos, slopes=torch.full((H,), 0.01, device=DEV))
+    cut = Lk - 300
+    ref, tol = attn_ref(q, k[:, cut:], v[:, cut:], lo - cut, hi - cut, pos=pos - cut, slopes=torch.full((H,), 0.01, device=DEV))
+    within(got, ref, tol)
 
 
 @pytest.mark.gpu
@@ -834,6 +920,33 @@ def test_lora_linear_infinite_weight_in_use(M, K, r, f32, order, word):
     rest[5] = rest[6] = False
     ref, tol = lora_ref(x, w, b, down, torch.where(up.isfinite(), up, torch.zeros_like(up)), ids, scales, L.EPI_BIAS, f32=f32)
     within(got[:, rest], ref[:, rest], tol[:, rest])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("epi", [L.EPI_NONE, L.EPI_BIAS_GELU, L.EPI_BIAS_SILU, L.EPI_BIAS_RES, L.EPI_BIAS_GATE_RES])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("M,K", [(12, 128), (150, 128), (260, 2048)])
+def test_lora_linear_epilogues_beside_broken_adapters(M, K, epi, f32, word):
+    """Tiles with non-finite weights have an epilogue of their own, with and without K shared by a cluster: the
+    rows of the other adapters get what they get without them."""
+    N, n, r = 96, 4, 16
+    x, w, b, down, up, ids, scales = lora_case(M, K, N, n, r, 230)
+    up[7, 2, 3], up[40, 2, 0], down[1, 2] = math.inf, math.nan, math.nan
+    dt = torch.float32 if f32 else BF16
+    kw, rf = {}, {}
+    if epi in (L.EPI_BIAS_RES, L.EPI_BIAS_GATE_RES):
+        kw["residual"] = rf["residual"] = randn(M, N, seed=40).to(dt)
+    if epi == L.EPI_BIAS_GATE_RES:
+        mod, e0 = randn(N, seed=41), torch.randn(5, N, device=DEV)
+        kw["gate"], kw["frames"] = (mod, e0), (M, -(-M // 5))
+        rf["gate"] = (mod.double() + e0.double())[(torch.arange(M, device=DEV) // -(-M // 5))]
+    bias = None if epi == L.EPI_NONE else b
+    got = ops.lora_linear(x, w, bias, down, up, ids, scales=scales, epilogue=epi, out=torch.empty(M, N, dtype=dt, device=DEV), **kw)
+    clean = [torch.where(t.isfinite(), t, torch.zeros_like(t)) for t in (down, up)]
+    ref, tol = lora_ref(x, w, bias, *clean, ids, scales, epi, f32=f32, **rf)
+    spared = ((ids != 2)[:, None] | ((torch.arange(N, device=DEV) != 7) & (torch.arange(N, device=DEV) != 40))) & (ids != 1)[:, None]
+    assert bool((ids == 2).any()) and bool((ids == 1).any()) and not bool(got[~spared].isfinite().all())
+    within(got[spared], ref[spared], tol[spared])
 
 
 @pytest.mark.gpu
