@@ -197,6 +197,24 @@ def test_ops_need_cuda_tensors():
         ops.lora_linear(x, x, None, x, x, r)
 
 
+def test_blocks_of_rows_that_share_no_byte():
+    """ops._apart against the bytes themselves; it may refuse, but never pass a pair that shares one."""
+    g = torch.Generator().manual_seed(3)
+    passed = 0
+    for _ in range(3000):
+        a, b = ([int(x) for x in torch.randint(0, hi, (4,), generator=g)] for hi in (24, 24))
+        if passed % 2:
+            b[1] = a[1]  # one stride
+        a[2], b[2], a[3], b[3] = a[2] % 6 + 1, b[2] % 6 + 1, a[3] % 4 + 1, b[3] % 4 + 1
+        bytes_of = [{p + i * st + k for i in range(m) for k in range(w)} for p, st, w, m in (a, b)]
+        if ops._apart(a, b):
+            passed += 1
+            assert not bytes_of[0] & bytes_of[1], (a, b)
+        assert ops._apart(a, b) == ops._apart(b, a)
+    assert passed > 300
+    assert ops._apart((0, 16, 4, 9), (4, 16, 12, 9)) and not ops._apart((0, 16, 4, 9), (3, 16, 4, 9))
+
+
 # ---------------------------------------------------------------------------- head norm
 def head_norm_ref(x, secs, d, rot, cos, sin, pos, inter, eps=1e-6):
     """fp64 (values, bound): the bound is half a bf16 step plus fp32 steps of the pair's magnitude."""
@@ -711,6 +729,32 @@ def test_range_attention_strided_views_and_out(word):
     assert bool((big[:, 0] == 3).all()) and bool((big[:, T + 1:] == 3).all()) and bool((big[:, :, H] == 3).all())
     one = ops.range_attention(q[:, :1], k, v, lo[:, :1].contiguous(), hi[:, :1].contiguous())
     within(one, ref[:, :1], tol[:, :1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [1, 2])
+def test_outputs_beside_inputs_in_one_buffer(B, word):
+    """Columns of one buffer that do not meet: each call writes its own and leaves the others alone."""
+    T, H, D, C = 150, 2, 64, 128
+    buf = randn(B, T, 6 * C, seed=83)
+    want = buf.clone()
+    q, k, v, o = (buf[..., i * C:(i + 1) * C].unflatten(2, (H, D)) for i in range(4))
+    lo, hi = random_ranges(B, T, T, 84)
+    want[..., 3 * C:4 * C] = ops.range_attention(q.contiguous(), k.contiguous(), v.contiguous(), lo, hi).flatten(2)
+    assert ops.range_attention(q, k, v, lo, hi, out=o) is o
+    rows, wrows = buf.view(B * T, 6 * C), want.view(B * T, 6 * C)
+    _, w, b, down, up, ids, scales = lora_case(B * T, C, C, 3, 16, 85)
+    wrows[:, 4 * C:5 * C] = ops.lora_linear(wrows[:, 3 * C:4 * C].contiguous(), w, b, down, up, ids, scales=scales)
+    ops.lora_linear(rows[:, 3 * C:4 * C], w, b, down, up, ids, scales=scales, out=rows[:, 4 * C:5 * C])
+    g = randn(D, seed=86)
+    wrows[:, 5 * C:] = ops.head_norm_rope(wrows[:, 4 * C:5 * C].contiguous(), [(0, H, g)], D)
+    ops.head_norm_rope(rows[:, 4 * C:5 * C], [(0, H, g)], D, out=rows[:, 5 * C:])
+    assert torch.equal(buf, want)
+    for at in (3 * C - 8, 2 * C, 5):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.range_attention(q, k, v, lo, hi, out=buf[..., at:at + C].unflatten(2, (H, D)))
+    with pytest.raises(ValueError, match="overlap"):
+        ops.lora_linear(rows[:, :C], w, b, down, up, ids, out=rows[:, C - 8:2 * C - 8])
 
 
 @pytest.mark.gpu

@@ -426,6 +426,18 @@ def _row_major(t, name, what):
     return m, n, sm if m != 1 else (n + 7) // 8 * 8
 
 
+def _apart(a, b):
+    """Whether two blocks of rows, each (address, row stride, bytes of a row, rows), share no byte: one lies
+    behind the other, or both are columns of rows of one stride that do not meet."""
+    (pa, sa, wa, ma), (pb, sb, wb, mb) = a, b
+    if pb >= pa + (ma - 1) * sa + wa or pa >= pb + (mb - 1) * sb + wb:
+        return True
+    if sa != sb or sa <= 0:
+        return False
+    at = (pb - pa) % sa
+    return at >= wa and at + wb <= sa
+
+
 def head_norm_rope(x, sections, head_dim, *, out=None, eps=1e-6, cos=None, sin=None, positions=None,
                    interleaved=True, kind="head_norm_rope"):
     """RMS norm of every head with the rotation in the same pass (wanb200_head_norm_rope): for each
@@ -450,8 +462,8 @@ def head_norm_rope(x, sections, head_dim, *, out=None, eps=1e-6, cos=None, sin=N
         mo, no, ldo = _row_major(out, "out", "head_norm_rope")
         _need(out.dtype == BF16 and mo == M, "head_norm_rope: out must be bf16 with x's rows")
         op_ = out.data_ptr()
-        _need((op_ == xp and ldo == ldx) or op_ >= xp + 2 * ((M - 1) * ldx + cols) or
-              xp >= op_ + 2 * ((M - 1) * ldo + no), "head_norm_rope: out must be x or not overlap it")
+        _need((op_ == xp and ldo == ldx) or _apart((xp, 2 * ldx, 2 * cols, M), (op_, 2 * ldo, 2 * no, M)),
+              "head_norm_rope: out must be x or not overlap it")
         cols = min(cols, no)
     if M == 0:
         return out
@@ -514,11 +526,15 @@ def range_attention(q, k, v, lo, hi, *, pos=None, out=None, softmax_scale=None, 
     qa, ka, va = layout(q, "q", Lq, H), layout(k, "k", Lk, Hkv), layout(v, "v", Lk, Hkv)
     oa = layout(out, "out", Lq, H)
     if not fresh:
-        def end(a, n, h):
-            return a[0] + 2 * ((B - 1) * a[2] + (n - 1) * a[1] + h * D)
-        oe = end(oa, Lq, H)
+        def block(a, n, h):
+            """All batch elements' rows for _apart, as columns of one buffer where the batch stride is whole rows."""
+            addr, st, sb = a
+            if st > 0 and (B == 1 or sb % st == 0):
+                return addr, 2 * st, 2 * h * D, (B - 1) * sb // st + n
+            return addr, 0, 2 * ((B - 1) * sb + (n - 1) * st + h * D), 1
+        ob = block(oa, Lq, H)
         for a, n, h in ((qa, Lq, H), (ka, Lk, Hkv), (va, Lk, Hkv)):
-            _need(oa[0] >= end(a, n, h) or a[0] >= oe, "range_attention: out must not overlap q, k or v")
+            _need(_apart(ob, block(a, n, h)), "range_attention: out must not overlap q, k or v")
     shape = lo.shape
     _need(shape == (Lq,) or shape == (B, Lq) or shape == (1, Lq), "range_attention: lo must be [Lq] or [B, Lq]")
     for t, name in ((lo, "lo"), (hi, "hi"), (pos, "pos")):
@@ -580,7 +596,7 @@ def lora_linear(a, w, bias, down, up, ids, *, scales=None, epilogue=L.EPI_BIAS, 
         f32 = int(out.dtype == torch.float32)
         _need((f32 or out.dtype == BF16) and mo == M and no == N, "lora_linear: out must be bf16 or fp32 [M, N]")
         d, es = out.data_ptr(), 4 if f32 else 2
-        _need(d >= ap + 2 * ((M - 1) * lda + K) or ap >= d + es * ((M - 1) * ldd + N), "lora_linear: out must not overlap a")
+        _need(_apart((ap, 2 * lda, 2 * K, M), (d, es * ldd, es * N, M)), "lora_linear: out must not overlap a")
     if M == 0:
         return out
     res = (None, 0)
