@@ -41,14 +41,15 @@ struct RangeArgs {
   int reach;
 };
 
-// Unnormalised results of the key splits, to be merged by range_combine_kernel: slot i holds one
-// split's [slot_rows][D] outputs and [slot_rows] (maximum in log2 units, sum; sum = -1 and no output
-// where the split saw no key tile).  The splits of row group x (slot_rows rows of one batch element and
-// key head) are the slots first[x].x + k * first[x].z for k < first[x].y.
+// Unnormalised results of the key splits: slot i holds one split's [slot_rows][D] outputs and [slot_rows]
+// (maximum in log2 units, sum).  Of the few-rows kernel: the splits of row group x (slot_rows rows of one
+// batch element and key head) are the slots first[x].x + k * first[x].z for k < first[x].y, merged by
+// range_combine_kernel.  Of the tiles: slots x, x + groups, ... of `splits`, merged by range_join_kernel;
+// a split that saw no key tile has sum -1 and no output.
 struct RangeParts {
   float* o;
   float2* ml;
-  int4* first;   // written by the few-rows kernel; the tiles' groups all have (x, splits, groups)
+  int4* first;  // few-rows kernel only
   int slot_rows, groups, splits;
 };
 
@@ -1279,7 +1280,6 @@ __global__ void __launch_bounds__(RC_WARPS * 32) range_combine_kernel(const Rang
 #pragma unroll 4
   for (int s = warp; s < f4.y; s += RC_WARPS) {
     const float2 ml = in.ml[row0 + s * next];
-    if (ml.y == -1.f) continue;
     const float f = ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - m);
     l = fmaf(f, ml.y, l);
 #pragma unroll

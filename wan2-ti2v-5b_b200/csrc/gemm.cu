@@ -10,14 +10,15 @@
 // of tile t overlaps the main loop of tile t+1.  One CTA per SM, tiles strided over the
 // persistent grid in grouped order so the CTAs running together share A rows and W.
 //
-// Warp roles (320 threads):
-//   warp 0      TMA producer (one lane)
-//   warp 1      TMEM allocator + UMMA issuer (one lane)
+// Warp roles (320 threads; 384 with adapters):
+//   warp 0      TMA producer (the whole warp walks the loop, an elected lane issues)
+//   warp 1      TMEM allocator + UMMA issuer (likewise)
 //   warps 2..9  epilogue: warp w drains TMEM lanes 32*(w%4)..+31 (= tile rows); the two warps
 //               on a lane quarter take alternate 32-column chunks (one tcgen05.ld each), apply
 //               the epilogue in fp32 and store.  Two warps per row block double the loads of the
 //               residual / gate in flight, which the fp32 residual stream needs to stay hidden
 //               behind the next tile's main loop.
+//   warps 10, 11  with adapters (lora.cu): look through the up-projection tiles for non-finite weights
 #include <atomic>
 
 #include "common.cuh"
