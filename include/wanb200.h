@@ -104,7 +104,8 @@ int wanb200_gemm_bf16(const wanb200_gemm_params* p, void* stream);
  * batch, rows in any order (rows of one adapter next to each other cost least).  The update joins
  * the accumulators before the epilogue (bias, GELU, gate, residual); all epilogues but SUMSQ and
  * SCATTER.  The rank-wide intermediate is held in bf16, or for fp32 outputs in three bf16 planes
- * (24 significant bits, those of fp32).  NaN or infinite weights of an adapter reach the rows that use it only.
+ * (24 significant bits, those of fp32); sums over K for fp32 outputs are carried in fp32 from run to run of
+ * 512 values, as the tensor core does not round but cut (1e-6 off at most, 4e-6 at K = 4096 otherwise).  NaN or infinite weights of an adapter reach the rows that use it only.
  * An id >= adapters counts as none and sets the device error word to 502.  d must not overlap a (it
  * may alias residual); tile_n does not act on calls of up to 16 rows, which read w once with other
  * kernels and keep the intermediate in fp32.

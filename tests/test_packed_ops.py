@@ -943,6 +943,28 @@ def test_lora_linear_fp32_output_keeps_the_intermediate(M, K, r, N, order, word)
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N,n,r", [(9, 4096, 96, 3, 16), (150, 4096, 160, 3, 16), (300, 8192, 96, 4, 64), (1300, 4096, 1056, 4, 64),
+                                       (5000, 4096, 512, 16, 16), (2600, 2048, 2048, 2, 8)])
+@pytest.mark.parametrize("order", ["mixed", "sorted"])
+def test_lora_linear_fp32_output_over_long_sums(M, K, N, n, r, order, word):
+    """The tensor core cuts a sum off at each of its steps of 16 K values: a step of fp32 is 2^-24 to 2^-23 of the
+    sum so far (0.72 x 2^-23 on average), half of it is cut on average, and the sum so far is 2/3 of the run's end
+    (it grows with the root of its length).  A run of 512 values is thus short by 32 x 2/3 x 0.36 x 2^-23 = 9.2e-7,
+    and so is the whole, a sum of runs (one sum over K = 4096 is short by 8 times that)."""
+    x, w, b, down, up, ids, scales = lora_case(M, K, N, n, r, 240, order)
+    y = x.double() @ w.double().t() + b.double()
+    for a in range(n):
+        on = ids == a
+        y[on] += scales[a].double() * (x[on].double() @ down[a].double().t()) @ up[:, a].double().t()
+    res = torch.randn(M, N, device=DEV)
+    for kw, ref in ((dict(epilogue=L.EPI_BIAS), y), (dict(epilogue=L.EPI_BIAS_RES, residual=res), y + res.double())):
+        got = ops.lora_linear(x, w, b, down, up, ids, scales=scales, out=torch.empty(M, N, device=DEV), **kw)
+        assert float((got.double() - ref).norm() / ref.norm()) < 1e-6
+        # none of it is lost to the order of the runs: the same bits again
+        assert torch.equal(got, ops.lora_linear(x, w, b, down, up, ids, scales=scales, out=torch.empty(M, N, device=DEV), **kw))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("order", ["mixed", "one"])
 @pytest.mark.parametrize("f32", [False, True])
 @pytest.mark.parametrize("M,K,r", [(9, 128, 16), (150, 128, 16), (150, 128, 24), (260, 2048, 16)])

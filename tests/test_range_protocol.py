@@ -215,7 +215,7 @@ def test_what_the_launch_before_writes_is_read_with_plain_loads():
     inputs = {
         "attn_range.cu": {"a.lo", "a.hi", "a.pos", "a.slopes", "a.table", "p.a.table", "a.q"},
         "lora.cu": {"a.ids", "a.scales", "xp", "dp", "x0", "x1", "up"},
-        "gemm.cu": {"a.bias", "a.gate_mod", "a.gate_e0", "lo->ids", "bp", "mp", "ep"},
+        "gemm.cu": {"a.bias", "a.gate_mod", "a.gate_e0", "gate_row", "lo->ids", "bp", "mp", "ep"},
     }
     for name, allowed in inputs.items():
         with open(os.path.join(csrc, name)) as f:

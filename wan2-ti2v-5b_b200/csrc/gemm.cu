@@ -149,8 +149,7 @@ __device__ __forceinline__ void residual_values(const GemmArgs& a, const uint4 (
 }
 
 template <int EPI>
-__device__ __forceinline__ void gemm_epilogue_chunk(const GemmArgs& a, float* v, int row, int col0,
-                                                    const uint4 (&res)[8], const float* gate_row) {
+__device__ __forceinline__ void bias_and_activation(const GemmArgs& a, float* v, int col0) {
   if constexpr (EPI != WANB200_EPI_NONE && EPI != WANB200_EPI_SCATTER) {
     const uint4* bp = reinterpret_cast<const uint4*>(a.bias + col0);
 #pragma unroll
@@ -169,6 +168,12 @@ __device__ __forceinline__ void gemm_epilogue_chunk(const GemmArgs& a, float* v,
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = silu(v[i]);
   }
+}
+
+template <int EPI>
+__device__ __forceinline__ void gemm_epilogue_chunk(const GemmArgs& a, float* v, int row, int col0,
+                                                    const uint4 (&res)[8], const float* gate_row) {
+  bias_and_activation<EPI>(a, v, col0);
   if constexpr (EPI == WANB200_EPI_BIAS_GATE_RES || EPI == WANB200_EPI_BIAS_RES) {
     if (row < a.M) {
       float r[32];
@@ -260,10 +265,10 @@ __device__ __noinline__ float lora_slow_value(const LoraPlan* lo, int row, int c
 
 // The whole epilogue of a tile that has such weights, value by value, for the warp on lane quarter
 // `quad` that takes the 32-column chunks half, half + 2, ...  A function of its own, so that nothing
-// of it burdens the registers of the ordinary epilogue.
+// of it burdens the registers of the ordinary epilogue.  has_residual: the accumulator has it already.
 template <int EPI>
 __device__ __noinline__ void lora_slow_tile(const GemmArgs* ap, const LoraPlan* lo, uint32_t t_row, int m0, int n0, int quad,
-                                            int half, int lane) {
+                                            int half, int lane, bool has_residual) {
   const GemmArgs& a = *ap;
   const int row = m0 + quad * 32 + lane;
   for (int c = half; c < a.bn / 32; c += 2) {
@@ -279,7 +284,7 @@ __device__ __noinline__ void lora_slow_tile(const GemmArgs* ap, const LoraPlan* 
       if constexpr (EPI != WANB200_EPI_NONE) x += __bfloat162float(a.bias[n]);
       if constexpr (EPI == WANB200_EPI_BIAS_GELU) x = gelu_tanh(x);
       if constexpr (EPI == WANB200_EPI_BIAS_SILU) x = silu(x);
-      if constexpr (epi_has_residual(EPI)) {
+      if (epi_has_residual(EPI) && !has_residual) {
         const int64_t at = (int64_t)row * a.ldr + n;
         const float r = a.res_f32 ? static_cast<const float*>(a.residual)[at]
                                   : __bfloat162float(static_cast<const __nv_bfloat16*>(a.residual)[at]);
@@ -461,9 +466,110 @@ __device__ __forceinline__ void residual_tile_staged(const GemmArgs& a, float* s
   }
 }
 
+// What an epilogue warp holds of a tile in registers: chunk half + 2 i of its lane's row in sum[i].  To and from
+// memory it goes along rows through the warp's staging buffer, as in residual_tile_staged: a row a lane costs 32
+// lines for each 16-byte access, 8192 cycles for a tile of 128 x 256, a quarter of its MMAs' time (bias 511 -> 465 us).
+__device__ __forceinline__ float4 lora_residual4(const GemmArgs& a, int64_t at) {
+  if (a.res_f32) return *reinterpret_cast<const float4*>(static_cast<const float*>(a.residual) + at);
+  const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(a.residual) + at);
+  return make_float4(bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y));
+}
+
+__device__ __forceinline__ void lora_add_residual(const GemmArgs& a, float* stg, float (&sum)[32], int m0, int col0, int quad,
+                                                  int lane) {
+  const int sub = lane >> 3, cg = lane & 7;
+  if (col0 >= a.N) return;  // warp-uniform
+#pragma unroll
+  for (int k0 = 0; k0 < 8; k0 += 4) {
+    float4 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int row = m0 + quad * 32 + 4 * (k0 + k) + sub;
+      x[k] = row < a.M ? lora_residual4(a, (int64_t)row * a.ldr + col0 + 4 * cg) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int rl = 4 * (k0 + k) + sub;
+      *reinterpret_cast<float4*>(stg + rl * 32 + ((cg ^ (rl & 7)) << 2)) = x[k];
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const float4 v = *reinterpret_cast<const float4*>(stg + lane * 32 + ((q ^ (lane & 7)) << 2));
+    sum[4 * q] += v.x, sum[4 * q + 1] += v.y, sum[4 * q + 2] += v.z, sum[4 * q + 3] += v.w;
+  }
+  __syncwarp();  // the staging buffer is rewritten by the next chunk
+}
+
+// The gated residual is read here: a gate in front of it leaves no place for it in the sums.
+template <int EPI>
+__device__ __forceinline__ void lora_store_sums(const GemmArgs& a, float* stg, float (&sum)[4][32], int m0, int n0, int quad,
+                                                int half, int lane) {
+  constexpr bool GATE = EPI == WANB200_EPI_BIAS_GATE_RES;
+  const int sub = lane >> 3, cg = lane & 7;
+  const float* gate_row = nullptr;
+  if constexpr (GATE) {
+    const int row = m0 + quad * 32 + lane;
+    gate_row = a.gate_e0 + (row < a.M ? frame_of_row(row, a.rows_per_seq, a.row_offset, a.seq_len, a.tokens_per_frame) : 0) * a.gate_frame_stride;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = half + 2 * i, col0 = n0 + c * 32;
+    if (c >= a.bn / 32 || col0 >= a.N) continue;  // warp-uniform
+    bias_and_activation<EPI>(a, sum[i], col0);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      if constexpr (GATE) {
+        const float4 e = __ldg(reinterpret_cast<const float4*>(gate_row + col0 + 4 * q));
+        const uint2 gu = __ldg(reinterpret_cast<const uint2*>(a.gate_mod + col0 + 4 * q));
+        sum[i][4 * q] *= bf16_lo(gu.x) + e.x;
+        sum[i][4 * q + 1] *= bf16_hi(gu.x) + e.y;
+        sum[i][4 * q + 2] *= bf16_lo(gu.y) + e.z;
+        sum[i][4 * q + 3] *= bf16_hi(gu.y) + e.w;
+      }
+      *reinterpret_cast<float4*>(stg + lane * 32 + ((q ^ (lane & 7)) << 2)) =
+          make_float4(sum[i][4 * q], sum[i][4 * q + 1], sum[i][4 * q + 2], sum[i][4 * q + 3]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int k0 = 0; k0 < 8; k0 += 4) {
+      float4 x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int row = m0 + quad * 32 + 4 * (k0 + k) + sub;
+        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (GATE && row < a.M) x[k] = lora_residual4(a, (int64_t)row * a.ldr + col0 + 4 * cg);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int rl = 4 * (k0 + k) + sub, row = m0 + quad * 32 + rl;
+        float4 v = *reinterpret_cast<const float4*>(stg + rl * 32 + ((cg ^ (rl & 7)) << 2));
+        if constexpr (GATE) v = make_float4(x[k].x + v.x, x[k].y + v.y, x[k].z + v.z, x[k].w + v.w);
+        if (row < a.M) *reinterpret_cast<float4*>(static_cast<float*>(a.d) + (int64_t)row * a.ldd + col0 + 4 * cg) = v;
+      }
+    }
+    __syncwarp();
+  }
+}
+
 // The kernel's body.  LORA: a tile's K loop goes on with the adapter steps that its rows use (h
 // through tmH, the up-projection columns through tmU), 64 columns per ring stage.
-template <int EPI, bool LORA>
+//
+// kLoraRuns (fp32 outputs): the tensor core cuts its sums off instead of rounding them, which shrinks a sum
+// over K = 4096 by 4e-6.  So the MMAs run over LORA_RUN stages at a time, in the two accumulators in turn,
+// and the epilogue warps add the runs up in fp32 registers (128 a thread, two warps on each of 128 rows): 4.7e-6
+// -> 6.4e-7 off.  The next tile's MMAs are no more than two runs ahead, so what an epilogue waits for is not
+// hidden behind a whole tile: the residual is added a chunk behind each of the first runs (a gated one is
+// brought to the L2), and the sums go from the registers to the output with both accumulators free.  Only a tile
+// with non-finite weights and K shared by a cluster put the sums back into the tile's last accumulator.
+// Measured, 15708 x 4096 x 4096 with 4 adapters of rank 64 (us, one run / runs): bias 437-465 / 465-475, residual
+// 436-450 / 509-524, gated residual 463 / 556.  With the whole residual loaded in front of the first run 530;
+// with the sums back in the accumulator and the ordinary epilogue 624, gated 665.
+enum GemmLora : int { kLoraNone = 0, kLoraOneRun = 1, kLoraRuns = 2 };
+constexpr int kLoraBad = 1, kLoraLast = 2;  // what the MMA warp says of an accumulator
+
+template <int EPI, int LORA>
 __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap* tmH,
                                           const CUtensorMap* tmU, const GemmArgs& args, const LoraPlan* lora) {
   extern __shared__ uint8_t smem_raw[];
@@ -489,7 +595,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       mbar_init(empty0 + 8 * s, 1);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(tfull0 + 8 * b, LORA ? 2 : 1);  // LORA: the MMA commit, and its thread once tile_bad is written
+      mbar_init(tfull0 + 8 * b, LORA ? 2 : 1);  // LORA: the MMA commit, and its thread once lora_said is written
       mbar_init(tempty0 + 8 * b, 32 * G_EPI_WARPS);
     }
     mbar_init(done_bar, 1);
@@ -505,10 +611,10 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
     tmem_relinquish();
   }
   // LORA: u_ok[stage] says that the stage's up-projection tile was looked through; bad[stage] by
-  // which of the two checking warps found something; tile_bad: the tile of an accumulator had some
+  // which of the two checking warps found something; said: of both accumulators, then of a cluster's one tile
   __shared__ uint64_t lora_ok_bar[LORA ? 2 * G_MAX_STAGES : 1];  // u_ok, u_req
   __shared__ int lora_bad[LORA ? 2 * G_MAX_STAGES : 1];
-  __shared__ int lora_tile_bad[LORA ? 2 : 1];
+  __shared__ int lora_said[LORA ? 3 : 1];
   const uint32_t u_ok0 = smem_u32(lora_ok_bar), u_req0 = u_ok0 + 8 * G_MAX_STAGES;
   if constexpr (LORA) {
     if (threadIdx.x == 0) {
@@ -614,18 +720,43 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       for (int tile = tile0; ok && tile < num_tiles; tile += tile_step) {
         if (!mbar_wait_warp(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag, err, kErrTimeoutGemmMma)) break;
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * GBN;
+        uint32_t d_tmem = tmem_base + acc * GBN;
+        [[maybe_unused]] int used = 0;  // stages of this run
+        // a full run is handed over; the next one goes to the other accumulator
+        [[maybe_unused]] auto next_run = [&]() -> bool {
+          if (lane == 0) {
+            lora_said[acc] = 0;
+            mbar_arrive(tfull0 + 8 * acc);
+          }
+          __syncwarp();
+          if (elect_one()) umma_commit(tfull0 + 8 * acc);
+          __syncwarp();
+          acc ^= 1;
+          if (acc == 0) acc_phase ^= 1;
+          used = 0;
+          d_tmem = tmem_base + acc * GBN;
+          const bool free = mbar_wait_warp(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag, err, kErrTimeoutGemmMma);
+          tc_fence_after();
+          return free;
+        };
         for (int kb = 0; kb < kblocks; ++kb) {
+          if constexpr (LORA == kLoraRuns) {
+            if (used == LORA_RUN && !next_run()) {
+              ok = false;
+              break;
+            }
+          }
           if (!mbar_wait_warp(full0 + 8 * stage, phase, abort_flag, err, kErrTimeoutGemmMma)) {
             ok = false;
             break;
           }
           tc_fence_after();
           const uint32_t a_lo = tiles_lo + stage * (SB >> 4);
+          const int before = LORA == kLoraRuns ? used++ : kb;
           if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < GBK / 16; ++kk)
-              umma_bf16_w(d_tmem, a_lo + kk * 2, a_lo + (G_A_BYTES >> 4) + kk * 2, sw128_hi(1024), idesc, (kb | kk) != 0);
+              umma_bf16_w(d_tmem, a_lo + kk * 2, a_lo + (G_A_BYTES >> 4) + kk * 2, sw128_hi(1024), idesc, (before | kk) != 0);
             umma_commit(empty0 + 8 * stage);
           }
           __syncwarp();
@@ -644,6 +775,12 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
             const uint32_t steps = lora_chunk_steps(mask, c);
             if (!steps || n++ % lora->ksplit != krank) continue;
             for (int pl = 0; pl < lora->planes; ++pl) {
+              if constexpr (LORA == kLoraRuns) {
+                if (used == LORA_RUN && !next_run()) {
+                  ok = false;
+                  break;
+                }
+              }
               if (!mbar_wait_warp(full0 + 8 * stage, phase, abort_flag, err, kErrTimeoutGemmMma) ||
                   (mixed && !mbar_wait_warp(u_ok0 + 8 * stage, (u_ok_ph >> stage) & 1, abort_flag, err, kErrTimeoutGemmMma))) {
                 ok = false;
@@ -655,11 +792,14 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
               }
               tc_fence_after();
               const uint32_t a_lo = tiles_lo + stage * (SB >> 4);
+              bool add = LORA != kLoraRuns || used++ != 0;
               if (elect_one()) {
 #pragma unroll
                 for (int kk = 0; kk < LORA_CHUNK / LORA_STEP; ++kk)
-                  if ((steps >> kk) & 1u)
-                    umma_bf16_w(d_tmem, a_lo + kk * 2, a_lo + (G_A_BYTES >> 4) + kk * 2, sw128_hi(1024), idesc, true);
+                  if ((steps >> kk) & 1u) {
+                    umma_bf16_w(d_tmem, a_lo + kk * 2, a_lo + (G_A_BYTES >> 4) + kk * 2, sw128_hi(1024), idesc, add);
+                    add = true;
+                  }
                 umma_commit(empty0 + 8 * stage);
               }
               __syncwarp();
@@ -669,7 +809,10 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
               }
             }
           }
-          if (lane == 0) lora_tile_bad[acc] = bad;
+          if (lane == 0) {
+            lora_said[acc] = (bad ? kLoraBad : 0) | kLoraLast;
+            if (lora->ksplit > 1) lora_said[2] = bad;
+          }
         }
         if (!ok) break;
         if constexpr (LORA) {
@@ -737,8 +880,72 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int tile = tile0; tile < num_tiles; tile += tile_step) {
-      const bool done = mbar_wait_warp(tfull0 + 8 * acc, acc_phase, abort_flag, err, kErrTimeoutGemmEpilogue);
-      tc_fence_after();
+      // the residual joins the sums (the first rank's, where a cluster shares K), a chunk behind each run
+      constexpr bool HAS_RESIDUAL = LORA == kLoraRuns && EPI == WANB200_EPI_BIAS_RES;
+      bool done;
+      if constexpr (LORA == kLoraRuns) {
+        int m0, n0;
+        tile_origin(tile, num_m, num_n, bn, m0, n0);
+        float sum[4][32];
+        float* stg = reinterpret_cast<float*>(smem + args.tiles_bytes + GemmCfg<EPI>::STAGING) + (warp - 2) * 1024;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) sum[i][j] = 0.f;
+        bool in_registers = false;
+        for (int n = 0;; ++n) {
+          done = mbar_wait_warp(tfull0 + 8 * acc, acc_phase, abort_flag, err, kErrTimeoutGemmEpilogue);
+          if (!done) break;
+          tc_fence_after();
+          const uint32_t t_run = tmem_base + (uint32_t(quad * 32) << 16) + acc * GBN + half * 32;
+          const int said = *reinterpret_cast<volatile int*>(lora_said + acc);
+          if (!HAS_RESIDUAL && n == 0 && (said & kLoraLast)) break;  // the only run lies where the epilogue looks for it
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (half + 2 * i < bn / 32) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 16) {
+                uint32_t v[16];
+                tmem_ld16(t_run + i * 64 + j, v);
+#pragma unroll
+                for (int q = 0; q < 16; ++q) sum[i][j + q] += __uint_as_float(v[q]);
+              }
+            }
+          in_registers = said == kLoraLast && lora->ksplit == 1;
+          if (!(said & kLoraLast) || in_registers) {
+            tc_fence_before();
+            mbar_arrive(tempty0 + 8 * acc);
+          }
+          if constexpr (HAS_RESIDUAL) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if ((i == n || (i > n && (said & kLoraLast))) && half + 2 * i < bn / 32 && krank == 0)
+                lora_add_residual(args, stg, sum[i], m0, n0 + (half + 2 * i) * 32, quad, lane);
+          }
+          if constexpr (EPI == WANB200_EPI_BIAS_GATE_RES) {  // to the L2, in time for lora_store_sums
+            const int c = half + 2 * n, es = args.res_f32 ? 4 : 2;
+            if (c < bn / 32 && m0 + r < args.M && n0 + c * 32 < args.N)
+              asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(args.residual) +
+                                                            ((int64_t)(m0 + r) * args.ldr + n0 + c * 32) * es));
+          }
+          if ((said & kLoraLast) && !in_registers) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (half + 2 * i < bn / 32) tmem_st32(t_run + i * 64, sum[i]);
+            break;
+          }
+          acc ^= 1;
+          if (acc == 0) acc_phase ^= 1;
+          if (in_registers) break;
+        }
+        if (in_registers) {
+          lora_store_sums<HAS_RESIDUAL ? WANB200_EPI_BIAS : EPI>(args, stg, sum, m0, n0, quad, half, lane);
+          continue;
+        }
+      } else {
+        done = mbar_wait_warp(tfull0 + 8 * acc, acc_phase, abort_flag, err, kErrTimeoutGemmEpilogue);
+        tc_fence_after();
+      }
       const uint32_t t_row = tmem_base + (uint32_t(quad * 32) << 16) + acc * GBN;
       if constexpr (LORA) {
         if (lora->ksplit > 1) {
@@ -756,9 +963,9 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
             int m0, n0;
             tile_origin(tile, num_m, num_n, bn, m0, n0);
             int bad = 0;
-            for (int k = 0; k < lora->ksplit; ++k) bad |= ld_cluster_int(smem_u32(lora_tile_bad), k);
-            lora_join_rows<EPI>(args, lora, tiles, bad != 0, m0, n0, krank,
-                                (warp - 2) * 32 + lane);
+            for (int k = 0; k < lora->ksplit; ++k) bad |= ld_cluster_int(smem_u32(lora_said + 2), k);
+            lora_join_rows<HAS_RESIDUAL ? WANB200_EPI_BIAS : EPI>(args, lora, tiles, bad != 0, m0, n0, krank,
+                                                                  (warp - 2) * 32 + lane);
           }
           break;  // a cluster has one tile
         }
@@ -769,10 +976,11 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       const int row = m0 + r;
       bool slow = false;
       if constexpr (LORA) {
-        slow = *reinterpret_cast<volatile int*>(lora_tile_bad + acc) != 0;
-        if (slow) lora_slow_tile<EPI>(&args, lora, t_row, m0, n0, quad, half, lane);
+        slow = *reinterpret_cast<volatile int*>(lora_said + acc) & kLoraBad;
+        if (slow) lora_slow_tile<EPI>(&args, lora, t_row, m0, n0, quad, half, lane, HAS_RESIDUAL);
       }
       if (slow) {  // done above
+      } else if constexpr (HAS_RESIDUAL) {  // has gone out of the registers
       } else if constexpr (EPI == WANB200_EPI_SCATTER) {
         // stage this warp's 32 rows (lane = row), then write each row as one 512-byte segment
         // (the first warp of each lane quarter does the whole tile; the second only arrives)
@@ -798,7 +1006,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
                 *reinterpret_cast<const uint4*>(stg + rr * SR + lane * 16);
         }
         __syncwarp();
-      } else if (epi_has_residual(EPI) && args.res_staging) {
+      } else if (epi_has_residual(EPI) && args.res_staging && args.res_f32) {
         if constexpr (epi_has_residual(EPI)) {
           float* stg = reinterpret_cast<float*>(smem + args.tiles_bytes + GemmCfg<EPI>::STAGING) + (warp - 2) * 1024;
           residual_tile_staged<EPI>(args, stg, t_row, m0, n0, quad, half, lane);
@@ -851,27 +1059,27 @@ template <int EPI>
 __global__ void __launch_bounds__(G_THREADS, 1)
     gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const GemmArgs args) {
-  gemm_body<EPI, false>(tmA, tmB, nullptr, nullptr, args, nullptr);
+  gemm_body<EPI, kLoraNone>(tmA, tmB, nullptr, nullptr, args, nullptr);
 }
 
-template <int EPI>
+template <int EPI, int LORA>
 __global__ void __launch_bounds__(G_LORA_THREADS, 1)
     gemm_lora_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmU,
                      const __grid_constant__ GemmArgs args, const __grid_constant__ LoraPlan lora) {
-  gemm_body<EPI, true>(tmA, tmB, &tmH, &tmU, args, &lora);
+  gemm_body<EPI, LORA>(tmA, tmB, &tmH, &tmU, args, &lora);
 }
 
 // ------------------------------------------------------------------ host launcher
-template <int EPI>
-static int launch_gemm_lora(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& th, const CUtensorMap& tu,
-                            const GemmArgs& ga, const LoraPlan& lora, int grid, cudaStream_t st) {
+template <int EPI, int LORA>
+static int launch_gemm_lora_form(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& th, const CUtensorMap& tu,
+                                 const GemmArgs& ga, const LoraPlan& lora, int grid, cudaStream_t st) {
   static std::atomic<bool> attr_set[kMaxDevices] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= kMaxDevices) return set_error(WANB200_EINVAL, "device index out of range");
   if (!attr_set[dev].load(std::memory_order_acquire)) {
-    cudaError_t e = cudaFuncSetAttribute(gemm_lora_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(gemm_lora_kernel<EPI, LORA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          G_SMEM_LIMIT - G_LORA_SMEM);
     if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute(gemm_lora)", e);
     attr_set[dev].store(true, std::memory_order_release);
@@ -891,9 +1099,16 @@ static int launch_gemm_lora(const CUtensorMap& ta, const CUtensorMap& tb, const 
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = lora.ksplit > 1 ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_lora_kernel<EPI>, ta, tb, th, tu, ga, lora);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_lora_kernel<EPI, LORA>, ta, tb, th, tu, ga, lora);
   if (e != cudaSuccess) return set_cuda_error("gemm_lora_kernel launch", e);
   return WANB200_OK;
+}
+
+template <int EPI>
+static int launch_gemm_lora(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& th, const CUtensorMap& tu,
+                            const GemmArgs& ga, const LoraPlan& lora, int grid, cudaStream_t st) {
+  return ga.out_f32 ? launch_gemm_lora_form<EPI, kLoraRuns>(ta, tb, th, tu, ga, lora, grid, st)
+                    : launch_gemm_lora_form<EPI, kLoraOneRun>(ta, tb, th, tu, ga, lora, grid, st);
 }
 
 template <int EPI>
@@ -1038,7 +1253,10 @@ int gemm_launch(const wanb200_gemm_params* p, const LoraPlan* lora, int* err, cu
     // ring depth as it is (measured at 15708 x 3072 x 3072: +6% GATE_RES, +10% RES; on 128-wide
     // tiles it lost 0-5%, so narrower tiles keep one row per lane)
     ga.res_staging = 0;
-    if ((epi == WANB200_EPI_BIAS_GATE_RES || epi == WANB200_EPI_BIAS_RES) && ga.res_f32 && ga.out_f32 &&
+    if (lora && ga.out_f32) {
+      ga.res_staging = G_RES_STAGING;  // every tile of sums goes through it; narrow ones give a stage for it
+      ga.stages = std::min<int>(G_MAX_STAGES, (G_SMEM_LIMIT - fixed - G_RES_STAGING) / (int)ga.stage_bytes);
+    } else if ((epi == WANB200_EPI_BIAS_GATE_RES || epi == WANB200_EPI_BIAS_RES) && ga.res_f32 && ga.out_f32 &&
         bn == GBN &&
         std::min<int>(G_MAX_STAGES, (G_SMEM_LIMIT - fixed - G_RES_STAGING) / (int)ga.stage_bytes) == ga.stages)
       ga.res_staging = G_RES_STAGING;

@@ -15,7 +15,7 @@
 namespace wanb200 {
 
 constexpr int LD_THREADS = 192;  // TMA, MMA, 4 epilogue warps
-constexpr int LD_BM = 128, LD_BK = 64, LD_GROUP = 4;  // chunks of one pass: N = 256
+constexpr int LD_BM = 128, LD_BK = 64, LD_GROUP = 4, LD_GROUP_F32 = 2;  // chunks of one pass
 constexpr int LD_STAGES = 4;
 constexpr int LD_STAGE_BYTES = LD_BM * LD_BK * 2 + LD_GROUP * LORA_CHUNK * LD_BK * 2;  // 48 KB
 constexpr int LD_RED_LD = LD_GROUP * LORA_CHUNK + 4;  // fp32 row of the partial sums, padded against bank conflicts
@@ -65,11 +65,16 @@ __device__ __forceinline__ void lora_store_h(const LoraDownArgs& a, int row, int
 // fill the SMs): x tile x the tile's used chunks of A, up to four (N = 256) in one pass over x.  The
 // read of x bounds it; with few row tiles the split of K brings enough SMs to the read.  The
 // partial sums meet in the cluster's shared memory, each block adding its share of the rows.
+// F32 (fp32 outputs): two chunks a pass, their sums over runs of LORA_RUN K blocks in two accumulators
+// in turn, added up in fp32 registers, since the tensor core cuts sums off (as in gemm.cu).
+template <bool F32>
 __global__ void __launch_bounds__(LD_THREADS, 1)
     lora_down_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmD,
                      const __grid_constant__ LoraDownArgs a) {
+  constexpr int GROUP = F32 ? LD_GROUP_F32 : LD_GROUP, ACCS = F32 ? 2 : 1, ACC_COLS = GROUP * LORA_CHUNK;
+  constexpr int RUN = F32 ? LORA_RUN : 1 << 30;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bars[2 * LD_STAGES + 3];
+  __shared__ uint64_t bars[2 * LD_STAGES + 2 * ACCS + 1];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   __shared__ uint32_t bits[LORA_MASK_WORDS];
@@ -80,8 +85,8 @@ __global__ void __launch_bounds__(LD_THREADS, 1)
   const int krank = blockIdx.x, ksize = gridDim.x, m0 = blockIdx.y * LD_BM;
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sbase = smem_u32(smem);
-  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * LD_STAGES, tfull = empty0 + 8 * LD_STAGES;
-  const uint32_t tempty = tfull + 8, done_bar = tfull + 16;
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * LD_STAGES, tfull0 = empty0 + 8 * LD_STAGES;
+  const uint32_t tempty0 = tfull0 + 8 * ACCS, done_bar = tempty0 + 8 * ACCS;
   volatile int* abort_flag = &abort_word;
   int* err = a.err;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -92,8 +97,10 @@ __global__ void __launch_bounds__(LD_THREADS, 1)
       mbar_init(full0 + 8 * s, 1);
       mbar_init(empty0 + 8 * s, 1);
     }
-    mbar_init(tfull, 1);
-    mbar_init(tempty, 128);
+    for (int b = 0; b < ACCS; ++b) {
+      mbar_init(tfull0 + 8 * b, 1);
+      mbar_init(tempty0 + 8 * b, 128);
+    }
     mbar_init(done_bar, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -103,7 +110,7 @@ __global__ void __launch_bounds__(LD_THREADS, 1)
     tma_prefetch_desc(&tmD);
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(&tmem_slot), LD_GROUP * LORA_CHUNK);
+    tmem_alloc(smem_u32(&tmem_slot), ACCS * ACC_COLS);
     tmem_relinquish();
   }
   __syncthreads();
@@ -143,12 +150,12 @@ __global__ void __launch_bounds__(LD_THREADS, 1)
   __syncthreads();
   const uint32_t tmem_base = tmem_slot;
   const int kb0 = krank * a.kblocks_per_rank, kblocks = min(a.K / LD_BK - kb0, a.kblocks_per_rank);  // >= 1 (host)
-  const int passes = (num_chunks + LD_GROUP - 1) / LD_GROUP;
+  const int passes = (num_chunks + GROUP - 1) / GROUP;
   uint32_t ph = 0, issued = 0, last_ph = 0;  // ring phases, per role
-  int stage = 0;
+  int stage = 0, run = 0;                    // run: of all passes, counted by the MMA warp and the epilogue
 
   for (int pass = 0; pass < passes; ++pass) {
-    const int c0 = pass * LD_GROUP, nc = min(LD_GROUP, num_chunks - c0);
+    const int c0 = pass * GROUP, nc = min(GROUP, num_chunks - c0);
     // (the whole warp walks the issue loops: see elect_one)
     if (warp == 0) {
       for (int kb = 0; kb < kblocks; ++kb) {
@@ -168,52 +175,92 @@ __global__ void __launch_bounds__(LD_THREADS, 1)
       }
     } else if (warp == 1) {
       const uint32_t idesc = idesc_bf16_f32(LD_BM, nc * LORA_CHUNK, false, false);
-      bool ok = mbar_wait_warp(tempty, (pass & 1) ^ 1, abort_flag, err, kErrTimeoutGemmMma);
-      tc_fence_after();
-      for (int kb = 0; ok && kb < kblocks; ++kb) {
-        ok = mbar_wait_warp(full0 + 8 * stage, ph, abort_flag, err, kErrTimeoutGemmMma);
-        if (!ok) break;
+      bool ok = true;
+      for (int r0 = 0; ok && r0 < kblocks; r0 += RUN, ++run) {
+        const int acc = run % ACCS;
+        const uint32_t d_tmem = tmem_base + acc * ACC_COLS;
+        ok = mbar_wait_warp(tempty0 + 8 * acc, ((run / ACCS) & 1) ^ 1, abort_flag, err, kErrTimeoutGemmMma);
         tc_fence_after();
-        const uint32_t x_lo = sw128_lo(sbase, 16) + stage * (LD_STAGE_BYTES >> 4), d_lo = x_lo + (LD_BM * LD_BK * 2 >> 4);
-        if (elect_one()) {
+        for (int kb = r0; ok && kb < min(kblocks, r0 + RUN); ++kb) {
+          ok = mbar_wait_warp(full0 + 8 * stage, ph, abort_flag, err, kErrTimeoutGemmMma);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t x_lo = sw128_lo(sbase, 16) + stage * (LD_STAGE_BYTES >> 4), d_lo = x_lo + (LD_BM * LD_BK * 2 >> 4);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < LD_BK / 16; ++kk)
-            umma_bf16_w(tmem_base, x_lo + kk * 2, d_lo + kk * 2, sw128_hi(1024), idesc, (kb | kk) != 0);
-          umma_commit(empty0 + 8 * stage);
+            for (int kk = 0; kk < LD_BK / 16; ++kk)
+              umma_bf16_w(d_tmem, x_lo + kk * 2, d_lo + kk * 2, sw128_hi(1024), idesc, ((kb - r0) | kk) != 0);
+            umma_commit(empty0 + 8 * stage);
+          }
+          __syncwarp();
+          if (++stage == LD_STAGES) stage = 0, ph ^= 1;
         }
+        if (ok && elect_one()) umma_commit(tfull0 + 8 * acc);
         __syncwarp();
-        if (++stage == LD_STAGES) stage = 0, ph ^= 1;
       }
-      if (ok && elect_one()) umma_commit(tfull);
-      __syncwarp();
     } else {
       const int quad = warp & 3, r = quad * 32 + lane, row = m0 + r;
       const int id = ids[r];
       const int first = id < 0 ? 0 : id * a.rank, last = id < 0 ? 0 : first + a.rank;
       const float scale = id >= 0 && a.scales ? __ldg(a.scales + id) : 1.f;
-      const bool ok = mbar_wait_warp(tfull, pass & 1, abort_flag, err, kErrTimeoutGemmEpilogue);
-      if (ok) {
-        tc_fence_after();
-        for (int c = 0; c < nc * 2; ++c) {
-          float v[32];
-          tmem_ld32(tmem_base + (uint32_t(quad * 32) << 16) + c * 32, v);
-          if (ksize == 1) {
-            if (row < a.M) {
-              const int col = chunks[c0 + (c >> 1)] * LORA_CHUNK + (c & 1) * 32;
+      // 32 columns from c * 32 on: h, or this block's part of it
+      auto put = [&](int c, const float (&v)[32]) {
+        if (ksize == 1) {
+          if (row < a.M) {
+            const int col = chunks[c0 + (c >> 1)] * LORA_CHUNK + (c & 1) * 32;
 #pragma unroll
-              for (int q = 0; q < 8; ++q)
-                lora_store_h(a, row, col + 4 * q, make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]), first, last,
-                             scale);
+            for (int q = 0; q < 8; ++q)
+              lora_store_h(a, row, col + 4 * q, make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]), first, last,
+                           scale);
+          }
+        } else {  // the ring is free: every MMA of the pass has completed
+          float4* red = reinterpret_cast<float4*>(smem + (r * LD_RED_LD + c * 32) * 4);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) red[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        }
+      };
+      const uint32_t t_row = tmem_base + (uint32_t(quad * 32) << 16);
+      if constexpr (F32) {
+        float sum[2 * GROUP][32];
+#pragma unroll
+        for (int c = 0; c < 2 * GROUP; ++c)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) sum[c][j] = 0.f;
+        bool ok = true;
+        for (int r0 = 0; ok && r0 < kblocks; r0 += RUN, ++run) {
+          const int acc = run % ACCS;
+          ok = mbar_wait_warp(tfull0 + 8 * acc, (run / ACCS) & 1, abort_flag, err, kErrTimeoutGemmEpilogue);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < 2 * GROUP; ++c)
+            if (c < 2 * nc) {
+              float v[32];
+              tmem_ld32(t_row + acc * ACC_COLS + c * 32, v);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) sum[c][j] += v[j];
             }
-          } else {  // the ring is free: every MMA of the pass has completed
-            float4* red = reinterpret_cast<float4*>(smem + (r * LD_RED_LD + c * 32) * 4);
+          tc_fence_before();
+          mbar_arrive(tempty0 + 8 * acc);
+        }
+        if (ok) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) red[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          for (int c = 0; c < 2 * GROUP; ++c)
+            if (c < 2 * nc) put(c, sum[c]);
+        }
+      } else {
+        const bool ok = mbar_wait_warp(tfull0, run++ & 1, abort_flag, err, kErrTimeoutGemmEpilogue);
+        if (ok) {
+          tc_fence_after();
+          for (int c = 0; c < nc * 2; ++c) {
+            float v[32];
+            tmem_ld32(t_row + c * 32, v);
+            put(c, v);
           }
         }
+        tc_fence_before();
+        mbar_arrive(tempty0);
       }
-      tc_fence_before();
-      mbar_arrive(tempty);
     }
     if (ksize > 1) {
       cluster_sync_all();
@@ -263,7 +310,7 @@ __global__ void __launch_bounds__(LD_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem_base, LD_GROUP * LORA_CHUNK);
+  if (warp == 1) tmem_dealloc(tmem_base, ACCS * ACC_COLS);
 }
 
 // ================================================================== up to 16 rows: W is read once
@@ -597,6 +644,35 @@ static LoraLaunch lora_plan_launch(int64_t M, int64_t N, int kblocks, int tile_n
   return best;
 }
 
+template <bool F32>
+static int launch_lora_down(const CUtensorMap& tx, const CUtensorMap& td, const LoraDownArgs& a, int ksize, int64_t num_m,
+                            cudaStream_t st) {
+  static std::atomic<bool> attr_set[kMaxDevices] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= kMaxDevices) return set_error(WANB200_EINVAL, "device index out of range");
+  cudaError_t e;
+  if (!attr_set[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(lora_down_kernel<F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, LD_SMEM);
+    if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute(lora_down)", e);
+    attr_set[dev].store(true, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ksize, (unsigned)num_m);
+  cfg.blockDim = dim3(LD_THREADS);
+  cfg.dynamicSmemBytes = LD_SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ksize;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, lora_down_kernel<F32>, tx, td, a);
+  if (e != cudaSuccess) return set_cuda_error("lora_down_kernel launch", e);
+  return WANB200_OK;
+}
+
 int gemm_lora(const wanb200_lora_params* p, cudaStream_t st) {
   if (!p) return set_error(WANB200_EINVAL, "gemm_lora: null params");
   const wanb200_gemm_params* g = &p->gemm;
@@ -638,29 +714,8 @@ int gemm_lora(const wanb200_lora_params* p, cudaStream_t st) {
   const LoraLaunch pl = lora_plan_launch(g->M, g->N, a.K / LD_BK, g->tile_n, num_sms());
   const int ksize = pl.down_ksize;
   a.kblocks_per_rank = (a.K / LD_BK + ksize - 1) / ksize;
-  static std::atomic<bool> attr_set[kMaxDevices] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= kMaxDevices) return set_error(WANB200_EINVAL, "device index out of range");
-  cudaError_t e;
-  if (!attr_set[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(lora_down_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LD_SMEM);
-    if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute(lora_down)", e);
-    attr_set[dev].store(true, std::memory_order_release);
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ksize, (unsigned)l.num_m);
-  cfg.blockDim = dim3(LD_THREADS);
-  cfg.dynamicSmemBytes = LD_SMEM;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)ksize;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, lora_down_kernel, tx, td, a);
-  if (e != cudaSuccess) return set_cuda_error("lora_down_kernel launch", e);
+  rc = g->out_f32 ? launch_lora_down<true>(tx, td, a, ksize, l.num_m, st) : launch_lora_down<false>(tx, td, a, ksize, l.num_m, st);
+  if (rc) return rc;
   LoraPlan plan;
   plan.step_mask = a.step_mask;
   plan.mixed = a.mixed;

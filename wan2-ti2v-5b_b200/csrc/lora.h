@@ -9,6 +9,7 @@ namespace wanb200 {
 // The adapters' columns (adapter a, rank index i -> column a * rank + i) are handled in steps of 16,
 // the K of one tcgen05.mma, and loaded in chunks of 64, one 128-byte swizzle row.
 constexpr int LORA_STEP = 16, LORA_CHUNK = 64, LORA_MAX_COLS = 4096;
+constexpr int LORA_RUN = 8;  // ring stages (of 64 K values) of one run of sums beside an fp32 output
 constexpr int LORA_F32_PLANES = 3;  // bf16 planes of h beside an fp32 output
 constexpr int LORA_MASK_WORDS = LORA_MAX_COLS / LORA_STEP / 32;  // 8 words of step bits per row tile
 
