@@ -563,9 +563,9 @@ __device__ __forceinline__ void lora_store_sums(const GemmArgs& a, float* stg, f
 // hidden behind a whole tile: the residual is added a chunk behind each of the first runs (a gated one is
 // brought to the L2), and the sums go from the registers to the output with both accumulators free.  Only a tile
 // with non-finite weights and K shared by a cluster put the sums back into the tile's last accumulator.
-// Measured, 15708 x 4096 x 4096 with 4 adapters of rank 64 (us, one run / runs): bias 437-465 / 465-475, residual
-// 436-450 / 509-524, gated residual 463 / 556.  With the whole residual loaded in front of the first run 530;
-// with the sums back in the accumulator and the ordinary epilogue 624, gated 665.
+// Measured, 15708 x 4096 x 4096 with 4 adapters of rank 64 (us, one run / runs): bias 437-475 / 444-449, residual
+// 436-450 / 494, gated residual 463 / 556.  With the whole residual loaded in front of the first run 15 more; with
+// the sums back in the accumulator and the ordinary epilogue 110 more, gated as well.
 enum GemmLora : int { kLoraNone = 0, kLoraOneRun = 1, kLoraRuns = 2 };
 constexpr int kLoraBad = 1, kLoraLast = 2;  // what the MMA warp says of an accumulator
 
