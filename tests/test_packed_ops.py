@@ -965,6 +965,44 @@ def test_lora_linear_fp32_output_over_long_sums(M, K, N, n, r, order, word):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("epi", [L.EPI_NONE, L.EPI_BIAS_GELU, L.EPI_BIAS_SILU, L.EPI_BIAS_RES, L.EPI_BIAS_GATE_RES])
+@pytest.mark.parametrize("M,N,K,tile_n", [(2600, 1024, 1024, 0), (2500, 1056, 640, 256), (700, 544, 1024, 96), (1300, 2016, 1600, 224),
+                                          (300, 1056, 1024, 64), (700, 256, 4096, 0)])
+@pytest.mark.parametrize("broken", [False, True])
+@pytest.mark.parametrize("res_bf16", [False, True])
+def test_lora_linear_fp32_epilogues_over_several_runs(M, N, K, tile_n, epi, broken, res_bf16, word):
+    """Tiles of every width whose sums come in several runs, whole and with non-finite weights, the residual in
+    bf16, or in fp32 and overwritten by the output."""
+    residual = epi in (L.EPI_BIAS_RES, L.EPI_BIAS_GATE_RES)
+    if res_bf16 and not residual:
+        pytest.skip("no residual")
+    n, r = 5, 24
+    x, w, b, down, up, ids, scales = lora_case(M, K, N, n, r, 250, "sorted")
+    if broken:
+        up[7, 2, 3], up[40, 2, 0], down[1, 2] = math.inf, math.nan, math.nan
+    kw, rf = {}, {}
+    out = torch.empty(M, N, device=DEV)
+    if residual:
+        rf["residual"] = randn(M, N, seed=40) if res_bf16 else torch.randn(M, N, device=DEV)
+        kw["residual"] = rf["residual"].clone()
+        out = out if res_bf16 else kw["residual"]
+    if epi == L.EPI_BIAS_GATE_RES:
+        mod, e0 = randn(N, seed=41), torch.randn(7, N, device=DEV)
+        kw["gate"], kw["frames"] = (mod, e0), (M, -(-M // 7))
+        rf["gate"] = (mod.double() + e0.double())[(torch.arange(M, device=DEV) // -(-M // 7))]
+    bias = None if epi == L.EPI_NONE else b
+    got = ops.lora_linear(x, w, bias, down, up, ids, scales=scales, epilogue=epi, out=out, tile_n=tile_n, **kw)
+    clean = [torch.where(t.isfinite(), t, torch.zeros_like(t)) for t in (down, up)]
+    ref, tol = lora_ref(x, w, bias, *clean, ids, scales, epi, f32=True, **rf)
+    spared = torch.ones(M, N, dtype=torch.bool, device=DEV)
+    if broken:
+        spared[ids == 2, 7] = spared[ids == 2, 40] = False
+        spared[ids == 1] = False
+        assert not bool(got[~spared].isfinite().all())
+    within(got[spared], ref[spared], tol[spared])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("order", ["mixed", "one"])
 @pytest.mark.parametrize("f32", [False, True])
 @pytest.mark.parametrize("M,K,r", [(9, 128, 16), (150, 128, 16), (150, 128, 24), (260, 2048, 16)])
