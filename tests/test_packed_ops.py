@@ -758,6 +758,24 @@ def test_outputs_beside_inputs_in_one_buffer(B, word):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Lq", [1, 7, 140])
+@pytest.mark.parametrize("two_dims", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+def test_range_attention_shared_ranges_and_other_scales(Lq, two_dims, D, word):
+    """One range for all batch elements, given as [Lq] or [1, Lq]; scales other than the root's."""
+    B, Lk, H, Hkv = 3, 333, 6, 2
+    q, k, v = randn(B, Lq, H, D, seed=87), randn(B, Lk, Hkv, D, seed=88), randn(B, Lk, Hkv, D, seed=89)
+    lo, hi = random_ranges(1, Lq, Lk, 90)
+    pos = torch.randint(-20, Lk + 20, (1, Lq), dtype=torch.int32, device=DEV)
+    if not two_dims:
+        lo, hi, pos = lo[0], hi[0], pos[0]
+    for scale in (1e-3, 0.3):
+        check_attn(q, k, v, lo, hi, scale=scale)
+        check_attn(q, k, v, lo, hi, pos=pos, scale=scale, cap=4.0, slopes=torch.rand(H, device=DEV))
+        check_attn(q, k, v, lo, hi, pos=pos, scale=scale, table=torch.randn(H, 31, device=DEV))
+
+
+@pytest.mark.gpu
 def test_range_attention_empty_tensors_and_refusals(word):
     q, k = randn(2, 3, 4, 64), randn(2, 5, 2, 64)
     lo = hi = torch.zeros(3, dtype=torch.int32, device=DEV)
@@ -1000,6 +1018,26 @@ def test_lora_linear_fp32_epilogues_over_several_runs(M, N, K, tile_n, epi, brok
         spared[ids == 1] = False
         assert not bool(got[~spared].isfinite().all())
     within(got[spared], ref[spared], tol[spared])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("M,K,frames", [(10, 128, (100, 25, 30, 0)), (10, 128, (100, 25, 30, 5)), (300, 1024, (100, 25, 30, 120)),
+                                        (2600, 1024, (500, 50, 130, 0)), (700, 2048, (90, 7, 0, 350))])
+def test_lora_linear_gate_of_a_row_s_frame(M, K, frames, f32, word):
+    """Rows that start inside a sequence, and several sequences in the rows."""
+    N, n, r = 544, 3, 16
+    x, w, b, down, up, ids, scales = lora_case(M, K, N, n, r, 260)
+    seq, tokens, offset, per = frames
+    row = torch.arange(M, device=DEV)
+    frame = ((row % per if per else row) + offset) % seq // tokens
+    mod, e0 = randn(N, seed=41), torch.randn(-(-seq // tokens), N, device=DEV)
+    dt = torch.float32 if f32 else BF16
+    res = randn(M, N, seed=42).to(dt)
+    got = ops.lora_linear(x, w, b, down, up, ids, scales=scales, epilogue=L.EPI_BIAS_GATE_RES, residual=res, gate=(mod, e0),
+                          frames=frames, out=torch.empty(M, N, dtype=dt, device=DEV))
+    within(got, *lora_ref(x, w, b, down, up, ids, scales, L.EPI_BIAS_GATE_RES, residual=res, f32=f32,
+                          gate=(mod.double() + e0.double())[frame]))
 
 
 @pytest.mark.gpu

@@ -511,7 +511,8 @@ __device__ __forceinline__ void lora_store_sums(const GemmArgs& a, float* stg, f
   const float* gate_row = nullptr;
   if constexpr (GATE) {
     const int row = m0 + quad * 32 + lane;
-    gate_row = a.gate_e0 + (row < a.M ? frame_of_row(row, a.rows_per_seq, a.row_offset, a.seq_len, a.tokens_per_frame) : 0) * a.gate_frame_stride;
+    const int64_t f = row < a.M ? frame_of_row(row, a.rows_per_seq, a.row_offset, a.seq_len, a.tokens_per_frame) : 0;
+    gate_row = a.gate_e0 + f * a.gate_frame_stride;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
